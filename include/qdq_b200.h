@@ -370,6 +370,96 @@ int fp4_moe_mxf4(const void* a, int64_t lda, int dtype, const void* w_codes, con
                  int64_t size_m, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
                  void* stream);
 
+/* ---------------------------------------------------------------------------
+ * MXFP8 products (tcgen05 kind::mxf8f6f4) and the row operators in front of
+ * them.  They serve the float8_e4m3fn layers, whose activations the reference
+ * only quant-dequantises (vllm_qdq_plugin/patch.py:61-67, :150-152).
+ *
+ * MXFP8 rows: codes [M, K] E4M3 bytes (row stride ldc) and scales [M, lds]
+ * E8M0 bytes, row-major: K / 32 scales of a row, then zeros up to a multiple
+ * of 16.  lds >= qdq_mxfp8_scale_stride(K); base addresses and row strides of
+ * codes and scales are multiples of 16 bytes; K % 32 == 0.
+ * ------------------------------------------------------------------------- */
+
+/* K / 32 rounded up to a multiple of 16: the least lds of MXFP8 rows. */
+int64_t qdq_mxfp8_scale_stride(int64_t K);
+
+/* MXFP8 rows of x [M, K] bf16/fp16 (dtype): the codes and scales of
+ * qdq_mxfp8.  Rows of x 16-byte aligned, K % 32 == 0. */
+int qdq_mxfp8_rows(const void* x, void* codes, void* scales, int64_t M, int64_t K, int64_t ldx,
+                   int64_t ldc, int64_t lds, int dtype, void* stream);
+
+/* MXFP8 rows of y = silu(x[:, :K]) * x[:, K:2K], x [M, 2K] (row stride ldx),
+ * y computed in fp32 and rounded to the dtype of x before its quantisation. */
+int qdq_silu_mul_mxfp8(const void* x, void* codes, void* scales, int64_t M, int64_t K, int64_t ldx,
+                       int64_t ldc, int64_t lds, int dtype, void* stream);
+
+/*
+ * RMSNorm with the residual's addition and MXFP8 output:
+ *   h = round(x + residual)          (residual NULL: h = x, residual_out NULL)
+ *   y = round(h * rsqrt(mean(h^2) + eps) * weight)
+ * and the MXFP8 rows of y; sums and products in fp32, `round` to the dtype of
+ * x.  residual_out [M, K] (row stride ldh) receives h; y [M, K] (row stride ldy)
+ * is written unless NULL.  No output may overlap an input.  weight [K] of the same dtype.  All rows 16-byte aligned,
+ * K % 32 == 0, K <= QDQ_RMSNORM_MAX_K.
+ */
+#define QDQ_RMSNORM_MAX_K 65536
+int qdq_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight, void* residual_out,
+                      void* y, void* codes, void* scales, int64_t M, int64_t K, int64_t ldx, int64_t ldr,
+                      int64_t ldh, int64_t ldy, int64_t ldc, int64_t lds, float eps, int dtype,
+                      void* stream);
+
+/*
+ * C[M, N] (out_dtype bf16/fp16, row stride ldc elements) = A . W^T (+ bias[N],
+ * out_dtype), fp32 accumulation.  A: MXFP8 rows (codes row stride lda, scales
+ * row stride lds).  W: E4M3 codes [N, K] (row stride ldw bytes, 16-byte
+ * aligned) with E8M0 scales per 32 in the tiled layout of qdq_sf_tile (block
+ * 32, qdq_sf_tiled_bytes(N, K)).  K % 32 == 0.
+ * Stream order: launched with programmatic dependent launch; W and its scales
+ * may be read while the previous kernel on the stream finishes and must not be
+ * written by it.  Everything else keeps full stream order.
+ */
+int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t lda, int64_t lds, const void* w_codes,
+                  const void* w_sf_tiled, const void* bias, void* c, int64_t M, int64_t N, int64_t K,
+                  int64_t ldw, int64_t ldc, int out_dtype, void* stream);
+
+/* Workspace bytes of fp8_linear_mxf8: the activation's MXFP8 rows. */
+int64_t fp8_linear_workspace_bytes(int64_t M, int64_t K);
+
+/*
+ * The same for a 16-bit activation a [M, K] (dtype, row stride lda elements,
+ * 16-byte aligned rows), quantised as qdq_mxfp8_rows does; c and bias have its
+ * dtype.  workspace: 256-byte aligned, fp8_linear_workspace_bytes(M, K).
+ */
+int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void* w_codes, const void* w_sf_tiled,
+                    const void* bias, void* c, int64_t M, int64_t N, int64_t K, int64_t ldw, int64_t ldc,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Grouped MXFP8 MoE product, the MXFP8 counterpart of fp4_moe_mxf4 (same
+ * routing operands and meaning): for every block b < num_tokens_post_padded /
+ * moe_block_size with expert e = expert_ids[b] in [0, num_experts) and every
+ * slot s = sorted_token_ids[b * moe_block_size + i] in [0, size_m * top_k):
+ *   C[s, :] = A[s / top_k, :] . W_e^T   (x topk_weights[s] if mul_topk_weights)
+ * with fp32 accumulation; rows of C that no slot names are not written.
+ *   A: either a (16-bit, dtype, row stride lda; quantised as qdq_mxfp8_rows
+ *      does, into the workspace) or, with a == NULL, MXFP8 rows a_codes /
+ *      a_scales (strides ldac, lds)
+ *   w_codes [num_experts, N, K] E4M3, contiguous; w_sf_tiled: num_experts
+ *      blocks of qdq_sf_tiled_bytes(N, K) bytes
+ *   c [size_m * top_k, N] of dtype, row stride ldc
+ *   workspace: 256-byte aligned, fp8_moe_workspace_bytes(size_m, num_sorted,
+ *      moe_block_size, K); two calls in flight need one each
+ * moe_block_size in [1, 64]; K % 32 == 0.
+ */
+int64_t fp8_moe_workspace_bytes(int64_t size_m, int64_t num_sorted, int moe_block_size, int64_t K);
+int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, const void* a_scales, int64_t ldac,
+                 int64_t lds, int dtype, const void* w_codes, const void* w_sf_tiled, int64_t num_experts,
+                 const int32_t* sorted_token_ids, const int32_t* expert_ids,
+                 const int32_t* num_tokens_post_padded, const float* topk_weights, int64_t num_sorted,
+                 int moe_block_size, int top_k, int mul_topk_weights, void* c, int64_t ldc, int64_t size_m,
+                 int64_t N, int64_t K, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

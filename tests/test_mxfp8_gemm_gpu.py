@@ -1,0 +1,251 @@
+"""GPU: the dense and grouped MXFP8 products against float64 products of the same codes.
+
+Every product of two E4M3 values with E8M0 scales is exact in fp32, so the
+tolerance is half a step of the output type plus the fp32 accumulation bound
+of the FP4 GEMM tests (2^-16 of sum |a_k w_k|).
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mxfp8_cases import activation, check_moe, check_product, random_weight, routing, values
+
+pytestmark = pytest.mark.gpu
+
+
+def _ok():
+    from vllm_qdq_plugin import _native
+    assert _native.device_status() == 0
+
+
+def _rows_values(rows):
+    return values(rows.codes, rows.scales)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 32), (1, 4096, 4096), (2, 300, 96), (16, 512, 1024),
+                                   (17, 129, 544), (33, 640, 512), (64, 1024, 2080), (65, 200, 288), (100, 1001, 2880),
+                                   (128, 256, 256), (129, 257, 352), (192, 384, 512), (193, 384, 512),
+                                   (333, 768, 2048), (1000, 136, 160), (257, 2050, 4128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear_against_64_bits(cuda_device, m, n, k, dtype):
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    a = activation(m, k, dtype, m + n + k, cuda_device)
+    codes, scales = random_weight(n, k, seed=n, dev=cuda_device)
+    w = prepare_mxfp8_weight(codes, scales)
+    bias = torch.randn(n, device=cuda_device).to(dtype)
+    rows = mxfp8_rows(a)
+    exact_a, exact_w = _rows_values(rows), values(codes, scales)
+    for x in (a, rows):
+        out = mxfp8_linear(x, w)
+        assert out.dtype == dtype and out.shape == (m, n)
+        check_product(out, exact_a, exact_w, what=f"linear {m}x{n}x{k}")
+        check_product(mxfp8_linear(x, w, bias), exact_a, exact_w, bias, f"linear {m}x{n}x{k} + bias")
+    _ok()
+
+
+def test_linear_takes_strided_rows_and_its_weights_bias(cuda_device):
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import Mxfp8Rows, mxfp8_rows
+    m, n, k = 40, 200, 320
+    a = activation(m, k, torch.bfloat16, 1, cuda_device)
+    codes, scales = random_weight(n, k, seed=2, dev=cuda_device)
+    bias = torch.randn(n, device=cuda_device)
+    w = prepare_mxfp8_weight(codes.view(torch.float8_e4m3fn), scales, bias)
+    want = mxfp8_linear(a, w)
+    rows = mxfp8_rows(a)
+    check_product(want, _rows_values(rows), values(codes, scales), bias.to(torch.bfloat16))
+    wide = torch.cat([a, a], 1)[:, :k]
+    assert torch.equal(mxfp8_linear(wide, w), want)
+    assert torch.equal(mxfp8_linear(torch.nn.functional.pad(a, (3, 0))[:, 3:], w), want)
+    held = torch.full((m, k + 64), 0x7F, dtype=torch.uint8, device=cuda_device)  # NaN codes behind every row
+    held[:, :k] = rows.codes
+    stored = torch.full((m, rows.stored.shape[1] + 16), 0xFF, dtype=torch.uint8, device=cuda_device)
+    stored[:, : rows.stored.shape[1]] = rows.stored
+    view = Mxfp8Rows(held[:, :k], stored[:, : rows.stored.shape[1]], torch.bfloat16)
+    assert torch.equal(mxfp8_linear(view, w), want)
+    wpad = torch.full((n, k + 16), 0x7F, dtype=torch.uint8, device=cuda_device)
+    wpad[:, :k] = codes
+    assert torch.equal(mxfp8_linear(a, prepare_mxfp8_weight(wpad[:, :k], scales, bias)), want)
+    _ok()
+
+
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_linear_keeps_nan_and_infinite_rows_apart(cuda_device, m):
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    n, k = 160, 416
+    a = activation(m, k, torch.bfloat16, 9, cuda_device)
+    w = prepare_mxfp8_weight(*random_weight(n, k, seed=4, dev=cuda_device))
+    want = mxfp8_linear(a, w)
+    b = a.clone()
+    b[m // 2, 5] = float("nan")
+    got = mxfp8_linear(b, w)
+    others = torch.arange(m, device=cuda_device) != m // 2
+    assert torch.equal(got[others], want[others]) and got[m // 2].isnan().all()
+
+
+def test_linear_empty(cuda_device):
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    w = prepare_mxfp8_weight(*random_weight(96, 64, seed=4, dev=cuda_device))
+    a = torch.empty(0, 64, dtype=torch.bfloat16, device=cuda_device)
+    assert mxfp8_linear(a, w).shape == (0, 96) and mxfp8_linear(mxfp8_rows(a), w).shape == (0, 96)
+
+
+@pytest.mark.parametrize("m,e,top_k,bs,n,k,mul", [(1, 4, 1, 16, 128, 128, False),
+                                                  (1, 8, 4, 8, 200, 2880, True),
+                                                  (5, 4, 2, 16, 256, 512, False),
+                                                  (37, 8, 2, 16, 384, 1024, True),
+                                                  (64, 16, 4, 32, 201, 2080, True),
+                                                  (3, 4, 1, 64, 128, 288, False),
+                                                  (100, 8, 8, 8, 256, 512, True),
+                                                  (300, 6, 2, 64, 384, 1024, True),
+                                                  (2048, 4, 2, 8, 128, 256, False),
+                                                  (700, 2, 2, 64, 320, 544, True),
+                                                  (150, 4, 2, 48, 257, 512, False),
+                                                  (90, 5, 2, 1, 130, 96, True),
+                                                  (50, 3, 1, 13, 128, 320, False),
+                                                  (61, 128, 4, 16, 128, 256, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_against_64_bits(cuda_device, m, e, top_k, bs, n, k, mul, dtype):
+    """Every routed slot's row; one block per expert, long runs cut into segments, layouts whose runs cross the
+    segment scan's chunks, block sizes that do not divide a segment, 128 experts of which few are hit."""
+    from vllm_qdq_plugin.gemm import mxfp8_moe_linear, prepare_mxfp8_moe_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    a = activation(m, k, dtype, m + e + bs, cuda_device)
+    codes, scales = random_weight(e, n, k, seed=n + e, dev=cuda_device)
+    w = prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, top_k, bs, m + e, cuda_device)
+    rows = mxfp8_rows(a)
+    for x in (a, rows):
+        out = mxfp8_moe_linear(x, w, sid, eid, ntp, tw, bs, top_k, mul)
+        assert out.dtype == dtype and out.shape == (m * top_k, n)
+        check_moe(out, _rows_values(rows), codes, scales, ids, f"moe m={m} e={e} bs={bs}", tw if mul else None)
+    _ok()
+
+
+def test_moe_leaves_what_no_slot_names(cuda_device):
+    """Blocks of experts outside [0, E), blocks behind num_tokens_post_padded and slots that no block names keep
+    their rows; sentinels and stray slot numbers write nothing."""
+    from vllm_qdq_plugin.gemm import mxfp8_moe_linear, prepare_mxfp8_moe_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    m, e, top_k, bs, n, k = 40, 4, 2, 16, 136, 256
+    dev = cuda_device
+    a = activation(m, k, torch.bfloat16, 1, dev)
+    codes, scales = random_weight(e, n, k, seed=3, dev=dev)
+    w = prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, top_k, bs, 2, dev)
+    full = mxfp8_moe_linear(a, w, sid, eid, ntp, tw, bs, top_k, True)
+    eid2 = eid.clone()
+    eid2[0], eid2[-1] = -1, e
+    sid2 = torch.cat([sid, torch.arange(2 * bs, dtype=torch.int32, device=dev)])  # live-looking, behind the end
+    eid2 = torch.cat([eid2, torch.tensor([1, 2], dtype=torch.int32, device=dev)])
+    sid2[bs + 3] = -7
+    sid2[bs + 4] = m * top_k + 5
+    held = torch.full((m * top_k + 3, n + 8), 7.0, dtype=torch.bfloat16, device=dev)
+    out = held[: m * top_k, :n]
+    assert mxfp8_moe_linear(mxfp8_rows(a), w, sid2, eid2, ntp, tw, bs, top_k, True, out=out) is out
+    named = torch.zeros(m * top_k, dtype=torch.bool, device=dev)
+    live = sid2[: int(ntp)].view(-1, bs)[1:-1].reshape(-1)
+    named[live[(live >= 0) & (live < m * top_k)].long()] = True
+    assert 0 < int(named.sum()) < m * top_k
+    assert torch.equal(out[named], full[named]) and (out[~named] == 7.0).all()
+    assert (held[m * top_k:] == 7.0).all() and (held[:, n:] == 7.0).all()
+    ntp0 = torch.zeros_like(ntp)
+    out.fill_(7.0)
+    mxfp8_moe_linear(a, w, sid2, eid2, ntp0, tw, bs, top_k, False, out=out)
+    assert (out == 7.0).all()
+    _ok()
+
+
+@pytest.mark.parametrize("k", [288, 2880])
+def test_moe_result_independent_of_stale_workspace(cuda_device, k):
+    from vllm_qdq_plugin import _native
+    from vllm_qdq_plugin.gemm import prepare_mxfp8_moe_weight
+    m, e, top_k, bs, n = 40, 4, 2, 16, 256
+    dev = cuda_device
+    a = activation(m, k, torch.bfloat16, 5, dev)
+    w = prepare_mxfp8_moe_weight(*random_weight(e, n, k, seed=6, dev=dev))
+    _, sid, eid, ntp, tw = routing(m, e, top_k, bs, 7, dev)
+    lib, outs = _native.lib(), []
+    for fill in (0x00, 0xFF, 0x7F):
+        ws = torch.full((lib.fp8_moe_workspace_bytes(m, sid.numel(), bs, k),), fill, dtype=torch.uint8, device=dev)
+        out = torch.zeros((m * top_k, n), dtype=torch.bfloat16, device=dev)
+        _native.call("fp8_moe_mxf8", a.data_ptr(), k, None, None, 0, 0, 0, w.codes.data_ptr(), w.sf_tiled.data_ptr(), e,
+                     sid.data_ptr(), eid.data_ptr(), ntp.data_ptr(), tw.data_ptr(), sid.numel(), bs, top_k, 1,
+                     out.data_ptr(), n, m, n, k, ws.data_ptr(), ws.numel(), _native.stream_ptr(dev))
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0].isfinite().all()
+    _ok()
+
+
+def test_products_in_graphs_and_on_two_streams(cuda_device):
+    """Two captured graphs and eager calls on two streams, each call with a workspace of its own."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    dev, m, n, k, e, top_k, bs = cuda_device, 48, 256, 512, 4, 2, 16
+    a = activation(m, k, torch.bfloat16, 1, dev)
+    w = prepare_mxfp8_weight(*random_weight(n, k, seed=1, dev=dev))
+    wm = prepare_mxfp8_moe_weight(*random_weight(e, n, k, seed=2, dev=dev))
+    _, sid, eid, ntp, tw = routing(m, e, top_k, bs, 3, dev)
+
+    def both(x):
+        return mxfp8_linear(x, w), mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, bs, top_k, True)
+
+    want, want2 = both(a), both(a * 2)
+    graphs = []
+    b = a.clone()
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = both(b)
+        graphs.append((graph, out))
+    for x, ref in ((a, want), (a * 2, want2), (a, want)):
+        b.copy_(x)
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(g, r) for g, r in zip(out, ref))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    results = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            results.append(both(a))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, r) for out in results for g, r in zip(out, want))
+    _ok()
+
+
+@pytest.mark.parametrize("m,bs", [(1, 16), (23, 16), (400, 64)])
+def test_a_gated_expert_layer_stage_by_stage(cuda_device, m, bs):
+    """Norm -> router -> first grouped product -> gate -> second grouped product, as a layer runs them; every stage
+    is checked against 64 bits on what the stage before it really produced."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_quantize, mxfp8_rows, rmsnorm_mxfp8, silu_mul_mxfp8
+    from oracle import gemm as og
+    dev, hidden, inner, e, top_k = cuda_device, 320, 288, 6, 2
+    x, residual = (activation(m, hidden, torch.bfloat16, s, dev) for s in (1, 2))
+    weight = (1 + 0.1 * torch.randn(hidden, device=dev)).to(torch.bfloat16)
+    w_attn = random_weight(hidden, hidden, seed=3, dev=dev)
+    w13, w2 = random_weight(e, 2 * inner, hidden, seed=4, dev=dev), random_weight(e, hidden, inner, seed=5, dev=dev)
+    router = torch.randn(e, hidden, device=dev)
+
+    proj = mxfp8_linear(mxfp8_rows(x), prepare_mxfp8_weight(*w_attn))
+    check_product(proj, _rows_values(mxfp8_rows(x)), values(*w_attn), what="projection")
+    rows, h, y = rmsnorm_mxfp8(proj, weight, residual, norm_out=True)
+    assert torch.equal(h, (proj.float() + residual.float()).to(torch.bfloat16))
+    assert torch.equal(rows.codes, mxfp8_quantize(y)[0])
+    prob, ids = torch.softmax(y.float() @ router.t(), 1).topk(top_k, 1)
+    sid, eid, ntp = (torch.from_numpy(t).to(dev) for t in og.moe_align(ids.cpu().numpy(), e, bs))
+    up = mxfp8_moe_linear(rows, prepare_mxfp8_moe_weight(*w13), sid, eid, ntp, None, bs, top_k, False)
+    check_moe(up, _rows_values(rows), *w13, ids.cpu().numpy(), "first product")
+    act = silu_mul_mxfp8(up)
+    down = mxfp8_moe_linear(act, prepare_mxfp8_moe_weight(*w2), sid, eid, ntp, prob, bs, 1, True)  # a row a slot
+    check_moe(down, _rows_values(act), *w2, ids.reshape(-1, 1).cpu().numpy(), "second product", prob)
+    out = h + down.view(m, top_k, hidden).sum(1)
+    assert out.shape == (m, hidden) and out.isfinite().all()
+    _ok()

@@ -1,0 +1,647 @@
+// MXFP8 products on the sm_100a tensor cores (tcgen05 kind::mxf8f6f4):
+//   dense    C[m, n] = sum_k A[m, k] W[n, k] (+ bias[n])
+//   grouped  C[s, n] = sum_k A[s / top_k, k] W_e[n, k] (x topk_weights[s])
+//            for the slots s of the blocks of expert e
+// A and W are E4M3 codes with one E8M0 scale per 32 elements of K; fp32
+// accumulation, one rounding to the 16-bit output.
+//
+// The MMA's M side is 128 rows of W and its N side the activation rows
+// ("swap AB"), so that few activation rows make a narrow N instead of an
+// idle M, and a ragged segment of an expert's rows costs its own width.
+//
+// One CTA per SM walks work items (a segment of at most NT activation rows,
+// 128 rows of W); 12 warps:
+//   warp 0      TMA producer: W codes and scales of a K-128 stage, and the
+//               segment's codes: one box of NT consecutive rows (dense), or
+//               4-row gathers by token index (grouped), so that routed rows
+//               are never copied into sorted order
+//   warp 1      MMA issuer: per stage 4 MMAs (K = 32 each), M = 128,
+//               N = the segment's rows rounded up to 16
+//   warps 2-3   activation scales: a lane owns rows, loads 16 scales (four
+//               stages) of a row at once and writes each stage's four bytes
+//               into the chunk layout that tcgen05.cp expects
+//   warps 4-11  epilogue: TMEM lanes = W rows, columns = activation rows
+// What the kernel before it on the stream may have written (scales, routing,
+// segments) is read past L1 (__ldcg): under programmatic dependent launch this
+// kernel's CTAs start before that one has finished.
+// The stage ring runs across items and the accumulator is double-buffered in
+// TMEM, so an item's epilogue overlaps the next item's MMAs.
+#include <algorithm>
+#include <cstring>
+
+#include "mx_quant.cuh"
+#include "sm100.cuh"
+
+namespace qdqb200 {
+namespace {
+
+using namespace sm100;
+
+constexpr int TM = 128;              // W rows per item (UMMA M)
+constexpr int TK = 128;              // K elements (= bytes) per stage: one swizzle row
+constexpr int NT_MAX = 192;          // activation rows per item: two accumulators + scales fit 512 TMEM columns
+constexpr int T_W = TM * TK;         // 16 KB
+constexpr int T_STAGES_MAX = 12;
+constexpr int T_EPI = 8;             // epilogue warps
+constexpr int T_SCALE = 2;           // scale warps
+constexpr int T_THREADS = 32 * (2 + T_SCALE + T_EPI);
+constexpr uint32_t T_TMEM = 512, T_SFW = 2 * NT_MAX, T_SFA = T_SFW + 4;
+
+__host__ __device__ constexpr int t_stage_bytes(int nt) { return (T_W + nt * TK + 512 + 1024 + 1023) / 1024 * 1024; }
+
+struct __align__(8) TBars {
+  uint64_t full[T_STAGES_MAX];   // codes and W scales landed (1 arrival + tx), activation scales written (1 per scale warp)
+  uint64_t empty[T_STAGES_MAX];  // the stage's MMAs completed
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+constexpr int kSmemMax = 227 * 1024;
+__host__ __device__ constexpr int t_stages(int nt) {
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars))) / t_stage_bytes(nt);
+  return n < T_STAGES_MAX ? n : T_STAGES_MAX;
+}
+
+template <int kDtype>
+struct Out16 {
+  using T = __nv_bfloat16;
+  __device__ static float load(const T* p) { return __bfloat162float(*p); }
+  __device__ static T one(float a) { return __float2bfloat16_rn(a); }
+};
+template <>
+struct Out16<QDQ_DTYPE_FP16> {
+  using T = __half;
+  __device__ static float load(const T* p) { return __half2float(*p); }
+  __device__ static T one(float a) { return __float2half_rn(a); }
+};
+
+struct GemmArgs {
+  const uint8_t* sfw;          // tiled W scales
+  int64_t sf_per_expert;
+  const uint8_t* sfa;          // row-major activation scales
+  int64_t lds;
+  const void* bias;            // dense
+  void* c;
+  int64_t ldc;
+  const int32_t* seg_tab;      // grouped: [count, (first block, blocks) ...]
+  const int32_t* sorted_ids;
+  const int32_t* expert_ids;
+  const float* topk_w;         // nullptr: no scaling
+  int M, N, K, kchunks;        // M: dense rows, grouped slots (size_m * top_k)
+  int top_k, bs, num_blocks, num_experts;
+  int nt;                      // activation rows per item
+  int* status;
+};
+
+// Grouped loads of four rows of a [rows, K] byte matrix into four consecutive
+// 128-byte swizzled rows of shared memory.
+__device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* map, int32_t x, int32_t r0, int32_t r1,
+                                            int32_t r2, int32_t r3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+struct Item {
+  int row0;     // first activation row (dense) or first sorted position (grouped)
+  int rows;     // rows of the segment
+  int n_tile;
+  int expert;
+};
+
+// Work item i, decoded alike by every role; false: nothing to do (grouped
+// only: a malformed segment).  Dense: tiles of one W panel run side by side,
+// so the CTAs in flight share it in L2.  Grouped: segment-major, so that each
+// expert's W streams from HBM once while its rows stay in L2.
+template <bool kGrouped>
+__device__ __forceinline__ bool item_of(const GemmArgs& p, int i, int n_tiles, int num_m, Item& it) {
+  if (!kGrouped) {
+    it.n_tile = i / num_m;
+    it.row0 = (i - it.n_tile * num_m) * p.nt;
+    it.rows = min(p.nt, p.M - it.row0);
+    it.expert = 0;
+    return true;
+  }
+  const int seg = i / n_tiles;
+  it.n_tile = i - seg * n_tiles;
+  const int blk0 = __ldcg(p.seg_tab + 1 + 2 * seg), nb = __ldcg(p.seg_tab + 2 + 2 * seg);
+  if (blk0 < 0 || nb < 1 || blk0 + nb > p.num_blocks || nb * p.bs > p.nt) return false;
+  it.expert = __ldcg(p.expert_ids + blk0);
+  it.row0 = blk0 * p.bs;
+  it.rows = nb * p.bs;
+  return it.expert >= 0 && it.expert < p.num_experts;
+}
+
+// The activation row behind row r of an item.  Rows that stand for nothing
+// (padding slots, the fill up to a multiple of 16) read row 0: their columns
+// of the accumulator are dropped.
+template <bool kGrouped>
+__device__ __forceinline__ int token_of(const GemmArgs& p, const Item& it, int r) {
+  if (!kGrouped) return min(it.row0 + r, p.M - 1);
+  if (r >= it.rows) return 0;
+  const int s = __ldcg(p.sorted_ids + it.row0 + r);
+  return (s >= 0 && s < p.M) ? s / p.top_k : 0;
+}
+
+template <int kDtype, bool kGrouped>
+__global__ void __launch_bounds__(T_THREADS, 1)
+mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                 const __grid_constant__ GemmArgs p) {
+  using O = Out16<kDtype>;
+  using T = typename O::T;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int S = t_stages(p.nt), stage_bytes = t_stage_bytes(p.nt);
+  const int st_a = T_W, st_sfw = T_W + p.nt * TK, st_sfa = st_sfw + 512;
+  TBars* bars = reinterpret_cast<TBars*>(smem + S * stage_bytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_tiles = (p.N + TM - 1) / TM;
+  const int num_m = kGrouped ? 1 : (p.M + p.nt - 1) / p.nt;
+  const int num_kt = (p.K + TK - 1) / TK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bars->full[s], 1 + T_SCALE);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc_full[b], 1);
+      mbar_init(&bars->acc_empty[b], 32 * T_EPI);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_a);
+  }
+  if (warp == 0) {
+    tmem_alloc(&bars->tmem_base, T_TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t tmem = bars->tmem_base;
+  const int num_items = kGrouped ? min(max(__ldcg(p.seg_tab), 0), p.num_blocks) * n_tiles : num_m * n_tiles;
+
+  if (warp == 0) {
+    // ---------------- producer
+    int it = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+      Item w;
+      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+      const int w_row = w.expert * p.N + w.n_tile * TM;
+      const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
+      const int gathers = kGrouped ? (w.rows + 15) / 16 * 4 : 0;  // rows up to the MMA's N, four at a time
+      int tok[2][4];
+      if (kGrouped) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) tok[j][q] = token_of<true>(p, w, 4 * (lane + 32 * j) + q);
+      }
+      for (int kt = 0; kt < num_kt; ++kt, ++it) {
+        const int s = it % S;
+        ok = mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, p.status, 0x601);
+        ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+        if (!ok) break;
+        uint8_t* st = smem + s * stage_bytes;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars->full[s], T_W + 512 + (kGrouped ? gathers * 4 : p.nt) * TK);
+          tma_load_2d(st, &tmap_w, kt * TK, w_row, &bars->full[s]);
+          bulk_load(st + st_sfw, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
+          if (!kGrouped) tma_load_2d(st + st_a, &tmap_a, kt * TK, w.row0, &bars->full[s]);
+        }
+        if (kGrouped) {
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (lane + 32 * j < gathers)
+              tma_gather4(st + st_a + (lane + 32 * j) * 4 * TK, &tmap_a, kt * TK, tok[j][0], tok[j][1], tok[j][2],
+                          tok[j][3], &bars->full[s]);
+        }
+      }
+    }
+    if (!ok) bars->abort = 1;
+    // every issued copy has landed before the CTA may exit
+    for (int j = (it > S ? it - S : 0); j < it; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
+  } else if (warp == 1) {
+    // ---------------- MMA issuer
+    if (elect_one()) {
+      int it = 0, j = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+        Item w;
+        if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+        const int n_mma = (w.rows + 15) / 16 * 16;
+        const uint32_t idesc = idesc_mxf8(TM, n_mma);
+        const int buf = j & 1;
+        if (!mbar_wait(&bars->acc_empty[buf], ((j >> 1) & 1) ^ 1, p.status, 0x603)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t acc = tmem + NT_MAX * buf;
+        for (int kt = 0; kt < num_kt; ++kt, ++it) {
+          const int s = it % S;
+          if (!mbar_wait(&bars->full[s], (it / S) & 1, p.status, 0x604)) { ok = false; break; }
+          if (*(volatile int*)&bars->abort) { ok = false; break; }
+          tc_fence_after();
+          uint8_t* st = smem + s * stage_bytes;
+          tmem_cp_sf(tmem + T_SFW, smem_desc_sf(st + st_sfw));
+          tmem_cp_sf(tmem + T_SFA, smem_desc_sf(st + st_sfa));
+          if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, smem_desc_sf(st + st_sfa + 512));
+          const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + st_a);
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; ++kk)  // K step kk reads scale byte kk of each row's four
+            mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + T_SFW) | (kk << 30),
+                     (tmem + T_SFA) | (kk << 30), (kt | kk) != 0);
+          tc_commit(&bars->empty[s]);
+        }
+        if (!ok) break;
+        tc_commit(&bars->acc_full[buf]);
+        ++j;
+      }
+      if (!ok) bars->abort = 1;
+      tc_commit(&bars->drain);
+      mbar_wait(&bars->drain, 0, p.status, 0x605);
+    }
+  } else if (warp < 2 + T_SCALE) {
+    // ---------------- activation scales
+    constexpr int kLanes = 32 * T_SCALE, kR = NT_MAX / kLanes;  // rows per lane
+    const int t = threadIdx.x - 64;
+    int it = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+      Item w;
+      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+      const int n_mma = (w.rows + 15) / 16 * 16;
+      const uint8_t* src[kR];
+#pragma unroll
+      for (int j = 0; j < kR; ++j)
+        src[j] = p.sfa + static_cast<int64_t>(token_of<kGrouped>(p, w, t + kLanes * j)) * p.lds;
+      uint4 cur[kR], nxt[kR];
+#pragma unroll
+      for (int j = 0; j < kR; ++j)
+        if (t + kLanes * j < n_mma) nxt[j] = __ldcg(reinterpret_cast<const uint4*>(src[j]));
+      for (int kt = 0; kt < num_kt; ++kt, ++it) {
+        if ((kt & 3) == 0) {
+#pragma unroll
+          for (int j = 0; j < kR; ++j) {
+            cur[j] = nxt[j];
+            if (kt + 4 < num_kt && t + kLanes * j < n_mma)
+              nxt[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + (kt + 4) * 4));
+          }
+        }
+        const int s = it % S;
+        ok = mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, p.status, 0x606);
+        ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+        if (!ok) break;
+        uint8_t* sf = smem + s * stage_bytes + st_sfa;
+#pragma unroll
+        for (int j = 0; j < kR; ++j) {
+          const int r = t + kLanes * j;
+          if (r < n_mma)
+            *reinterpret_cast<uint32_t*>(sf + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4) = cur[j].x;
+          cur[j] = make_uint4(cur[j].y, cur[j].z, cur[j].w, 0u);  // the next stage's four
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->full[s]);
+      }
+    }
+    if (!ok) bars->abort = 1;
+  } else {
+    // ---------------- epilogue: warp reads TMEM lanes 32 (warp % 4).., column chunks half, half + 2, ...
+    const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
+    constexpr int kCh = (NT_MAX / 32 + 1) / 2;
+    T* C = static_cast<T*>(p.c);
+    bool ok = true;
+    int j = 0;
+    for (int i = blockIdx.x; i < num_items; i += gridDim.x) {
+      Item w;
+      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+      const int nchunks = (w.rows + 31) / 32;
+      // output rows of this warp's columns, fetched while the MMAs run: lane l holds that of column 32 c + l
+      int slot[kCh];
+      float wt[kCh];
+#pragma unroll
+      for (int u = 0; u < kCh; ++u) {
+        const int col = 32 * (half + 2 * u) + lane;
+        int s = -1;
+        if (col < w.rows) s = kGrouped ? __ldcg(p.sorted_ids + w.row0 + col) : w.row0 + col;
+        if (s >= p.M) s = -1;
+        slot[u] = s;
+        wt[u] = (kGrouped && p.topk_w != nullptr && s >= 0) ? __ldcg(p.topk_w + s) : 1.0f;
+      }
+      const int n = w.n_tile * TM + q * 32 + lane;
+      const bool in_n = n < p.N;
+      const float bias = (!kGrouped && p.bias != nullptr && in_n) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+      const int buf = j & 1;
+      if (ok) ok = mbar_wait(&bars->acc_full[buf], (j >> 1) & 1, p.status, 0x607);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + NT_MAX * buf;
+      const bool store = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+      if (half >= nchunks) {
+        tc_fence_before();
+        mbar_arrive(&bars->acc_empty[buf]);
+      }
+#pragma unroll
+      for (int u = 0; u < kCh; ++u) {
+        const int c = half + 2 * u;
+        if (c >= nchunks) break;
+        uint32_t r[32];
+        tmem_ld32(taddr + 32 * c, r);
+        tmem_ld_wait();
+        if (c + 2 >= nchunks) {  // this warp's last chunk of the item
+          tc_fence_before();
+          mbar_arrive(&bars->acc_empty[buf]);
+        }
+        if (!store) continue;
+#pragma unroll
+        for (int l = 0; l < 32; ++l) {
+          const int s = __shfl_sync(0xffffffffu, slot[u], l);
+          float v = __uint_as_float(r[l]);
+          if (kGrouped) v *= __shfl_sync(0xffffffffu, wt[u], l);
+          else v += bias;
+          if (s >= 0 && in_n) C[static_cast<int64_t>(s) * p.ldc + n] = O::one(v);
+        }
+      }
+      ++j;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, T_TMEM);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Segments of the grouped product: runs of consecutive live blocks that name
+// the same expert, cut into at most nbmax blocks.  One CTA; blocks are walked
+// in chunks of the CTA's size with carries, entries come out in order.
+// ---------------------------------------------------------------------------
+constexpr int SEG_THREADS = 1024;
+
+__device__ void build_segments(const int32_t* __restrict__ expert_ids, int live, int num_experts, int nbmax,
+                               int32_t* __restrict__ seg_tab) {
+  __shared__ int s_start[32], s_count[32];
+  const int t = threadIdx.x, lane = t & 31, wid = t >> 5, nw = blockDim.x >> 5;
+  int carry_start = -1, carry_count = 0;
+  for (int base = 0; base < live; base += blockDim.x) {
+    const int b = base + t;
+    const int e = b < live ? __ldg(expert_ids + b) : -1;
+    const bool valid = e >= 0 && e < num_experts;
+    const bool first = valid && (b == 0 || __ldg(expert_ids + b - 1) != e);
+    int start = first ? b : -1;  // the first block of b's run: a running maximum
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, start, o);
+      if (lane >= o) start = max(start, v);
+    }
+    if (lane == 31) s_start[wid] = start;
+    __syncthreads();
+    for (int w = 0; w < wid; ++w) start = max(start, s_start[w]);
+    start = max(start, carry_start);
+    int last = carry_start;
+    for (int w = 0; w < nw; ++w) last = max(last, s_start[w]);
+    const bool seg = valid && (b - start) % nbmax == 0;
+    const unsigned bal = __ballot_sync(0xffffffffu, seg);
+    if (lane == 0) s_count[wid] = __popc(bal);
+    __syncthreads();
+    int at = carry_count + __popc(bal & ((1u << lane) - 1u)), all = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < wid) at += s_count[w];
+      all += s_count[w];
+    }
+    if (seg) {
+      int nb = 1;
+      while (nb < nbmax && b + nb < live && __ldg(expert_ids + b + nb) == e) ++nb;
+      seg_tab[1 + 2 * at] = b;
+      seg_tab[2 + 2 * at] = nb;
+    }
+    carry_start = last;
+    carry_count += all;
+    __syncthreads();
+  }
+  if (t == 0) seg_tab[0] = carry_count;
+}
+
+__global__ void __launch_bounds__(SEG_THREADS)
+mxf8_segments_kernel(const int32_t* __restrict__ expert_ids, const int32_t* __restrict__ num_post_padded, int bs,
+                     int num_blocks, int num_experts, int nbmax, int32_t* __restrict__ seg_tab) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int npp = __ldg(num_post_padded);
+  const int live = npp <= 0 ? 0 : min(num_blocks, (npp - 1) / bs + 1);
+  build_segments(expert_ids, live, num_experts, nbmax, seg_tab);
+}
+
+int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+bool off(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+
+template <typename... P, typename... A>
+int launch_pdl(const char* who, void (*fn)(P...), int64_t grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...);
+  if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
+  return check_launch(who);
+}
+
+template <int kDtype, bool kGrouped>
+int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, const GemmArgs& p, int64_t items,
+                cudaStream_t s) {
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(&mxf8_gemm_kernel<kDtype, kGrouped>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
+    attr_set[dev] = true;
+  }
+  const size_t smem = 1024 + static_cast<size_t>(t_stages(p.nt)) * t_stage_bytes(p.nt) + sizeof(TBars);
+  return launch_pdl(who, &mxf8_gemm_kernel<kDtype, kGrouped>, std::min<int64_t>(items, device_sm_count()), T_THREADS,
+                    smem, s, tw, ta, p);
+}
+
+int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
+  if (dtype != QDQ_DTYPE_BF16 && dtype != QDQ_DTYPE_FP16)
+    return fail(QDQ_ERR_INVALID_ARG, "%s: dtype must be bf16 (0) or fp16 (1)", who);
+  if (M < 0 || N < 0 || K < 0) return fail(QDQ_ERR_INVALID_ARG, "%s: negative shape", who);
+  if (K % 32 != 0) return fail(QDQ_ERR_UNSUPPORTED, "%s: K=%lld must be a multiple of 32", who, (long long)K);
+  if (M >= (1ll << 30) || N >= (1ll << 30) || K >= (1ll << 30))
+    return fail(QDQ_ERR_UNSUPPORTED, "%s: dimension too large", who);
+  if (K == 0 && M > 0 && N > 0) return fail(QDQ_ERR_UNSUPPORTED, "%s: K == 0", who);
+  return QDQ_OK;
+}
+
+}  // namespace
+}  // namespace qdqb200
+
+using namespace qdqb200;
+
+extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t lda, int64_t lds,
+                             const void* w_codes, const void* w_sf_tiled, const void* bias, void* c, int64_t M,
+                             int64_t N, int64_t K, int64_t ldw, int64_t ldc, int out_dtype, void* stream) {
+  const char* who = "fp8_gemm_mxf8";
+  if (int st = check_product(who, out_dtype, M, N, K)) return st;
+  if (M == 0 || N == 0) return QDQ_OK;
+  if (!a_codes || !a_scales || !w_codes || !w_sf_tiled || !c) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (lda < K || ldw < K || ldc < N || lds < qdq_mxfp8_scale_stride(K))
+    return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
+  if (off(a_codes, 16) || lda % 16 || off(a_scales, 16) || lds % 16 || off(w_codes, 16) || ldw % 16 ||
+      off(w_sf_tiled, 16) || off(c, 2) || off(bias, 2))
+    return fail(QDQ_ERR_ALIGNMENT, "%s: codes and scales must be 16-byte aligned", who);
+  int* status = device_status_ptr();
+  if (status == nullptr) return QDQ_ERR_CUDA;
+  GemmArgs p = {};
+  p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
+  p.sfa = static_cast<const uint8_t*>(a_scales);
+  p.lds = lds;
+  p.bias = bias;
+  p.c = c;
+  p.ldc = ldc;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
+  p.top_k = 1;
+  p.nt = M >= NT_MAX ? NT_MAX : static_cast<int>((M + 15) / 16 * 16);
+  p.status = status;
+  CUtensorMap tw, ta;
+  if (int st = make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128)) return st;
+  if (int st = make_tmap_u8_2d(&ta, a_codes, M, K, lda, TK, p.nt, 128)) return st;
+  const int64_t items = ((M + p.nt - 1) / p.nt) * ((N + TM - 1) / TM);
+  if (items >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, p, items, s)
+                                     : launch_gemm<QDQ_DTYPE_BF16, false>(who, tw, ta, p, items, s);
+}
+
+extern "C" int64_t fp8_linear_workspace_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return up256(M * K) + up256(M * qdq_mxfp8_scale_stride(K));
+}
+
+extern "C" int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void* w_codes, const void* w_sf_tiled,
+                               const void* bias, void* c, int64_t M, int64_t N, int64_t K, int64_t ldw, int64_t ldc,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* who = "fp8_linear_mxf8";
+  if (int st = check_product(who, dtype, M, N, K)) return st;
+  if (M == 0 || N == 0) return QDQ_OK;
+  if (!a || !w_codes || !w_sf_tiled || !c) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (workspace == nullptr || off(workspace, 256) || workspace_bytes < fp8_linear_workspace_bytes(M, K))
+    return fail(QDQ_ERR_INVALID_ARG, "%s: workspace missing, unaligned or smaller than fp8_linear_workspace_bytes()",
+                who);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + up256(M * K);
+  const int64_t lds = qdq_mxfp8_scale_stride(K);
+  // K % 32 == 0, so the codes' rows are 16-byte aligned at stride K
+  if (int st = qdq_mxfp8_rows(a, codes, scales, M, K, lda, K, lds, dtype, stream)) return st;
+  return fp8_gemm_mxf8(codes, scales, K, lds, w_codes, w_sf_tiled, bias, c, M, N, K, ldw, ldc, dtype, stream);
+}
+
+extern "C" int64_t fp8_moe_workspace_bytes(int64_t size_m, int64_t num_sorted, int moe_block_size, int64_t K) {
+  if (size_m <= 0 || num_sorted <= 0 || moe_block_size <= 0 || K <= 0) return 0;
+  return up256(4 * (1 + 2 * (num_sorted / moe_block_size))) + up256(size_m * K) +
+         up256(size_m * qdq_mxfp8_scale_stride(K));
+}
+
+extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, const void* a_scales, int64_t ldac,
+                            int64_t lds, int dtype, const void* w_codes, const void* w_sf_tiled, int64_t num_experts,
+                            const int32_t* sorted_token_ids, const int32_t* expert_ids,
+                            const int32_t* num_tokens_post_padded, const float* topk_weights, int64_t num_sorted,
+                            int moe_block_size, int top_k, int mul_topk_weights, void* c, int64_t ldc,
+                            int64_t size_m, int64_t N, int64_t K, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  const char* who = "fp8_moe_mxf8";
+  if (int st = check_product(who, dtype, size_m, N, K)) return st;
+  if (num_sorted < 0 || num_experts < 0) return fail(QDQ_ERR_INVALID_ARG, "%s: negative size", who);
+  if (moe_block_size < 1 || moe_block_size > 64)
+    return fail(QDQ_ERR_UNSUPPORTED, "%s: moe_block_size must be in [1, 64] (got %d)", who, moe_block_size);
+  if (top_k < 1) return fail(QDQ_ERR_INVALID_ARG, "%s: top_k must be >= 1", who);
+  if (size_m == 0 || N == 0 || num_sorted == 0 || num_experts == 0) return QDQ_OK;
+  if ((!a && (!a_codes || !a_scales)) || !w_codes || !w_sf_tiled || !sorted_token_ids || !expert_ids ||
+      !num_tokens_post_padded || !c || (mul_topk_weights && !topk_weights))
+    return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if ((a ? lda < K : ldac < K || lds < qdq_mxfp8_scale_stride(K)) || ldc < N)
+    return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
+  if ((!a && (off(a_codes, 16) || ldac % 16 || off(a_scales, 16) || lds % 16)) || off(w_codes, 16) ||
+      off(w_sf_tiled, 16) || off(c, 2))
+    return fail(QDQ_ERR_ALIGNMENT, "%s: codes and scales must be 16-byte aligned", who);
+  if (num_experts >= (1ll << 31) / N || size_m >= (1ll << 30) / top_k || num_sorted >= (1ll << 30))
+    return fail(QDQ_ERR_UNSUPPORTED, "%s: too many rows", who);
+  if (workspace == nullptr || off(workspace, 256) ||
+      workspace_bytes < fp8_moe_workspace_bytes(size_m, num_sorted, moe_block_size, K))
+    return fail(QDQ_ERR_INVALID_ARG, "%s: workspace missing, unaligned or smaller than fp8_moe_workspace_bytes()", who);
+  const int64_t num_blocks = num_sorted / moe_block_size;
+  if (num_blocks == 0) return QDQ_OK;
+  const int64_t n_tiles = (N + TM - 1) / TM;
+  if (num_blocks * n_tiles >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  int* status = device_status_ptr();
+  if (status == nullptr) return QDQ_ERR_CUDA;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int32_t* seg_tab = static_cast<int32_t*>(workspace);
+  if (a) {
+    uint8_t* ws = static_cast<uint8_t*>(workspace) + up256(4 * (1 + 2 * num_blocks));
+    uint8_t* scales = ws + up256(size_m * K);
+    lds = qdq_mxfp8_scale_stride(K);
+    if (int st = qdq_mxfp8_rows(a, ws, scales, size_m, K, lda, K, lds, dtype, stream)) return st;
+    a_codes = ws;
+    a_scales = scales;
+    ldac = K;
+  }
+  GemmArgs p = {};
+  // Rows per item: the average expert's, rounded up to whole blocks, so that few rows leave the shared memory to
+  // more stages of W in flight; never less than a block.
+  const int64_t average = (num_sorted + num_experts - 1) / num_experts;
+  const int64_t rows = (average + moe_block_size - 1) / moe_block_size * moe_block_size;
+  p.nt = static_cast<int>((std::min<int64_t>(std::max<int64_t>(rows, moe_block_size), NT_MAX) + 15) / 16 * 16);
+  const int nbmax = p.nt / moe_block_size;
+  if (int st = launch_pdl(who, &mxf8_segments_kernel, 1, SEG_THREADS, 0, s, expert_ids, num_tokens_post_padded,
+                          moe_block_size, static_cast<int>(num_blocks), static_cast<int>(num_experts), nbmax, seg_tab))
+    return st;
+  p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
+  p.sf_per_expert = qdq_sf_tiled_bytes(N, K);
+  p.sfa = static_cast<const uint8_t*>(a_scales);
+  p.lds = lds;
+  p.c = c;
+  p.ldc = ldc;
+  p.seg_tab = seg_tab;
+  p.sorted_ids = sorted_token_ids;
+  p.expert_ids = expert_ids;
+  p.topk_w = mul_topk_weights ? topk_weights : nullptr;
+  p.M = static_cast<int>(size_m * top_k);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
+  p.top_k = top_k;
+  p.bs = moe_block_size;
+  p.num_blocks = static_cast<int>(num_blocks);
+  p.num_experts = static_cast<int>(num_experts);
+  p.status = status;
+  CUtensorMap tw, ta;
+  if (int st = make_tmap_u8_2d(&tw, w_codes, num_experts * N, K, K, TK, TM, 128)) return st;
+  if (int st = make_tmap_u8_2d(&ta, a_codes, size_m, K, ldac, TK, 1, 128)) return st;  // 4-row gathers: a box of one row
+  return dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, true>(who, tw, ta, p, num_blocks * n_tiles, s)
+                                 : launch_gemm<QDQ_DTYPE_BF16, true>(who, tw, ta, p, num_blocks * n_tiles, s);
+}

@@ -1,7 +1,8 @@
-// MXFP4 group quantisation shared by the QDQ kernels and the fused decode
-// GEMM: the reference's per-dtype exponent / scale rules
-// (vllm_qdq_plugin/qdq/mxfp4.py:98-156) and the E2M1 codes of one 32-element
-// group.  Everything here reproduces the reference bit for bit.
+// MX group quantisation shared by the QDQ kernels and the fused linears: the
+// reference's per-dtype exponent / scale rules and the codes of one group,
+// MXFP4 (vllm_qdq_plugin/qdq/mxfp4.py:98-156), NVFP4 and MXFP8
+// (vllm_qdq_plugin/qdq/mxfp8.py:73-125).  Everything here reproduces the
+// reference bit for bit.
 #pragma once
 
 #include "common.cuh"
@@ -205,6 +206,97 @@ __device__ __forceinline__ uint32_t nv_group_codes(const uint4 (&v)[2], float gs
     }
   }
   return g.sbyte;
+}
+
+// ---------------------------------------------------------------------------
+// MXFP8 group math (vllm_qdq_plugin/qdq/mxfp8.py:73-125), bit-exact
+// ---------------------------------------------------------------------------
+// Scale exponent 127 + floor(log2(max(amax, FLT_MIN))) - 8, clamped to
+// [0, 254] (mxfp8.py:104-112).  For a bf16/fp16 maximum, floor(log2) is the
+// fp32 exponent field (their mantissas are too short for log2 to round up to
+// the next integer); a zero or sub-FLT_MIN maximum sits at FLT_MIN (-126);
+// inf / NaN give 0, the x86 float->int32 cast of +-inf / NaN.
+template <int kDtype>
+__device__ __forceinline__ int mx8_exp(uint32_t amax_bits) {
+  const uint32_t b = __float_as_uint(Fmt<kDtype>::amax_value(amax_bits));
+  const int ef = static_cast<int>(b >> 23);
+  if (ef == 255) return 0;
+  return min(max((ef == 0 ? -126 : ef - 127) + 119, 0), 254);
+}
+__device__ __forceinline__ float pow2f(int e) {  // 2^e, e in [-127, 127]
+  return __uint_as_float(e > -127 ? static_cast<uint32_t>(e + 127) << 23 : 0x00400000u);
+}
+// The reference's E4M3 grid (mxfp8.py:40-70) is round-to-nearest-even with
+// saturation at 448, except that its subnormal branch is clamped to 7 * 2^-9
+// (:57): magnitudes in [7.5, 8) * 2^-9 give 7 * 2^-9 where RNE gives 2^-6.
+// Lowering [7, 8) * 2^-9 to 7 * 2^-9 before the hardware conversion
+// reproduces that.
+__device__ __forceinline__ float mx8_sub_clamp(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return ((u & 0x7FFFFFFFu) - 0x3C600000u < 0x00200000u) ? __uint_as_float((u & 0x80000000u) | 0x3C600000u) : v;
+}
+// Two values -> E4M3 pair (a in the low byte) and its exact fp16x2 decode.
+__device__ __forceinline__ uint32_t e4m3x2_roundtrip(float a, float b, uint32_t& h) {
+  uint32_t out;
+  asm("{\n\t.reg .b16 t;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 t, %3, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, t;\n\t"
+      "cvt.u32.u16 %0, t;\n\t}"
+      : "=r"(out), "=r"(h)
+      : "f"(a), "f"(b));
+  return out;
+}
+// The same two steps on an f16x2 pair of quotients: magnitudes in
+// [7, 8) * 2^-9 (fp16 0x2300 .. 0x23FF) lose their low mantissa bits, which
+// leaves 7 * 2^-9 with the sign; then E4M3 with the exact fp16x2 decode.  The
+// quotients of the fast path fit fp16 exactly: |x / scale| < 2^9, at most 11
+// significant bits, and those below 2^-14 (fp16 subnormals, rounded) are far
+// below 2^-10, where every E4M3 code is zero.
+__device__ __forceinline__ uint32_t mx8_pair_f16(uint32_t h, uint32_t& dec) {
+  uint32_t eq, out;
+  asm("{\n\t.reg .b32 m;\n\t"
+      "and.b32 m, %1, 0x7F007F00;\n\t"
+      "set.eq.u32.f16x2 %0, m, %2;\n\t}"
+      : "=r"(eq)
+      : "r"(h), "r"(0x23002300u));
+  h &= ~(eq & 0x00FF00FFu);
+  asm("{\n\t.reg .b16 t;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 t, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, t;\n\t"
+      "cvt.u32.u16 %0, t;\n\t}"
+      : "=r"(out), "=r"(dec)
+      : "r"(h));
+  return out;
+}
+// x / scale for a pair.  torch.sign makes a zero quotient +0 (mxfp8.py:46,
+// :70): with fma(x, inv, zero), zero = +0.0 a kernel argument, an exact -0
+// becomes +0.  That covers every zero quotient while no nonzero input can
+// underflow: inv >= 2^-16 (scale exponent <= 143), always so for fp16.
+// Above it, zero quotients are cleared by comparison.
+__device__ __forceinline__ float2 mx8_scaled(float a, float b, float inv, float zero, bool fast) {
+  if (fast) return fma_f32x2(make_float2(a, b), make_float2(inv, inv), make_float2(zero, zero));
+  float2 t = mul_f32x2(make_float2(a, b), make_float2(inv, inv));
+  if (t.x == 0.0f) t.x = 0.0f;
+  if (t.y == 0.0f) t.y = 0.0f;
+  return t;
+}
+
+// E4M3 codes of eight elements (one 16-byte chunk) of a 32-group with scale
+// exponent e: the codes mxfp8_vec_kernel emits for the same group.
+template <int kDtype>
+__device__ __forceinline__ uint2 mx8_chunk_codes(const uint4& v, int e, float zero) {
+  using F = Fmt<kDtype>;
+  const float inv = pow2f(127 - e);
+  const bool fast = e <= 143;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t p[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 t = mx8_scaled(F::lo(w[j]), F::hi(w[j]), inv, zero, fast);
+    uint32_t h;
+    p[j] = fast ? mx8_pair_f16(pack_f16x2(t.x, t.y), h) : e4m3x2_roundtrip(mx8_sub_clamp(t.x), mx8_sub_clamp(t.y), h);
+  }
+  return make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
 }
 
 }  // namespace

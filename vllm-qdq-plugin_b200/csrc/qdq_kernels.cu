@@ -418,78 +418,8 @@ amax_gs_small_kernel(const uint16_t* __restrict__ x, int M, int K, int64_t ldx, 
 
 // ---------------------------------------------------------------------------
 // MXFP8: E4M3 elements, E8M0 scale per 32 (vllm_qdq_plugin/qdq/mxfp8.py:73-125),
-// bit-exact.
+// bit-exact; the group rule is in mx_quant.cuh.
 // ---------------------------------------------------------------------------
-// Scale exponent 127 + floor(log2(max(amax, FLT_MIN))) - 8, clamped to
-// [0, 254] (mxfp8.py:104-112).  For a bf16/fp16 maximum, floor(log2) is the
-// fp32 exponent field (their mantissas are too short for log2 to round up to
-// the next integer); a zero or sub-FLT_MIN maximum sits at FLT_MIN (-126);
-// inf / NaN give 0, the x86 float->int32 cast of +-inf / NaN.
-template <int kDtype>
-__device__ __forceinline__ int mx8_exp(uint32_t amax_bits) {
-  const uint32_t b = __float_as_uint(Fmt<kDtype>::amax_value(amax_bits));
-  const int ef = static_cast<int>(b >> 23);
-  if (ef == 255) return 0;
-  return min(max((ef == 0 ? -126 : ef - 127) + 119, 0), 254);
-}
-__device__ __forceinline__ float pow2f(int e) {  // 2^e, e in [-127, 127]
-  return __uint_as_float(e > -127 ? static_cast<uint32_t>(e + 127) << 23 : 0x00400000u);
-}
-// The reference's E4M3 grid (mxfp8.py:40-70) is round-to-nearest-even with
-// saturation at 448, except that its subnormal branch is clamped to 7 * 2^-9
-// (:57): magnitudes in [7.5, 8) * 2^-9 give 7 * 2^-9 where RNE gives 2^-6.
-// Lowering [7, 8) * 2^-9 to 7 * 2^-9 before the hardware conversion
-// reproduces that.
-__device__ __forceinline__ float mx8_sub_clamp(float v) {
-  const uint32_t u = __float_as_uint(v);
-  return ((u & 0x7FFFFFFFu) - 0x3C600000u < 0x00200000u) ? __uint_as_float((u & 0x80000000u) | 0x3C600000u) : v;
-}
-// Two values -> E4M3 pair (a in the low byte) and its exact fp16x2 decode.
-__device__ __forceinline__ uint32_t e4m3x2_roundtrip(float a, float b, uint32_t& h) {
-  uint32_t out;
-  asm("{\n\t.reg .b16 t;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f32 t, %3, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, t;\n\t"
-      "cvt.u32.u16 %0, t;\n\t}"
-      : "=r"(out), "=r"(h)
-      : "f"(a), "f"(b));
-  return out;
-}
-// The same two steps on an f16x2 pair of quotients: magnitudes in
-// [7, 8) * 2^-9 (fp16 0x2300 .. 0x23FF) lose their low mantissa bits, which
-// leaves 7 * 2^-9 with the sign; then E4M3 with the exact fp16x2 decode.  The
-// quotients of the fast path fit fp16 exactly: |x / scale| < 2^9, at most 11
-// significant bits, and those below 2^-14 (fp16 subnormals, rounded) are far
-// below 2^-10, where every E4M3 code is zero.
-__device__ __forceinline__ uint32_t mx8_pair_f16(uint32_t h, uint32_t& dec) {
-  uint32_t eq, out;
-  asm("{\n\t.reg .b32 m;\n\t"
-      "and.b32 m, %1, 0x7F007F00;\n\t"
-      "set.eq.u32.f16x2 %0, m, %2;\n\t}"
-      : "=r"(eq)
-      : "r"(h), "r"(0x23002300u));
-  h &= ~(eq & 0x00FF00FFu);
-  asm("{\n\t.reg .b16 t;\n\t"
-      "cvt.rn.satfinite.e4m3x2.f16x2 t, %2;\n\t"
-      "cvt.rn.f16x2.e4m3x2 %1, t;\n\t"
-      "cvt.u32.u16 %0, t;\n\t}"
-      : "=r"(out), "=r"(dec)
-      : "r"(h));
-  return out;
-}
-// x / scale for a pair.  torch.sign makes a zero quotient +0 (mxfp8.py:46,
-// :70): with fma(x, inv, zero), zero = +0.0 a kernel argument, an exact -0
-// becomes +0.  That covers every zero quotient while no nonzero input can
-// underflow: inv >= 2^-16 (scale exponent <= 143), always so for fp16.
-// Above it, zero quotients are cleared by comparison.
-__device__ __forceinline__ float2 mx8_scaled(float a, float b, float inv, float zero, bool fast) {
-  if (fast) return fma_f32x2(make_float2(a, b), make_float2(inv, inv), make_float2(zero, zero));
-  float2 t = mul_f32x2(make_float2(a, b), make_float2(inv, inv));
-  if (t.x == 0.0f) t.x = 0.0f;
-  if (t.y == 0.0f) t.y = 0.0f;
-  return t;
-}
-
 template <int kDtype, bool kContig, bool kY, bool kCodes, bool kScales>
 __global__ void __launch_bounds__(kThreads)
 mxfp8_vec_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ y,

@@ -68,6 +68,20 @@ _SIGNATURES: dict[str, list] = {
                                 _i64, _i64, _i64, _i64, _i64, _c_void_p],
     "fp4_linear_mxf4": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64,
                         _i64, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p],
+    "qdq_mxfp8_scale_stride": [_i64],
+    "qdq_mxfp8_rows": [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _int, _c_void_p],
+    "qdq_silu_mul_mxfp8": [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _int, _c_void_p],
+    "qdq_rmsnorm_mxfp8": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                          _i64, _i64, _i64, _i64, _i64, _i64, _f32, _int, _c_void_p],
+    "fp8_gemm_mxf8": [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64,
+                      _i64, _i64, _i64, _int, _c_void_p],
+    "fp8_linear_workspace_bytes": [_i64, _i64],
+    "fp8_linear_mxf8": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64,
+                        _i64, _c_void_p, _i64, _c_void_p],
+    "fp8_moe_workspace_bytes": [_i64, _i64, _int, _i64],
+    "fp8_moe_mxf8": [_c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64, _int, _c_void_p, _c_void_p, _i64, _c_void_p,
+                     _c_void_p, _c_void_p, _c_void_p, _i64, _int, _int, _int, _c_void_p, _i64, _i64, _i64, _i64,
+                     _c_void_p, _i64, _c_void_p],
 }
 _RESTYPES = {"qdq_last_error": ctypes.c_char_p, "qdq_sf_tiled_bytes": ctypes.c_int64,
              "fp4_linear_workspace_bytes": ctypes.c_int64,
@@ -76,7 +90,10 @@ _RESTYPES = {"qdq_last_error": ctypes.c_char_p, "qdq_sf_tiled_bytes": ctypes.c_i
              "fp4_linear_noalloc_scratch_bytes": ctypes.c_int64,
              "sage3_attn_workspace_bytes": ctypes.c_int64,
              "fp4_moe_workspace_bytes": ctypes.c_int64,
-             "qdq_host_stream_staging_bytes": ctypes.c_int64}
+             "qdq_host_stream_staging_bytes": ctypes.c_int64,
+             "qdq_mxfp8_scale_stride": ctypes.c_int64,
+             "fp8_linear_workspace_bytes": ctypes.c_int64,
+             "fp8_moe_workspace_bytes": ctypes.c_int64}
 
 
 def lib() -> ctypes.CDLL:
@@ -137,6 +154,39 @@ def require_cuda(*tensors: torch.Tensor) -> None:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+class on_device:
+    """Context in which the C ABI launches on `device`: makes it the current
+    device for the call where it is not already."""
+
+    __slots__ = ("_index", "_previous")
+
+    def __init__(self, device: torch.device):
+        self._index = device.index
+
+    def __enter__(self):
+        current = torch.cuda.current_device()
+        self._previous = None if current == self._index else current
+        if self._previous is not None:
+            torch.cuda.set_device(self._index)
+
+    def __exit__(self, *exc):
+        if self._previous is not None:
+            torch.cuda.set_device(self._previous)
+
+
+def same_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise RuntimeError(f"expected every tensor on {device}, got one on {t.device}")
+
+
+def rows16(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it whose rows start on 16-byte boundaries with unit element stride."""
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[0] <= 1 or x.stride(0) * x.element_size() % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

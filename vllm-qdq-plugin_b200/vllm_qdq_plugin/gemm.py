@@ -28,6 +28,7 @@ import torch
 from . import _native
 from ._log import init_logger
 from .qdq.mxfp4 import mxfp4_quantize
+from .qdq.mxfp8_rows import Mxfp8Rows, scale_stride
 
 logger = init_logger(__name__)
 
@@ -425,3 +426,209 @@ def capture_moe_weights() -> bool:
         mu.prepare_moe_mxfp4_layer_for_marlin = prepare_moe_mxfp4_layer_for_marlin
     logger.warning("vllm-qdq-plugin: capturing raw MXFP4 MoE weights for the grouped FP4 GEMM")
     return True
+
+
+# ---------------------------------------------------------------------------
+# MXFP8 linear and grouped MoE product (E4M3 + E8M0 per 32), kind::mxf8f6f4
+# ---------------------------------------------------------------------------
+@dataclasses.dataclass
+class Mxfp8Weight:
+    """An MXFP8 weight [N, K] in the layout the tcgen05 product reads."""
+
+    codes: torch.Tensor     # uint8 [N, K] E4M3
+    sf_tiled: torch.Tensor  # uint8, tiled E8M0 scales (qdq_sf_tile, block 32)
+    n: int
+    k: int
+    bias: torch.Tensor | None = None
+
+
+@dataclasses.dataclass
+class Mxfp8MoeWeight:
+    """MXFP8 expert weights [E, N, K] in the layout the grouped product reads."""
+
+    codes: torch.Tensor     # uint8 [E, N, K] E4M3
+    sf_tiled: torch.Tensor  # uint8 [E * qdq_sf_tiled_bytes(N, K)], per-expert tiled E8M0 scales
+    e: int
+    n: int
+    k: int
+
+
+def _check_mxfp8_weight(codes: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
+    _native.require_cuda(codes, scales)
+    _native.same_device(codes.device, scales)
+    assert codes.element_size() == 1 and scales.element_size() == 1, (codes.dtype, scales.dtype)
+    assert codes.dim() == dims and codes.shape[-1] > 0 and codes.shape[-1] % 32 == 0, tuple(codes.shape)
+    assert tuple(scales.shape) == (*codes.shape[:-1], codes.shape[-1] // 32), (codes.shape, scales.shape)
+
+
+def prepare_mxfp8_weight(codes: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None) -> Mxfp8Weight:
+    """codes [N, K] E4M3 (uint8 or float8_e4m3fn), scales [N, K/32] E8M0 (uint8), as `mxfp8_quantize` returns them."""
+    _check_mxfp8_weight(codes, scales, 2)
+    codes = _native.rows16(codes.view(torch.uint8))
+    scales = scales.view(torch.uint8).contiguous()
+    n, k = codes.shape
+    with _native.on_device(codes.device):
+        sf = _tile_scales(scales, n, k)
+    return Mxfp8Weight(codes=codes, sf_tiled=sf, n=n, k=k, bias=bias)
+
+
+def prepare_mxfp8_moe_weight(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp8MoeWeight:
+    """codes [E, N, K] E4M3 (uint8 or float8_e4m3fn), scales [E, N, K/32] E8M0 (uint8)."""
+    _check_mxfp8_weight(codes, scales, 3)
+    codes = codes.view(torch.uint8).contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    scales = scales.view(torch.uint8).contiguous()
+    e, n, k = codes.shape
+    per = _native.lib().qdq_sf_tiled_bytes(n, k)
+    sf = torch.empty((e * per,), dtype=torch.uint8, device=codes.device)
+    with _native.on_device(codes.device):
+        stream = _native.stream_ptr(codes.device)
+        for i in range(e if n else 0):
+            _native.call("qdq_sf_tile", scales[i].data_ptr(), sf[i * per:].data_ptr(), n, k, k // 32, 32, stream)
+    return Mxfp8MoeWeight(codes=codes, sf_tiled=sf, e=e, n=n, k=k)
+
+
+_LIB = torch.library.Library("qdq_b200", "FRAGMENT")
+_LIB.define("mxfp8_linear(Tensor a, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias) -> Tensor")
+_LIB.define("mxfp8_linear_rows(Tensor codes, Tensor scales, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias, "
+            "bool out_fp16) -> Tensor")
+_LIB.define("mxfp8_moe_linear(Tensor a, Tensor? a_scales, Tensor w_codes, Tensor w_sf_tiled, Tensor sorted_token_ids, "
+            "Tensor expert_ids, Tensor num_tokens_post_padded, Tensor? topk_weights, int moe_block_size, int top_k, "
+            "Tensor(a!) out) -> ()")
+
+
+def _mxfp8_linear_op(a, w_codes, w_sf_tiled, bias):
+    a = _native.rows16(a)
+    m, k = a.shape
+    n = w_codes.shape[0]
+    ws = torch.empty((_native.lib().fp8_linear_workspace_bytes(m, k),), dtype=torch.uint8, device=a.device)
+    out = torch.empty((m, n), dtype=a.dtype, device=a.device)
+    with _native.on_device(a.device):
+        _native.call("fp8_linear_mxf8", a.data_ptr(), a.stride(0) if m > 1 else k, _native.DTYPE_CODE[a.dtype],
+                     w_codes.data_ptr(), w_sf_tiled.data_ptr(), _native.ptr(bias), out.data_ptr(), m, n, k,
+                     w_codes.stride(0) if n > 1 else k, n, ws.data_ptr(), ws.numel(), _native.stream_ptr(a.device))
+    return out
+
+
+def _mxfp8_linear_rows_op(codes, scales, w_codes, w_sf_tiled, bias, out_fp16):
+    m, k = codes.shape
+    n = w_codes.shape[0]
+    out = torch.empty((m, n), dtype=torch.float16 if out_fp16 else torch.bfloat16, device=codes.device)
+    with _native.on_device(codes.device):
+        _native.call("fp8_gemm_mxf8", codes.data_ptr(), scales.data_ptr(), codes.stride(0) if m > 1 else k,
+                     scales.stride(0) if m > 1 else scales.shape[1], w_codes.data_ptr(), w_sf_tiled.data_ptr(),
+                     _native.ptr(bias), out.data_ptr(), m, n, k, w_codes.stride(0) if n > 1 else k, n,
+                     int(out_fp16), _native.stream_ptr(codes.device))
+    return out
+
+
+def _mxfp8_moe_linear_op(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded,
+                         topk_weights, moe_block_size, top_k, out):
+    m, k = a.shape
+    e, n, _ = w_codes.shape
+    num_sorted = sorted_token_ids.numel()
+    ws = torch.empty((_native.lib().fp8_moe_workspace_bytes(m, num_sorted, moe_block_size, k),), dtype=torch.uint8,
+                     device=a.device)
+    if a_scales is None:
+        a = _native.rows16(a)
+        raw, lda, codes, scales, ldac, lds = a.data_ptr(), a.stride(0) if m > 1 else k, None, None, 0, 0
+    else:
+        raw, lda, codes, scales = None, 0, a.data_ptr(), a_scales.data_ptr()
+        ldac, lds = a.stride(0) if m > 1 else k, a_scales.stride(0) if m > 1 else a_scales.shape[1]
+    with _native.on_device(a.device):
+        _native.call("fp8_moe_mxf8", raw, lda, codes, scales, ldac, lds, _native.DTYPE_CODE[out.dtype],
+                     w_codes.data_ptr(), w_sf_tiled.data_ptr(), e, sorted_token_ids.data_ptr(), expert_ids.data_ptr(),
+                     num_tokens_post_padded.data_ptr(), _native.ptr(topk_weights), num_sorted, moe_block_size, top_k,
+                     int(topk_weights is not None), out.data_ptr(), out.stride(0) if out.shape[0] > 1 else n, m, n, k,
+                     ws.data_ptr(), ws.numel(), _native.stream_ptr(a.device))
+
+
+_LIB.impl("mxfp8_linear", _mxfp8_linear_op, "CUDA")
+_LIB.impl("mxfp8_linear_rows", _mxfp8_linear_rows_op, "CUDA")
+_LIB.impl("mxfp8_moe_linear", _mxfp8_moe_linear_op, "CUDA")
+
+
+@torch.library.register_fake("qdq_b200::mxfp8_linear")
+def _(a, w_codes, w_sf_tiled, bias):
+    return a.new_empty((a.shape[0], w_codes.shape[0]))
+
+
+@torch.library.register_fake("qdq_b200::mxfp8_linear_rows")
+def _(codes, scales, w_codes, w_sf_tiled, bias, out_fp16):
+    return codes.new_empty((codes.shape[0], w_codes.shape[0]), dtype=torch.float16 if out_fp16 else torch.bfloat16)
+
+
+@torch.library.register_fake("qdq_b200::mxfp8_moe_linear")
+def _(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded, topk_weights,
+      moe_block_size, top_k, out):
+    return None
+
+
+def _check_mxfp8_rows(name: str, a: torch.Tensor | Mxfp8Rows, k: int) -> None:
+    if isinstance(a, Mxfp8Rows):
+        _native.require_cuda(a.codes, a.stored)
+        m = a.codes.shape[0]
+        assert a.codes.dim() == 2 and a.codes.dtype == torch.uint8 and a.stored.dtype == torch.uint8 and (
+            tuple(a.stored.shape) == (m, scale_stride(a.codes.shape[1]))), f"{name}: malformed MXFP8 rows"
+        assert a.codes.stride(1) == 1 and a.stored.stride(1) == 1, f"{name}: MXFP8 rows must be dense along K"
+        _native.same_device(a.codes.device, a.stored)
+    else:
+        assert a.dim() == 2 and a.dtype in (torch.bfloat16, torch.float16), (
+            f"{name}: the activation must be 2-D bf16/fp16 or MXFP8 rows")
+        _native.require_cuda(a)
+    assert a.shape[1] == k, (tuple(a.shape), k)
+
+
+def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """out[M, N] = mxfp8(a) @ dequant(weight)^T (+ bias), fp32 accumulation.
+
+    a: [M, K] bf16/fp16 CUDA tensor (quantised as mxfp8_qdq does) or the MXFP8
+    rows that a norm or gate before it left.  Output dtype = a.dtype.  The
+    product equals that of the dequantised operands up to fp32 summation order.
+    """
+    _check_mxfp8_rows("mxfp8_linear", a, weight.k)
+    if bias is None:
+        bias = weight.bias
+    if bias is not None:
+        assert bias.dim() == 1 and bias.shape[0] == weight.n, (tuple(bias.shape), weight.n)
+        bias = bias.to(a.dtype).contiguous()
+    _native.same_device(a.device, weight.codes, bias)
+    if isinstance(a, Mxfp8Rows):
+        return torch.ops.qdq_b200.mxfp8_linear_rows(a.codes, a.stored, weight.codes, weight.sf_tiled, bias,
+                                                    a.dtype == torch.float16)
+    return torch.ops.qdq_b200.mxfp8_linear(a, weight.codes, weight.sf_tiled, bias)
+
+
+def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted_token_ids: torch.Tensor,
+                     expert_ids: torch.Tensor, num_tokens_post_padded: torch.Tensor,
+                     topk_weights: torch.Tensor | None, moe_block_size: int, top_k: int, mul_topk_weights: bool,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The grouped product of `mxfp4_moe_linear` in MXFP8: for every routed slot s (vLLM's
+    moe_align_block_size layout)
+    out[s] = mxfp8(a[s // top_k]) @ dequant(W[expert of s's block])^T (x topk_weights[s]).
+
+    a: [M, K] bf16/fp16, or MXFP8 rows; out: [M * top_k, N] of a's dtype (allocated when None; rows of
+    slots that are not routed keep their contents).  moe_block_size in [1, 64]."""
+    _check_mxfp8_rows("mxfp8_moe_linear", a, weight.k)
+    slots = a.shape[0] * top_k
+    assert top_k >= 1 and 1 <= moe_block_size <= 64, (top_k, moe_block_size)
+    for t in (sorted_token_ids, expert_ids, num_tokens_post_padded):
+        assert t.dtype == torch.int32 and t.is_contiguous(), "routing tensors are dense int32"
+    assert num_tokens_post_padded.numel() >= 1
+    assert expert_ids.numel() >= sorted_token_ids.numel() // moe_block_size, "expert_ids: one entry per block"
+    tw = None
+    if mul_topk_weights:
+        assert topk_weights is not None and topk_weights.numel() == slots, "topk_weights: one per slot"
+        tw = topk_weights.reshape(-1).float().contiguous()
+    if out is None:
+        out = torch.empty((slots, weight.n), dtype=a.dtype, device=a.device)
+    else:
+        assert tuple(out.shape) == (slots, weight.n) and out.dtype == a.dtype and (weight.n <= 1 or out.stride(1) == 1), (
+            "out must be [M * top_k, N] of the activation's dtype with dense rows")
+    _native.same_device(a.device, weight.codes, sorted_token_ids, expert_ids, num_tokens_post_padded, tw, out)
+    rows = isinstance(a, Mxfp8Rows)
+    torch.ops.qdq_b200.mxfp8_moe_linear(a.codes if rows else a, a.stored if rows else None, weight.codes,
+                                        weight.sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded, tw,
+                                        moe_block_size, top_k, out)
+    return out

@@ -1,0 +1,213 @@
+# SPDX-License-Identifier: Apache-2.0
+"""MXFP8 rows: activations held as E4M3 codes with E8M0 scales, and the
+operators that end in them.
+
+`mxfp8_qdq` returns the values that MXFP8 leaves of an activation; these
+return the codes and scales themselves, for `gemm.mxfp8_linear` and
+`gemm.mxfp8_moe_linear` to multiply.  The codes are those of `mxfp8_qdq` (and
+so of the reference, src/vllm_qdq_plugin/qdq/mxfp8.py:73-125) on the 16-bit
+tensor that the unfused operator would have stored.  One HBM pass each
+(`qdq_mxfp8_rows`, `qdq_rmsnorm_mxfp8`, `qdq_silu_mul_mxfp8` in
+include/qdq_b200.h).
+"""
+
+from __future__ import annotations
+
+import dataclasses
+
+import torch
+
+from .. import _native
+
+RMSNORM_MAX_K = 65536  # QDQ_RMSNORM_MAX_K of include/qdq_b200.h
+_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def scale_stride(k: int) -> int:
+    """Scales per stored row: K / 32 rounded up to a multiple of 16."""
+    return (k + 511) // 512 * 16
+
+
+@dataclasses.dataclass(slots=True)
+class Mxfp8Rows:
+    """Rows of MXFP8: element (m, k) stands for E4M3(codes[m, k]) * 2^(scales[m, k // 32] - 127).
+
+    `stored` holds the scales as the products read them: rows padded with
+    zeros to `scale_stride(K)` bytes.  `dtype` is the 16-bit type of the tensor
+    the rows were made from, and of a product's output.
+    """
+
+    codes: torch.Tensor    # uint8 [M, K] E4M3
+    stored: torch.Tensor   # uint8 [M, scale_stride(K)] E8M0
+    dtype: torch.dtype
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def scales(self) -> torch.Tensor:
+        """E8M0 scales [M, K / 32] (a view)."""
+        n = self.codes.shape[1] // 32
+        return self.stored if self.stored.shape[1] == n else self.stored[:, :n]
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> "Mxfp8Rows":
+        """From codes uint8 [M, K] and scales uint8 [M, K / 32], as `mxfp8_quantize` returns them (K % 32 == 0)."""
+        _native.require_cuda(codes, scales)
+        _native.same_device(codes.device, scales)
+        assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8, (codes.dtype, scales.dtype)
+        assert dtype in _DTYPES, f"MXFP8 rows stand for fp16/bf16 tensors, but got {dtype}"
+        assert codes.dim() == 2 and codes.shape[1] > 0 and codes.shape[1] % 32 == 0, tuple(codes.shape)
+        m, k = codes.shape
+        assert tuple(scales.shape) == (m, k // 32), (tuple(codes.shape), tuple(scales.shape))
+        stored = torch.zeros((m, scale_stride(k)), dtype=torch.uint8, device=codes.device)
+        stored[:, : k // 32] = scales
+        return cls(_native.rows16(codes), stored, dtype)
+
+    def dequantize(self) -> torch.Tensor:
+        """The values in `dtype`: what `mxfp8_qdq` returns for the same tensor."""
+        m, k = self.codes.shape
+        scale = torch.exp2(self.scales.float() - 127)
+        v = self.codes.view(torch.float8_e4m3fn).float().view(m, k // 32, 32) * scale.unsqueeze(-1)
+        return v.view(m, k).to(self.dtype)
+
+
+# These ops sit on the path of single tokens, where the host's time is the call's time: they are
+# registered with torch.library directly, which dispatches in half the time of a custom_op.
+_LIB = torch.library.Library("qdq_b200", "FRAGMENT")
+_LIB.define("mxfp8_rows(Tensor x) -> (Tensor, Tensor)")
+_LIB.define("silu_mul_mxfp8(Tensor x) -> (Tensor, Tensor)")
+_LIB.define("rmsnorm_mxfp8(Tensor x, Tensor weight, Tensor? residual, float eps, bool norm_out) -> Tensor[]")
+
+
+def _new_rows(x: torch.Tensor, m: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    return (torch.empty((m, k), dtype=torch.uint8, device=x.device),
+            torch.empty((m, scale_stride(k)), dtype=torch.uint8, device=x.device))
+
+
+def _rows_op(fn: str, x: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
+    x = _native.rows16(x)
+    m = x.shape[0]
+    codes, scales = _new_rows(x, m, k)
+    with _native.on_device(x.device):
+        _native.call(fn, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k,
+                     x.stride(0) if m > 1 else x.shape[1], k, scales.shape[1], _native.DTYPE_CODE[x.dtype],
+                     _native.stream_ptr(x.device))
+    return codes, scales
+
+
+def _mxfp8_rows_op(x):
+    return _rows_op("qdq_mxfp8_rows", x, x.shape[1])
+
+
+def _silu_mul_mxfp8_op(x):
+    return _rows_op("qdq_silu_mul_mxfp8", x, x.shape[1] // 2)
+
+
+def _rmsnorm_mxfp8_op(x, weight, residual, eps, norm_out):
+    x = _native.rows16(x)
+    m, k = x.shape
+    if weight.data_ptr() % 16:
+        weight = weight.clone()
+    codes, scales = _new_rows(x, m, k)
+    out = [codes, scales]
+    ldx = x.stride(0) if m > 1 else k
+    h = y = None
+    ldr = k
+    if residual is not None:
+        residual = _native.rows16(residual)
+        ldr = residual.stride(0) if m > 1 else k
+        h = torch.empty((m, k), dtype=x.dtype, device=x.device)
+        out.append(h)
+    if norm_out:
+        y = torch.empty((m, k), dtype=x.dtype, device=x.device)
+        out.append(y)
+    with _native.on_device(x.device):
+        _native.call("qdq_rmsnorm_mxfp8", x.data_ptr(), _native.ptr(residual), weight.data_ptr(), _native.ptr(h),
+                     _native.ptr(y), codes.data_ptr(), scales.data_ptr(), m, k, ldx, ldr, k, k, k, scales.shape[1],
+                     eps, _native.DTYPE_CODE[x.dtype], _native.stream_ptr(x.device))
+    return out
+
+
+_LIB.impl("mxfp8_rows", _mxfp8_rows_op, "CUDA")
+_LIB.impl("silu_mul_mxfp8", _silu_mul_mxfp8_op, "CUDA")
+_LIB.impl("rmsnorm_mxfp8", _rmsnorm_mxfp8_op, "CUDA")
+
+
+@torch.library.register_fake("qdq_b200::mxfp8_rows")
+def _(x):
+    return _new_rows(x, x.shape[0], x.shape[1])
+
+
+@torch.library.register_fake("qdq_b200::silu_mul_mxfp8")
+def _(x):
+    return _new_rows(x, x.shape[0], x.shape[1] // 2)
+
+
+@torch.library.register_fake("qdq_b200::rmsnorm_mxfp8")
+def _(x, weight, residual, eps, norm_out):
+    more = int(residual is not None) + int(norm_out)
+    return [*_new_rows(x, *x.shape), *(x.new_empty(x.shape) for _ in range(more))]
+
+
+def _check(name: str, x: torch.Tensor, k: int) -> None:
+    assert x.dim() == 2, f"{name} only supports 2D tensors, but got {x.dim()}D"
+    assert x.dtype in _DTYPES, f"{name} only supports fp16/bf16 tensors, but got {x.dtype}"
+    assert k > 0 and k % 32 == 0, f"{name}: K={k} must be a positive multiple of 32"
+    _native.require_cuda(x)
+
+
+def mxfp8_rows(x: torch.Tensor) -> Mxfp8Rows:
+    """MXFP8 rows of x [M, K] bf16/fp16 (CUDA, K % 32 == 0): the codes and scales of `mxfp8_quantize`."""
+    _check("mxfp8_rows", x, x.shape[-1])
+    return Mxfp8Rows(*torch.ops.qdq_b200.mxfp8_rows(x), x.dtype)
+
+
+def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
+    """MXFP8 rows [M, K] of silu(x[:, :K]) * x[:, K:], the gated activation between a layer's two products.
+
+    Args:
+        x: [M, 2K] bf16/fp16 (CUDA, K % 32 == 0), gate first.
+
+    The product is formed in fp32 and rounded to x's dtype before it is quantised.
+    """
+    k = x.shape[-1] // 2
+    _check("silu_mul_mxfp8", x, k)
+    assert x.shape[1] == 2 * k, f"silu_mul_mxfp8: {x.shape[1]} columns are not two halves"
+    return Mxfp8Rows(*torch.ops.qdq_b200.silu_mul_mxfp8(x), x.dtype)
+
+
+def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                  norm_out: bool = False) -> tuple[Mxfp8Rows, torch.Tensor | None, torch.Tensor | None]:
+    """RMSNorm in front of an MXFP8 product, with the residual's addition.
+
+        h = x + residual              (rounded to x's dtype; h = x without a residual)
+        y = h * rsqrt(mean(h^2) + eps) * weight     (fp32, rounded to x's dtype)
+
+    Args:
+        x: [M, K] bf16/fp16 (CUDA), K a multiple of 32 up to 65536.
+        weight: [K] of x's dtype.
+        residual: [M, K] of x's dtype, or None.
+        eps: added to the mean square; not negative.
+        norm_out: also return y, e.g. for a router that reads it in 16 bits.
+
+    Returns:
+        (MXFP8 rows of y, h or None without a residual, y or None).
+    """
+    _check("rmsnorm_mxfp8", x, x.shape[-1])
+    k = x.shape[1]
+    assert k <= RMSNORM_MAX_K, f"rmsnorm_mxfp8: K={k} is above {RMSNORM_MAX_K}"
+    assert weight.dim() == 1 and weight.shape[0] == k and weight.dtype == x.dtype and weight.stride(0) == 1, (
+        f"rmsnorm_mxfp8: weight must be a dense [{k}] tensor of {x.dtype}")
+    assert residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), (
+        "rmsnorm_mxfp8: residual must have x's shape and dtype")
+    assert eps >= 0, f"rmsnorm_mxfp8: eps={eps} must not be negative"
+    _native.same_device(x.device, weight, residual)
+    out = torch.ops.qdq_b200.rmsnorm_mxfp8(x, weight, residual, eps, norm_out)
+    return (Mxfp8Rows(out[0], out[1], x.dtype), out[2] if residual is not None else None,
+            out[-1] if norm_out else None)
