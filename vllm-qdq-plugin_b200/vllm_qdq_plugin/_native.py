@@ -115,6 +115,20 @@ def lib() -> ctypes.CDLL:
     return _LIB
 
 
+_OPS_LOADED = False
+
+
+def load_ops() -> None:
+    """Load (building first if missing or stale) the torch.library kernels of csrc/torch_ops.cpp."""
+    global _OPS_LOADED
+    if not _OPS_LOADED:
+        lib()
+        with _LOCK:
+            if not _OPS_LOADED:
+                torch.ops.load_library(str(_build.TORCH_OPS_PATH))
+                _OPS_LOADED = True
+
+
 def library_path() -> str:
     return str(_build.LIB_PATH)
 

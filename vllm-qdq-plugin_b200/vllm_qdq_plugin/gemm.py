@@ -489,6 +489,7 @@ def prepare_mxfp8_moe_weight(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp8
     return Mxfp8MoeWeight(codes=codes, sf_tiled=sf, e=e, n=n, k=k)
 
 
+# The CUDA kernels of these schemas are csrc/torch_ops.cpp, loaded by the first call.
 _LIB = torch.library.Library("qdq_b200", "FRAGMENT")
 _LIB.define("mxfp8_linear(Tensor a, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias) -> Tensor")
 _LIB.define("mxfp8_linear_rows(Tensor codes, Tensor scales, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias, "
@@ -498,55 +499,9 @@ _LIB.define("mxfp8_moe_linear(Tensor a, Tensor? a_scales, Tensor w_codes, Tensor
             "Tensor(a!) out) -> ()")
 
 
-def _mxfp8_linear_op(a, w_codes, w_sf_tiled, bias):
-    a = _native.rows16(a)
-    m, k = a.shape
-    n = w_codes.shape[0]
-    ws = torch.empty((_native.lib().fp8_linear_workspace_bytes(m, k),), dtype=torch.uint8, device=a.device)
-    out = torch.empty((m, n), dtype=a.dtype, device=a.device)
-    with _native.on_device(a.device):
-        _native.call("fp8_linear_mxf8", a.data_ptr(), a.stride(0) if m > 1 else k, _native.DTYPE_CODE[a.dtype],
-                     w_codes.data_ptr(), w_sf_tiled.data_ptr(), _native.ptr(bias), out.data_ptr(), m, n, k,
-                     w_codes.stride(0) if n > 1 else k, n, ws.data_ptr(), ws.numel(), _native.stream_ptr(a.device))
-    return out
-
-
-def _mxfp8_linear_rows_op(codes, scales, w_codes, w_sf_tiled, bias, out_fp16):
-    m, k = codes.shape
-    n = w_codes.shape[0]
-    out = torch.empty((m, n), dtype=torch.float16 if out_fp16 else torch.bfloat16, device=codes.device)
-    with _native.on_device(codes.device):
-        _native.call("fp8_gemm_mxf8", codes.data_ptr(), scales.data_ptr(), codes.stride(0) if m > 1 else k,
-                     scales.stride(0) if m > 1 else scales.shape[1], w_codes.data_ptr(), w_sf_tiled.data_ptr(),
-                     _native.ptr(bias), out.data_ptr(), m, n, k, w_codes.stride(0) if n > 1 else k, n,
-                     int(out_fp16), _native.stream_ptr(codes.device))
-    return out
-
-
-def _mxfp8_moe_linear_op(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded,
-                         topk_weights, moe_block_size, top_k, out):
-    m, k = a.shape
-    e, n, _ = w_codes.shape
-    num_sorted = sorted_token_ids.numel()
-    ws = torch.empty((_native.lib().fp8_moe_workspace_bytes(m, num_sorted, moe_block_size, k),), dtype=torch.uint8,
-                     device=a.device)
-    if a_scales is None:
-        a = _native.rows16(a)
-        raw, lda, codes, scales, ldac, lds = a.data_ptr(), a.stride(0) if m > 1 else k, None, None, 0, 0
-    else:
-        raw, lda, codes, scales = None, 0, a.data_ptr(), a_scales.data_ptr()
-        ldac, lds = a.stride(0) if m > 1 else k, a_scales.stride(0) if m > 1 else a_scales.shape[1]
-    with _native.on_device(a.device):
-        _native.call("fp8_moe_mxf8", raw, lda, codes, scales, ldac, lds, _native.DTYPE_CODE[out.dtype],
-                     w_codes.data_ptr(), w_sf_tiled.data_ptr(), e, sorted_token_ids.data_ptr(), expert_ids.data_ptr(),
-                     num_tokens_post_padded.data_ptr(), _native.ptr(topk_weights), num_sorted, moe_block_size, top_k,
-                     int(topk_weights is not None), out.data_ptr(), out.stride(0) if out.shape[0] > 1 else n, m, n, k,
-                     ws.data_ptr(), ws.numel(), _native.stream_ptr(a.device))
-
-
-_LIB.impl("mxfp8_linear", _mxfp8_linear_op, "CUDA")
-_LIB.impl("mxfp8_linear_rows", _mxfp8_linear_rows_op, "CUDA")
-_LIB.impl("mxfp8_moe_linear", _mxfp8_moe_linear_op, "CUDA")
+_mxfp8_linear_op = torch.ops.qdq_b200.mxfp8_linear.default
+_mxfp8_linear_rows_op = torch.ops.qdq_b200.mxfp8_linear_rows.default
+_mxfp8_moe_linear_op = torch.ops.qdq_b200.mxfp8_moe_linear.default
 
 
 @torch.library.register_fake("qdq_b200::mxfp8_linear")
@@ -578,6 +533,7 @@ def _check_mxfp8_rows(name: str, a: torch.Tensor | Mxfp8Rows, k: int) -> None:
             f"{name}: the activation must be 2-D bf16/fp16 or MXFP8 rows")
         _native.require_cuda(a)
     assert a.shape[1] == k, (tuple(a.shape), k)
+    _native.load_ops()
 
 
 def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -595,9 +551,8 @@ def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.T
         bias = bias.to(a.dtype).contiguous()
     _native.same_device(a.device, weight.codes, bias)
     if isinstance(a, Mxfp8Rows):
-        return torch.ops.qdq_b200.mxfp8_linear_rows(a.codes, a.stored, weight.codes, weight.sf_tiled, bias,
-                                                    a.dtype == torch.float16)
-    return torch.ops.qdq_b200.mxfp8_linear(a, weight.codes, weight.sf_tiled, bias)
+        return _mxfp8_linear_rows_op(a.codes, a.stored, weight.codes, weight.sf_tiled, bias, a.dtype == torch.float16)
+    return _mxfp8_linear_op(a, weight.codes, weight.sf_tiled, bias)
 
 
 def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted_token_ids: torch.Tensor,
@@ -628,7 +583,6 @@ def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted
             "out must be [M * top_k, N] of the activation's dtype with dense rows")
     _native.same_device(a.device, weight.codes, sorted_token_ids, expert_ids, num_tokens_post_padded, tw, out)
     rows = isinstance(a, Mxfp8Rows)
-    torch.ops.qdq_b200.mxfp8_moe_linear(a.codes if rows else a, a.stored if rows else None, weight.codes,
-                                        weight.sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded, tw,
-                                        moe_block_size, top_k, out)
+    _mxfp8_moe_linear_op(a.codes if rows else a, a.stored if rows else None, weight.codes, weight.sf_tiled,
+                         sorted_token_ids, expert_ids, num_tokens_post_padded, tw, moe_block_size, top_k, out)
     return out

@@ -77,66 +77,18 @@ class Mxfp8Rows:
         return v.view(m, k).to(self.dtype)
 
 
-# These ops sit on the path of single tokens, where the host's time is the call's time: they are
-# registered with torch.library directly, which dispatches in half the time of a custom_op.
+# The CUDA kernels of these schemas are csrc/torch_ops.cpp, loaded by the first call.
 _LIB = torch.library.Library("qdq_b200", "FRAGMENT")
 _LIB.define("mxfp8_rows(Tensor x) -> (Tensor, Tensor)")
 _LIB.define("silu_mul_mxfp8(Tensor x) -> (Tensor, Tensor)")
 _LIB.define("rmsnorm_mxfp8(Tensor x, Tensor weight, Tensor? residual, float eps, bool norm_out) -> Tensor[]")
+_rows_op = torch.ops.qdq_b200.mxfp8_rows.default
+_silu_mul_op = torch.ops.qdq_b200.silu_mul_mxfp8.default
+_rmsnorm_op = torch.ops.qdq_b200.rmsnorm_mxfp8.default
 
 
 def _new_rows(x: torch.Tensor, m: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return (torch.empty((m, k), dtype=torch.uint8, device=x.device),
-            torch.empty((m, scale_stride(k)), dtype=torch.uint8, device=x.device))
-
-
-def _rows_op(fn: str, x: torch.Tensor, k: int) -> tuple[torch.Tensor, torch.Tensor]:
-    x = _native.rows16(x)
-    m = x.shape[0]
-    codes, scales = _new_rows(x, m, k)
-    with _native.on_device(x.device):
-        _native.call(fn, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), m, k,
-                     x.stride(0) if m > 1 else x.shape[1], k, scales.shape[1], _native.DTYPE_CODE[x.dtype],
-                     _native.stream_ptr(x.device))
-    return codes, scales
-
-
-def _mxfp8_rows_op(x):
-    return _rows_op("qdq_mxfp8_rows", x, x.shape[1])
-
-
-def _silu_mul_mxfp8_op(x):
-    return _rows_op("qdq_silu_mul_mxfp8", x, x.shape[1] // 2)
-
-
-def _rmsnorm_mxfp8_op(x, weight, residual, eps, norm_out):
-    x = _native.rows16(x)
-    m, k = x.shape
-    if weight.data_ptr() % 16:
-        weight = weight.clone()
-    codes, scales = _new_rows(x, m, k)
-    out = [codes, scales]
-    ldx = x.stride(0) if m > 1 else k
-    h = y = None
-    ldr = k
-    if residual is not None:
-        residual = _native.rows16(residual)
-        ldr = residual.stride(0) if m > 1 else k
-        h = torch.empty((m, k), dtype=x.dtype, device=x.device)
-        out.append(h)
-    if norm_out:
-        y = torch.empty((m, k), dtype=x.dtype, device=x.device)
-        out.append(y)
-    with _native.on_device(x.device):
-        _native.call("qdq_rmsnorm_mxfp8", x.data_ptr(), _native.ptr(residual), weight.data_ptr(), _native.ptr(h),
-                     _native.ptr(y), codes.data_ptr(), scales.data_ptr(), m, k, ldx, ldr, k, k, k, scales.shape[1],
-                     eps, _native.DTYPE_CODE[x.dtype], _native.stream_ptr(x.device))
-    return out
-
-
-_LIB.impl("mxfp8_rows", _mxfp8_rows_op, "CUDA")
-_LIB.impl("silu_mul_mxfp8", _silu_mul_mxfp8_op, "CUDA")
-_LIB.impl("rmsnorm_mxfp8", _rmsnorm_mxfp8_op, "CUDA")
+    return x.new_empty((m, k), dtype=torch.uint8), x.new_empty((m, scale_stride(k)), dtype=torch.uint8)
 
 
 @torch.library.register_fake("qdq_b200::mxfp8_rows")
@@ -160,12 +112,13 @@ def _check(name: str, x: torch.Tensor, k: int) -> None:
     assert x.dtype in _DTYPES, f"{name} only supports fp16/bf16 tensors, but got {x.dtype}"
     assert k > 0 and k % 32 == 0, f"{name}: K={k} must be a positive multiple of 32"
     _native.require_cuda(x)
+    _native.load_ops()
 
 
 def mxfp8_rows(x: torch.Tensor) -> Mxfp8Rows:
     """MXFP8 rows of x [M, K] bf16/fp16 (CUDA, K % 32 == 0): the codes and scales of `mxfp8_quantize`."""
     _check("mxfp8_rows", x, x.shape[-1])
-    return Mxfp8Rows(*torch.ops.qdq_b200.mxfp8_rows(x), x.dtype)
+    return Mxfp8Rows(*_rows_op(x), x.dtype)
 
 
 def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
@@ -179,7 +132,7 @@ def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
     k = x.shape[-1] // 2
     _check("silu_mul_mxfp8", x, k)
     assert x.shape[1] == 2 * k, f"silu_mul_mxfp8: {x.shape[1]} columns are not two halves"
-    return Mxfp8Rows(*torch.ops.qdq_b200.silu_mul_mxfp8(x), x.dtype)
+    return Mxfp8Rows(*_silu_mul_op(x), x.dtype)
 
 
 def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -208,6 +161,6 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
         "rmsnorm_mxfp8: residual must have x's shape and dtype")
     assert eps >= 0, f"rmsnorm_mxfp8: eps={eps} must not be negative"
     _native.same_device(x.device, weight, residual)
-    out = torch.ops.qdq_b200.rmsnorm_mxfp8(x, weight, residual, eps, norm_out)
+    out = _rmsnorm_op(x, weight, residual, eps, norm_out)
     return (Mxfp8Rows(out[0], out[1], x.dtype), out[2] if residual is not None else None,
             out[-1] if norm_out else None)
