@@ -385,6 +385,291 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------
+// Few rows (a decode step): one launch, bound by the bytes of W.
+//
+// A cluster of `split` CTAs owns 128 rows of W and one set of at most 64
+// activation rows (dense: all of them; grouped: one block of one expert); its
+// CTAs take equal ranges of K, so that a narrow W still streams through most
+// SMs.  A CTA keeps its range of the activation resident in shared memory, as
+// swizzled codes and scale chunks made from 16-bit rows (kRaw, quantised here
+// with the rule of qdq_mxfp8) or copied from MXFP8 rows, while W comes through
+// a TMA ring that starts before the previous kernel on the stream has ended.
+// The partial sums meet in distributed shared memory: each CTA adds the
+// cluster's partials of its share of the W rows, always in rank order.
+//
+//   warp 0      TMA producer (W codes and scales)
+//   warp 1      MMA issuer (M = 128, N = n_pad, K = 32)
+//   warps 2-9   activation fill in passes of 256 groups, one barrier a pass,
+//               then the epilogue
+// ---------------------------------------------------------------------------
+constexpr int F_FILL = 256;
+constexpr int F_THREADS = 64 + F_FILL;
+constexpr int F_RING_MAX = 13, F_PASS_MAX = 16;
+constexpr int F_ROWS_MAX = 64;
+constexpr int F_ACT_MAX = 96 * 1024;      // resident activation bytes of a CTA
+constexpr uint32_t F_TMEM = 128, F_SFW = 64, F_SFA = 68;
+
+struct __align__(8) FBars {
+  uint64_t full[F_RING_MAX];
+  uint64_t empty[F_RING_MAX];
+  uint64_t ready[F_PASS_MAX];  // the pass's groups are in shared memory
+  uint64_t acc_full;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct FewArgs {
+  const void* a;               // 16-bit rows (kRaw) or codes
+  int64_t lda;                 // elements / bytes
+  const uint8_t* sfa;
+  int64_t lds;
+  const uint8_t* sfw;
+  int64_t sf_per_expert;
+  const void* bias;
+  void* c;
+  int64_t ldc;
+  const int32_t* sorted_ids;
+  const int32_t* expert_ids;
+  const int32_t* num_post_padded;
+  const float* topk_w;
+  int M, N, K, kchunks;        // M: dense rows, grouped slots
+  int rows, n_pad;             // rows of an item (dense M, grouped block size), rounded up to 16
+  int top_k, num_experts;
+  int split, kt_per, ring;     // CTAs of a cluster, K-128 stages per CTA, W stages in the ring
+  float zero;
+  int* status;
+};
+
+__host__ __device__ constexpr int f_act_bytes(int n_pad, int kt_per) { return kt_per * (n_pad * TK + 512); }
+
+template <int kDtype, bool kGrouped, bool kRaw>
+__global__ void __launch_bounds__(F_THREADS, 1)
+mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ FewArgs p) {
+  using O = Out16<kDtype>;
+  using T = typename O::T;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // W ring (also the partial sums once the MMAs are done) | activation codes | W scales | activation scales | barriers
+  uint8_t* s_act = smem + p.ring * T_W;
+  uint8_t* s_sfw = s_act + p.kt_per * p.n_pad * TK;
+  uint8_t* s_sfa = s_sfw + p.ring * 512;
+  FBars* bars = reinterpret_cast<FBars*>(s_sfa + p.kt_per * 512);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.split;
+  const int item = static_cast<int>(blockIdx.x) / p.split;
+  const int n_tiles = (p.N + TM - 1) / TM;
+  const int blk = kGrouped ? item / n_tiles : 0;
+  const int n_tile = item - blk * n_tiles;
+  const int num_kt = (p.K + TK - 1) / TK;
+  const int kt0 = rank * p.kt_per, nkt = max(0, min(p.kt_per, num_kt - kt0));
+
+  pdl_launch_dependents();
+  int expert = 0;
+  if (kGrouped) {
+    pdl_wait();  // the routing may come from the kernel before
+    expert = __ldcg(p.expert_ids + blk);
+    // the whole cluster shares the block, so it leaves as one
+    if (static_cast<int64_t>(blk) * p.rows >= __ldcg(p.num_post_padded) || expert < 0 || expert >= p.num_experts) return;
+  }
+  const int w_row = expert * p.N + n_tile * TM;
+  const uint8_t* sfw = p.sfw + expert * p.sf_per_expert + (static_cast<int64_t>(n_tile) * p.kchunks + kt0) * 512;
+  auto issue = [&](int kt) {
+    const int s = kt % p.ring;
+    mbar_arrive_expect_tx(&bars->full[s], T_W + 512);
+    tma_load_2d(smem + s * T_W, &tmap_w, (kt0 + kt) * TK, w_row, &bars->full[s]);
+    bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
+  };
+  const int pre = min(p.ring, nkt);
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int i = 0; i < F_PASS_MAX; ++i) mbar_init(&bars->ready[i], F_FILL);
+    mbar_init(&bars->acc_full, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+    for (int kt = 0; kt < pre; ++kt) issue(kt);  // W needs nothing that the previous kernel writes
+  }
+  if (warp == 1) {
+    tmem_alloc(&bars->tmem_base, F_TMEM);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == 0) {
+    // ---------------- producer
+    if (elect_one()) {
+      int issued = pre;
+      for (int kt = pre; kt < nkt; ++kt) {
+        if (!mbar_wait(&bars->empty[kt % p.ring], ((kt / p.ring) & 1) ^ 1, p.status, 0x701)) {
+          bars->abort = 1;
+          break;
+        }
+        if (*(volatile int*)&bars->abort) break;
+        issue(kt);
+        ++issued;
+      }
+      for (int kt = max(0, issued - p.ring); kt < issued; ++kt)
+        mbar_wait(&bars->full[kt % p.ring], (kt / p.ring) & 1, p.status, 0x702);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer
+    if (elect_one()) {
+      const uint32_t idesc = idesc_mxf8(TM, p.n_pad);
+      bool ok = true;
+      int passes = 0;  // passes seen complete
+      for (int kt = 0; kt < nkt; ++kt) {
+        const int need = ((kt + 1) * 4 * p.rows + F_FILL - 1) / F_FILL;
+        for (; ok && passes < need; ++passes) ok = mbar_wait(&bars->ready[passes], 0, p.status, 0x703);
+        const int s = kt % p.ring;
+        if (ok) ok = mbar_wait(&bars->full[s], (kt / p.ring) & 1, p.status, 0x704);
+        if (!ok || *(volatile int*)&bars->abort) { ok = false; break; }
+        tc_fence_after();
+        tmem_cp_sf(tmem + F_SFW, smem_desc_sf(s_sfw + s * 512));
+        tmem_cp_sf(tmem + F_SFA, smem_desc_sf(s_sfa + kt * 512));
+        const uint64_t dw = smem_desc_sw128(smem + s * T_W), da = smem_desc_sw128(s_act + kt * p.n_pad * TK);
+#pragma unroll
+        for (uint32_t kk = 0; kk < 4; ++kk)
+          mma_mxf8(tmem, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + F_SFW) | (kk << 30),
+                   (tmem + F_SFA) | (kk << 30), (kt | kk) != 0);
+        tc_commit(&bars->empty[s]);
+      }
+      if (!ok) bars->abort = 1;
+      tc_commit(&bars->acc_full);  // also on abort: the epilogue waits for the issued MMAs
+    }
+  } else {
+    // ---------------- activation fill: group g of row r of stage kt, four neighbouring lanes a stage's row
+    if (!kGrouped) pdl_wait();
+    const int t = threadIdx.x - 64;
+    const int groups = nkt * 4 * p.rows, passes = (groups + F_FILL - 1) / F_FILL;
+    uint4 v[4];
+    uint32_t sb = 0;
+    int kt = 0, r = 0, g = 0;
+    bool live = false;
+    auto fetch = [&](int i) {
+      kt = i / (4 * p.rows);
+      const int j = i - kt * 4 * p.rows;
+      r = j >> 2;
+      g = j & 3;
+      live = false;
+      if (i >= groups) return;
+      int tok = r;
+      if (kGrouped) {
+        const int s = __ldcg(p.sorted_ids + static_cast<int64_t>(blk) * p.rows + r);
+        if (s < 0 || s >= p.M) return;
+        tok = s / p.top_k;
+      }
+      const int k = (kt0 + kt) * TK + g * 32;  // element of K
+      live = true;
+      sb = 0;
+      if (k >= p.K) {  // behind K: zero codes with scale 2^-127
+        v[0] = v[1] = v[2] = v[3] = make_uint4(0, 0, 0, 0);
+      } else if (kRaw) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a) + tok * p.lda + k);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = __ldcg(src + q);
+      } else {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.a) + tok * p.lda + k);
+        v[0] = __ldcg(src);
+        v[1] = __ldcg(src + 1);
+        sb = __ldcg(p.sfa + tok * p.lds + (k >> 5));
+      }
+    };
+    fetch(t);
+    for (int pass = 0; pass < passes; ++pass) {
+      if (live) {
+        uint4 c0 = v[0], c1 = v[1];
+        if (kRaw) {
+          const uint32_t amax = max(max(absmax8(v[0]), absmax8(v[1])), max(absmax8(v[2]), absmax8(v[3])));
+          const int e = mx8_exp<kDtype>(amax);
+          sb = static_cast<uint32_t>(e);
+          const uint2 q0 = mx8_chunk_codes<kDtype>(v[0], e, p.zero), q1 = mx8_chunk_codes<kDtype>(v[1], e, p.zero);
+          const uint2 q2 = mx8_chunk_codes<kDtype>(v[2], e, p.zero), q3 = mx8_chunk_codes<kDtype>(v[3], e, p.zero);
+          c0 = make_uint4(q0.x, q0.y, q1.x, q1.y);
+          c1 = make_uint4(q2.x, q2.y, q3.x, q3.y);
+        }
+        // 128-byte swizzle: 16-byte chunk c of row r sits at chunk c ^ (r % 8)
+        uint8_t* row = s_act + kt * p.n_pad * TK + r * TK;
+        *reinterpret_cast<uint4*>(row + (((2 * g) ^ (r & 7)) << 4)) = c0;
+        *reinterpret_cast<uint4*>(row + (((2 * g + 1) ^ (r & 7)) << 4)) = c1;
+        s_sfa[kt * 512 + (r & 31) * 16 + (r >> 5) * 4 + g] = static_cast<uint8_t>(sb);
+      }
+      if (pass + 1 < passes) fetch(t + (pass + 1) * F_FILL);
+      fence_proxy_async_smem();
+      mbar_arrive(&bars->ready[pass]);
+    }
+  }
+
+  // ---------------- epilogue (warps 2-9): TMEM lanes = W rows, columns = activation rows
+  float* part = reinterpret_cast<float*>(smem);
+  T* C = static_cast<T*>(p.c);
+  const int q = warp & 3, half = (warp - 2) >> 2;
+  bool ok = true;
+  // output row of activation row r, -1: none
+  auto out_row = [&](int r) {
+    if (!kGrouped) return r < p.rows ? r : -1;
+    if (r >= p.rows) return -1;
+    const int s = __ldcg(p.sorted_ids + static_cast<int64_t>(blk) * p.rows + r);
+    return s < p.M ? s : -1;
+  };
+  auto store = [&](int s, int n, float v) {
+    if (s < 0 || n >= p.N) return;
+    if (kGrouped) v *= p.topk_w != nullptr ? __ldcg(p.topk_w + s) : 1.0f;
+    else if (p.bias != nullptr) v += O::load(static_cast<const T*>(p.bias) + n);
+    C[static_cast<int64_t>(s) * p.ldc + n] = O::one(v);
+  };
+  if (warp >= 2) {
+    ok = mbar_wait(&bars->acc_full, 0, p.status, 0x705);
+    ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+    tc_fence_after();
+    if (32 * half < p.rows) {
+      uint32_t acc[32];
+      tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + 32 * half, acc);
+      tmem_ld_wait();
+      const int row = q * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const int r = 32 * half + i;
+        if (r < p.rows) {
+          const float v = nkt > 0 ? __uint_as_float(acc[i]) : 0.f;
+          if (p.split > 1) part[r * TM + row] = v;
+          else if (ok) store(out_row(r), n_tile * TM + row, v);
+        }
+      }
+    }
+  }
+  if (p.split > 1) {
+    __syncwarp();
+    cluster_sync();  // every CTA's partials are in its shared memory
+    if (warp >= 2 && ok) {
+      const int share = TM / p.split;  // W rows this CTA adds up
+      for (int i = threadIdx.x - 64; i < share * p.rows; i += F_FILL) {
+        const int r = i / share, row = rank * share + (i - r * share);
+        float v = 0.f;
+        for (int c = 0; c < p.split; ++c) {
+          float x;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_addr(part + r * TM + row, c)));
+          v += x;
+        }
+        store(out_row(r), n_tile * TM + row, v);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while another reads its partials
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, F_TMEM);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Segments of the grouped product: runs of consecutive live blocks that name
 // the same expert, cut into at most nbmax blocks.  One CTA; blocks are walked
 // in chunks of the CTA's size with carries, entries come out in order.
@@ -483,6 +768,76 @@ int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, c
                     smem, s, tw, ta, p);
 }
 
+// How a few-rows launch splits: `split` CTAs of a cluster share an item's K so
+// that the items fill the SMs; 0: the rows do not fit (see F_ACT_MAX).
+struct FewPlan {
+  int split, kt_per, ring;
+  size_t smem;
+};
+FewPlan few_plan(int64_t items, int rows, int64_t K) {
+  FewPlan f = {0, 0, 0, 0};
+  if (rows < 1 || rows > F_ROWS_MAX) return f;
+  const int num_kt = static_cast<int>((K + TK - 1) / TK), n_pad = (rows + 15) / 16 * 16;
+  int split = 1;
+  while (split < 8 && items * split * 2 <= device_sm_count() && num_kt >= split * 4) split *= 2;
+  f.kt_per = (num_kt + split - 1) / split;
+  if (f_act_bytes(n_pad, f.kt_per) > F_ACT_MAX) return f;
+  if ((f.kt_per * 4 * rows + F_FILL - 1) / F_FILL > F_PASS_MAX) return f;
+  const int room = (kSmemMax - 1024 - static_cast<int>(sizeof(FBars)) - f_act_bytes(n_pad, f.kt_per)) / (T_W + 512);
+  // the ring also holds the partial sums, 512 bytes an activation row
+  f.ring = std::max(std::min(std::min(room, F_RING_MAX), f.kt_per), (n_pad * TM * 4 + T_W - 1) / T_W);
+  if (f.ring > room) return f;
+  f.smem = 1024 + sizeof(FBars) + f_act_bytes(n_pad, f.kt_per) + static_cast<size_t>(f.ring) * (T_W + 512);
+  f.split = split;
+  return f;
+}
+
+template <int kDtype, bool kGrouped, bool kRaw>
+int launch_few(const char* who, const CUtensorMap& tw, const FewArgs& p, int64_t items, size_t smem, cudaStream_t s) {
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(&mxf8_few_rows_kernel<kDtype, kGrouped, kRaw>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+    if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
+    attr_set[dev] = true;
+  }
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(items * p.split));
+  cfg.blockDim = dim3(F_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mxf8_few_rows_kernel<kDtype, kGrouped, kRaw>, tw, p);
+  if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
+  return check_launch(who);
+}
+
+template <bool kGrouped>
+int run_few(const char* who, const CUtensorMap& tw, FewArgs& p, const FewPlan& f, int64_t items, int dtype, bool raw,
+            cudaStream_t s) {
+  p.split = f.split;
+  p.kt_per = f.kt_per;
+  p.ring = f.ring;
+  p.n_pad = (p.rows + 15) / 16 * 16;
+  p.zero = 0.0f;  // +0.0 as an operand the compiler cannot fold (see mx8_scaled)
+  if (dtype == QDQ_DTYPE_FP16)
+    return raw ? launch_few<QDQ_DTYPE_FP16, kGrouped, true>(who, tw, p, items, f.smem, s)
+               : launch_few<QDQ_DTYPE_FP16, kGrouped, false>(who, tw, p, items, f.smem, s);
+  return raw ? launch_few<QDQ_DTYPE_BF16, kGrouped, true>(who, tw, p, items, f.smem, s)
+             : launch_few<QDQ_DTYPE_BF16, kGrouped, false>(who, tw, p, items, f.smem, s);
+}
+
 int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
   if (dtype != QDQ_DTYPE_BF16 && dtype != QDQ_DTYPE_FP16)
     return fail(QDQ_ERR_INVALID_ARG, "%s: dtype must be bf16 (0) or fp16 (1)", who);
@@ -499,18 +854,66 @@ int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
 
 using namespace qdqb200;
 
+namespace qdqb200 {
+namespace {
+
+// The few-rows launch of a dense product, or false where its rows do not fit.
+bool dense_few(const char* who, const void* a, int64_t lda, const void* a_scales, int64_t lds, bool raw,
+               const void* w_codes, const void* w_sf_tiled, const void* bias, void* c, int64_t M, int64_t N, int64_t K,
+               int64_t ldw, int64_t ldc, int dtype, cudaStream_t s, int* st) {
+  const int64_t n_tiles = (N + TM - 1) / TM;
+  const FewPlan f = M <= F_ROWS_MAX ? few_plan(n_tiles, static_cast<int>(M), K) : FewPlan{0, 0, 0, 0};
+  if (f.split == 0) return false;
+  FewArgs p = {};
+  p.a = a;
+  p.lda = lda;
+  p.sfa = static_cast<const uint8_t*>(a_scales);
+  p.lds = lds;
+  p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
+  p.bias = bias;
+  p.c = c;
+  p.ldc = ldc;
+  p.M = p.rows = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
+  p.top_k = 1;
+  p.status = device_status_ptr();
+  CUtensorMap tw;
+  *st = p.status == nullptr ? QDQ_ERR_CUDA : make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128);
+  if (*st == QDQ_OK) *st = run_few<false>(who, tw, p, f, n_tiles, dtype, raw, s);
+  return true;
+}
+
+int check_dense(const char* who, const void* w_codes, const void* w_sf_tiled, const void* bias, const void* c,
+                int64_t N, int64_t K, int64_t ldw, int64_t ldc) {
+  if (!w_codes || !w_sf_tiled || !c) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (ldw < K || ldc < N) return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
+  if (off(w_codes, 16) || ldw % 16 || off(w_sf_tiled, 16) || off(c, 2) || off(bias, 2))
+    return fail(QDQ_ERR_ALIGNMENT, "%s: codes and scales must be 16-byte aligned", who);
+  return QDQ_OK;
+}
+
+}  // namespace
+}  // namespace qdqb200
+
 extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t lda, int64_t lds,
                              const void* w_codes, const void* w_sf_tiled, const void* bias, void* c, int64_t M,
                              int64_t N, int64_t K, int64_t ldw, int64_t ldc, int out_dtype, void* stream) {
   const char* who = "fp8_gemm_mxf8";
   if (int st = check_product(who, out_dtype, M, N, K)) return st;
   if (M == 0 || N == 0) return QDQ_OK;
-  if (!a_codes || !a_scales || !w_codes || !w_sf_tiled || !c) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
-  if (lda < K || ldw < K || ldc < N || lds < qdq_mxfp8_scale_stride(K))
+  if (int st = check_dense(who, w_codes, w_sf_tiled, bias, c, N, K, ldw, ldc)) return st;
+  if (!a_codes || !a_scales) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (lda < K || lds < qdq_mxfp8_scale_stride(K))
     return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
-  if (off(a_codes, 16) || lda % 16 || off(a_scales, 16) || lds % 16 || off(w_codes, 16) || ldw % 16 ||
-      off(w_sf_tiled, 16) || off(c, 2) || off(bias, 2))
+  if (off(a_codes, 16) || lda % 16 || off(a_scales, 16) || lds % 16)
     return fail(QDQ_ERR_ALIGNMENT, "%s: codes and scales must be 16-byte aligned", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int few = QDQ_OK;
+  if (dense_few(who, a_codes, lda, a_scales, lds, false, w_codes, w_sf_tiled, bias, c, M, N, K, ldw, ldc, out_dtype, s,
+                &few))
+    return few;
   int* status = device_status_ptr();
   if (status == nullptr) return QDQ_ERR_CUDA;
   GemmArgs p = {};
@@ -532,7 +935,6 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   if (int st = make_tmap_u8_2d(&ta, a_codes, M, K, lda, TK, p.nt, 128)) return st;
   const int64_t items = ((M + p.nt - 1) / p.nt) * ((N + TM - 1) / TM);
   if (items >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, p, items, s)
                                      : launch_gemm<QDQ_DTYPE_BF16, false>(who, tw, ta, p, items, s);
 }
@@ -548,10 +950,17 @@ extern "C" int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void
   const char* who = "fp8_linear_mxf8";
   if (int st = check_product(who, dtype, M, N, K)) return st;
   if (M == 0 || N == 0) return QDQ_OK;
-  if (!a || !w_codes || !w_sf_tiled || !c) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (!a) return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (int st = check_dense(who, w_codes, w_sf_tiled, bias, c, N, K, ldw, ldc)) return st;
+  if (lda < K) return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
+  if (off(a, 16) || lda % 8) return fail(QDQ_ERR_ALIGNMENT, "%s: rows of a must be 16-byte aligned", who);
   if (workspace == nullptr || off(workspace, 256) || workspace_bytes < fp8_linear_workspace_bytes(M, K))
     return fail(QDQ_ERR_INVALID_ARG, "%s: workspace missing, unaligned or smaller than fp8_linear_workspace_bytes()",
                 who);
+  int few = QDQ_OK;
+  if (dense_few(who, a, lda, nullptr, 0, true, w_codes, w_sf_tiled, bias, c, M, N, K, ldw, ldc, dtype,
+                static_cast<cudaStream_t>(stream), &few))
+    return few;
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + up256(M * K);
   const int64_t lds = qdq_mxfp8_scale_stride(K);
@@ -585,7 +994,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
     return fail(QDQ_ERR_INVALID_ARG, "%s: null pointer", who);
   if ((a ? lda < K : ldac < K || lds < qdq_mxfp8_scale_stride(K)) || ldc < N)
     return fail(QDQ_ERR_INVALID_ARG, "%s: leading dimension too small", who);
-  if ((!a && (off(a_codes, 16) || ldac % 16 || off(a_scales, 16) || lds % 16)) || off(w_codes, 16) ||
+  if ((a ? off(a, 16) || lda % 8 : off(a_codes, 16) || ldac % 16 || off(a_scales, 16) || lds % 16) || off(w_codes, 16) ||
       off(w_sf_tiled, 16) || off(c, 2))
     return fail(QDQ_ERR_ALIGNMENT, "%s: codes and scales must be 16-byte aligned", who);
   if (num_experts >= (1ll << 31) / N || size_m >= (1ll << 30) / top_k || num_sorted >= (1ll << 30))
@@ -600,6 +1009,37 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   int* status = device_status_ptr();
   if (status == nullptr) return QDQ_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap tw, ta;
+  if (int st = make_tmap_u8_2d(&tw, w_codes, num_experts * N, K, K, TK, TM, 128)) return st;
+  const int64_t n_slots = size_m * top_k;
+  // A decode step of few blocks: one launch without quantisation pass or segments, an item per block.
+  if (num_blocks * n_tiles <= 2 * device_sm_count()) {
+    const FewPlan f = few_plan(num_blocks * n_tiles, moe_block_size, K);
+    if (f.split != 0) {
+      FewArgs p = {};
+      p.a = a ? a : a_codes;
+      p.lda = a ? lda : ldac;
+      p.sfa = static_cast<const uint8_t*>(a_scales);
+      p.lds = lds;
+      p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
+      p.sf_per_expert = qdq_sf_tiled_bytes(N, K);
+      p.c = c;
+      p.ldc = ldc;
+      p.sorted_ids = sorted_token_ids;
+      p.expert_ids = expert_ids;
+      p.num_post_padded = num_tokens_post_padded;
+      p.topk_w = mul_topk_weights ? topk_weights : nullptr;
+      p.M = static_cast<int>(n_slots);
+      p.N = static_cast<int>(N);
+      p.K = static_cast<int>(K);
+      p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
+      p.rows = moe_block_size;
+      p.top_k = top_k;
+      p.num_experts = static_cast<int>(num_experts);
+      p.status = status;
+      return run_few<true>(who, tw, p, f, num_blocks * n_tiles, dtype, a != nullptr, s);
+    }
+  }
   int32_t* seg_tab = static_cast<int32_t*>(workspace);
   if (a) {
     uint8_t* ws = static_cast<uint8_t*>(workspace) + up256(4 * (1 + 2 * num_blocks));
@@ -630,7 +1070,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.sorted_ids = sorted_token_ids;
   p.expert_ids = expert_ids;
   p.topk_w = mul_topk_weights ? topk_weights : nullptr;
-  p.M = static_cast<int>(size_m * top_k);
+  p.M = static_cast<int>(n_slots);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
@@ -639,8 +1079,6 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.num_blocks = static_cast<int>(num_blocks);
   p.num_experts = static_cast<int>(num_experts);
   p.status = status;
-  CUtensorMap tw, ta;
-  if (int st = make_tmap_u8_2d(&tw, w_codes, num_experts * N, K, K, TK, TM, 128)) return st;
   if (int st = make_tmap_u8_2d(&ta, a_codes, size_m, K, ldac, TK, 1, 128)) return st;  // 4-row gathers: a box of one row
   return dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, true>(who, tw, ta, p, num_blocks * n_tiles, s)
                                  : launch_gemm<QDQ_DTYPE_BF16, true>(who, tw, ta, p, num_blocks * n_tiles, s);
