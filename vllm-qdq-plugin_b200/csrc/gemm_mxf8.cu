@@ -12,15 +12,16 @@
 // One CTA per SM walks work items (a segment of at most NT activation rows,
 // 128 rows of W); 12 warps:
 //   warp 0      TMA producer: W codes and scales of a K-128 stage, and the
-//               segment's codes: one box of NT consecutive rows (dense), or
-//               4-row gathers by token index (grouped), so that routed rows
-//               are never copied into sorted order
+//               codes of the segment's rows, which are consecutive (grouped:
+//               a pass before copies the routed rows into sorted order)
 //   warp 1      MMA issuer: per stage 4 MMAs (K = 32 each), M = 128,
 //               N = the segment's rows rounded up to 16
-//   warps 2-3   activation scales: a lane owns rows, loads 16 scales (four
-//               stages) of a row at once and writes each stage's four bytes
-//               into the chunk layout that tcgen05.cp expects
-//   warps 4-11  epilogue: TMEM lanes = W rows, columns = activation rows
+//   warps 2-5   activation scales, four stages ("quad") at a time into a ring
+//               of four quads, one per warp: a lane loads 16 scales of a row
+//               at once and writes each stage's four bytes into the chunk
+//               layout that tcgen05.cp expects.  One proxy fence a quad: a
+//               fence per stage held the whole ring to 0.55 us a stage
+//   warps 6-13  epilogue: TMEM lanes = W rows, columns = activation rows
 // What the kernel before it on the stream may have written (scales, routing,
 // segments) is read past L1 (__ldcg): under programmatic dependent launch this
 // kernel's CTAs start before that one has finished.
@@ -43,15 +44,18 @@ constexpr int NT_MAX = 192;          // activation rows per item: two accumulato
 constexpr int T_W = TM * TK;         // 16 KB
 constexpr int T_STAGES_MAX = 12;
 constexpr int T_EPI = 8;             // epilogue warps
-constexpr int T_SCALE = 2;           // scale warps
+constexpr int T_SCALE = 4;           // scale warps = quads of stages in the scale ring
 constexpr int T_THREADS = 32 * (2 + T_SCALE + T_EPI);
 constexpr uint32_t T_TMEM = 512, T_SFW = 2 * NT_MAX, T_SFA = T_SFW + 4;
 
-__host__ __device__ constexpr int t_stage_bytes(int nt) { return (T_W + nt * TK + 512 + 1024 + 1023) / 1024 * 1024; }
+__host__ __device__ constexpr int t_stage_bytes(int nt) { return T_W + nt * TK + 512; }  // codes, W scales
+__host__ __device__ constexpr int t_sf_bytes(int nt) { return nt > 128 ? 1024 : 512; }     // a stage's activation scales
 
 struct __align__(8) TBars {
-  uint64_t full[T_STAGES_MAX];   // codes and W scales landed (1 arrival + tx), activation scales written (1 per scale warp)
+  uint64_t full[T_STAGES_MAX];   // codes and W scales landed (1 arrival + tx)
   uint64_t empty[T_STAGES_MAX];  // the stage's MMAs completed
+  uint64_t sf_full[T_SCALE];     // a quad's activation scales are written
+  uint64_t sf_empty[T_SCALE];    // the quad's MMAs completed
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t drain;
@@ -60,8 +64,11 @@ struct __align__(8) TBars {
 };
 constexpr int kSmemMax = 227 * 1024;
 __host__ __device__ constexpr int t_stages(int nt) {
-  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars))) / t_stage_bytes(nt);
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars)) - 4 * T_SCALE * t_sf_bytes(nt)) / t_stage_bytes(nt);
   return n < T_STAGES_MAX ? n : T_STAGES_MAX;
+}
+__host__ __device__ constexpr int t_smem(int nt) {
+  return 1024 + t_stages(nt) * t_stage_bytes(nt) + 4 * T_SCALE * t_sf_bytes(nt) + static_cast<int>(sizeof(TBars));
 }
 
 template <int kDtype>
@@ -91,20 +98,24 @@ struct GemmArgs {
   const float* topk_w;         // nullptr: no scaling
   int M, N, K, kchunks;        // M: dense rows, grouped slots (size_m * top_k)
   int top_k, bs, num_blocks, num_experts;
-  int nt;                      // activation rows per item
+  int a_rows;                  // rows of the activation codes (grouped: sorted positions)
+  int nt, box;                 // activation rows per item, and per TMA box
   int* status;
 };
 
-// Grouped loads of four rows of a [rows, K] byte matrix into four consecutive
-// 128-byte swizzled rows of shared memory.
-__device__ __forceinline__ void tma_gather4(void* smem_dst, const CUtensorMap* map, int32_t x, int32_t r0, int32_t r1,
-                                            int32_t r2, int32_t r3, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(smem_u32(bar))
-      : "memory");
-}
+// Position in a ring of n slots and the phase parity of the current lap.  The
+// depths are run-time values: dividing a running count by them cost the single
+// issuing thread half of a stage's time.
+struct Cursor {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int n) {
+    if (++slot == n) {
+      slot = 0;
+      phase ^= 1u;
+    }
+  }
+};
 
 struct Item {
   int row0;     // first activation row (dense) or first sorted position (grouped)
@@ -136,17 +147,6 @@ __device__ __forceinline__ bool item_of(const GemmArgs& p, int i, int n_tiles, i
   return it.expert >= 0 && it.expert < p.num_experts;
 }
 
-// The activation row behind row r of an item.  Rows that stand for nothing
-// (padding slots, the fill up to a multiple of 16) read row 0: their columns
-// of the accumulator are dropped.
-template <bool kGrouped>
-__device__ __forceinline__ int token_of(const GemmArgs& p, const Item& it, int r) {
-  if (!kGrouped) return min(it.row0 + r, p.M - 1);
-  if (r >= it.rows) return 0;
-  const int s = __ldcg(p.sorted_ids + it.row0 + r);
-  return (s >= 0 && s < p.M) ? s / p.top_k : 0;
-}
-
 template <int kDtype, bool kGrouped>
 __global__ void __launch_bounds__(T_THREADS, 1)
 mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
@@ -155,9 +155,11 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int S = t_stages(p.nt), stage_bytes = t_stage_bytes(p.nt);
-  const int st_a = T_W, st_sfw = T_W + p.nt * TK, st_sfa = st_sfw + 512;
-  TBars* bars = reinterpret_cast<TBars*>(smem + S * stage_bytes);
+  // code stages | W scale stages | quads of activation scales | barriers
+  const int S = t_stages(p.nt), stage_bytes = T_W + p.nt * TK, sf_bytes = t_sf_bytes(p.nt);
+  uint8_t* s_sfw = smem + S * stage_bytes;
+  uint8_t* s_sfa = s_sfw + S * 512;
+  TBars* bars = reinterpret_cast<TBars*>(s_sfa + 4 * T_SCALE * sf_bytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_tiles = (p.N + TM - 1) / TM;
   const int num_m = kGrouped ? 1 : (p.M + p.nt - 1) / p.nt;
@@ -165,8 +167,12 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&bars->full[s], 1 + T_SCALE);
+      mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < T_SCALE; ++b) {
+      mbar_init(&bars->sf_full[b], 1);
+      mbar_init(&bars->sf_empty[b], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
@@ -192,89 +198,87 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 
   if (warp == 0) {
     // ---------------- producer
-    int it = 0;
-    bool ok = true;
-    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-      Item w;
-      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
-      const int w_row = w.expert * p.N + w.n_tile * TM;
-      const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
-      const int gathers = kGrouped ? (w.rows + 15) / 16 * 4 : 0;  // rows up to the MMA's N, four at a time
-      int tok[2][4];
-      if (kGrouped) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) tok[j][q] = token_of<true>(p, w, 4 * (lane + 32 * j) + q);
-      }
-      for (int kt = 0; kt < num_kt; ++kt, ++it) {
-        const int s = it % S;
-        ok = mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, p.status, 0x601);
-        ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
-        if (!ok) break;
-        uint8_t* st = smem + s * stage_bytes;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&bars->full[s], T_W + 512 + (kGrouped ? gathers * 4 : p.nt) * TK);
+    if (elect_one()) {
+      Cursor at;
+      int issued = 0;
+      bool ok = true;
+      for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+        Item w;
+        if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+        const int w_row = w.expert * p.N + w.n_tile * TM;
+        const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
+        const int boxes = (w.rows + p.box - 1) / p.box;
+        const uint32_t tx = T_W + 512 + boxes * p.box * TK;
+        bool ready = mbar_test(&bars->empty[at.slot], at.phase ^ 1u);
+        for (int kt = 0; kt < num_kt; ++kt, ++issued) {
+          const int s = at.slot;
+          if (!ready && !mbar_wait(&bars->empty[s], at.phase ^ 1u, p.status, 0x601)) { ok = false; break; }
+          at.next(S);
+          ready = mbar_test(&bars->empty[at.slot], at.phase ^ 1u);  // the next stage's, while this one is issued
+          uint8_t* st = smem + s * stage_bytes;
+          mbar_arrive_expect_tx(&bars->full[s], tx);
           tma_load_2d(st, &tmap_w, kt * TK, w_row, &bars->full[s]);
-          bulk_load(st + st_sfw, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
-          if (!kGrouped) tma_load_2d(st + st_a, &tmap_a, kt * TK, w.row0, &bars->full[s]);
-        }
-        if (kGrouped) {
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if (lane + 32 * j < gathers)
-              tma_gather4(st + st_a + (lane + 32 * j) * 4 * TK, &tmap_a, kt * TK, tok[j][0], tok[j][1], tok[j][2],
-                          tok[j][3], &bars->full[s]);
+          bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d(st + T_W + b * p.box * TK, &tmap_a, kt * TK, w.row0 + b * p.box, &bars->full[s]);
         }
       }
+      if (!ok) bars->abort = 1;
+      // every issued copy has landed before the CTA may exit
+      for (int j = max(0, issued - S); j < issued; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
     }
-    if (!ok) bars->abort = 1;
-    // every issued copy has landed before the CTA may exit
-    for (int j = (it > S ? it - S : 0); j < it; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
   } else if (warp == 1) {
     // ---------------- MMA issuer
     if (elect_one()) {
-      int it = 0, j = 0;
+      Cursor at, sf_at, acc_at;
+      const uint64_t dw0 = smem_desc_sw128(smem), da0 = smem_desc_sw128(smem + T_W);
+      const uint64_t dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
       bool ok = true;
       for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
         Item w;
         if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
         const int n_mma = (w.rows + 15) / 16 * 16;
         const uint32_t idesc = idesc_mxf8(TM, n_mma);
-        const int buf = j & 1;
-        if (!mbar_wait(&bars->acc_empty[buf], ((j >> 1) & 1) ^ 1, p.status, 0x603)) { ok = false; break; }
+        if (!mbar_wait(&bars->acc_empty[acc_at.slot], acc_at.phase ^ 1u, p.status, 0x603)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t acc = tmem + NT_MAX * buf;
-        for (int kt = 0; kt < num_kt; ++kt, ++it) {
-          const int s = it % S;
-          if (!mbar_wait(&bars->full[s], (it / S) & 1, p.status, 0x604)) { ok = false; break; }
-          if (*(volatile int*)&bars->abort) { ok = false; break; }
+        const uint32_t acc = tmem + NT_MAX * acc_at.slot;
+        bool ready = mbar_test(&bars->full[at.slot], at.phase);
+        for (int kt = 0; kt < num_kt; ++kt) {
+          const int s = at.slot;
+          if ((kt & 3) == 0 && !mbar_wait(&bars->sf_full[sf_at.slot], sf_at.phase, p.status, 0x608)) { ok = false; break; }
+          if (!ready && !mbar_wait(&bars->full[s], at.phase, p.status, 0x604)) { ok = false; break; }
           tc_fence_after();
-          uint8_t* st = smem + s * stage_bytes;
-          tmem_cp_sf(tmem + T_SFW, smem_desc_sf(st + st_sfw));
-          tmem_cp_sf(tmem + T_SFA, smem_desc_sf(st + st_sfa));
-          if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, smem_desc_sf(st + st_sfa + 512));
-          const uint64_t dw = smem_desc_sw128(st), da = smem_desc_sw128(st + st_a);
+          at.next(S);
+          ready = mbar_test(&bars->full[at.slot], at.phase);  // the next stage's, while this one is issued
+          const uint64_t dsa = dsa0 + ((sf_at.slot * 4 + (kt & 3)) * sf_bytes >> 4);
+          tmem_cp_sf(tmem + T_SFW, dsw0 + (s * 512 >> 4));
+          tmem_cp_sf(tmem + T_SFA, dsa);
+          if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, dsa + (512 >> 4));
+          const uint64_t dw = dw0 + (s * stage_bytes >> 4), da = da0 + (s * stage_bytes >> 4);
 #pragma unroll
           for (uint32_t kk = 0; kk < 4; ++kk)  // K step kk reads scale byte kk of each row's four
             mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + T_SFW) | (kk << 30),
                      (tmem + T_SFA) | (kk << 30), (kt | kk) != 0);
           tc_commit(&bars->empty[s]);
+          if ((kt & 3) == 3 || kt + 1 == num_kt) {
+            tc_commit(&bars->sf_empty[sf_at.slot]);
+            sf_at.next(T_SCALE);
+          }
         }
         if (!ok) break;
-        tc_commit(&bars->acc_full[buf]);
-        ++j;
+        tc_commit(&bars->acc_full[acc_at.slot]);
+        acc_at.next(2);
       }
       if (!ok) bars->abort = 1;
       tc_commit(&bars->drain);
       mbar_wait(&bars->drain, 0, p.status, 0x605);
     }
   } else if (warp < 2 + T_SCALE) {
-    // ---------------- activation scales
-    constexpr int kLanes = 32 * T_SCALE, kR = NT_MAX / kLanes;  // rows per lane
-    const int t = threadIdx.x - 64;
-    int it = 0;
+    // ---------------- activation scales: warp u fills the quads u, u + 4, ... of the CTA's stages
+    constexpr int kR = NT_MAX / 32;  // rows per lane
+    const int u = warp - 2;
+    const int quads = (num_kt + 3) / 4;
+    int quad = 0;  // first quad of the item, counted over the CTA's items
     bool ok = true;
     for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
       Item w;
@@ -283,36 +287,32 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       const uint8_t* src[kR];
 #pragma unroll
       for (int j = 0; j < kR; ++j)
-        src[j] = p.sfa + static_cast<int64_t>(token_of<kGrouped>(p, w, t + kLanes * j)) * p.lds;
-      uint4 cur[kR], nxt[kR];
+        src[j] = p.sfa + static_cast<int64_t>(min(w.row0 + lane + 32 * j, p.a_rows - 1)) * p.lds;
+      for (int h = (u - quad) & (T_SCALE - 1); h < quads; h += T_SCALE) {
+        uint4 v[kR];
 #pragma unroll
-      for (int j = 0; j < kR; ++j)
-        if (t + kLanes * j < n_mma) nxt[j] = __ldcg(reinterpret_cast<const uint4*>(src[j]));
-      for (int kt = 0; kt < num_kt; ++kt, ++it) {
-        if ((kt & 3) == 0) {
-#pragma unroll
-          for (int j = 0; j < kR; ++j) {
-            cur[j] = nxt[j];
-            if (kt + 4 < num_kt && t + kLanes * j < n_mma)
-              nxt[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + (kt + 4) * 4));
-          }
-        }
-        const int s = it % S;
-        ok = mbar_wait(&bars->empty[s], ((it / S) & 1) ^ 1, p.status, 0x606);
-        ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+        for (int j = 0; j < kR; ++j)
+          if (lane + 32 * j < n_mma) v[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + 16 * h));
+        ok = mbar_wait(&bars->sf_empty[u], (((quad + h) / T_SCALE) & 1) ^ 1, p.status, 0x606);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        uint8_t* sf = smem + s * stage_bytes + st_sfa;
+        uint8_t* sf = s_sfa + u * 4 * sf_bytes;
 #pragma unroll
         for (int j = 0; j < kR; ++j) {
-          const int r = t + kLanes * j;
-          if (r < n_mma)
-            *reinterpret_cast<uint32_t*>(sf + (r >> 7) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4) = cur[j].x;
-          cur[j] = make_uint4(cur[j].y, cur[j].z, cur[j].w, 0u);  // the next stage's four
+          const int r = lane + 32 * j;
+          if (r < n_mma) {
+            uint8_t* at = sf + (j >> 2) * 512 + lane * 16 + (j & 3) * 4;
+            *reinterpret_cast<uint32_t*>(at) = v[j].x;
+            *reinterpret_cast<uint32_t*>(at + sf_bytes) = v[j].y;
+            *reinterpret_cast<uint32_t*>(at + 2 * sf_bytes) = v[j].z;
+            *reinterpret_cast<uint32_t*>(at + 3 * sf_bytes) = v[j].w;
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars->full[s]);
+        if (lane == 0) mbar_arrive(&bars->sf_full[u]);
       }
+      quad += quads;
     }
     if (!ok) bars->abort = 1;
   } else {
@@ -473,8 +473,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   }
   const int w_row = expert * p.N + n_tile * TM;
   const uint8_t* sfw = p.sfw + expert * p.sf_per_expert + (static_cast<int64_t>(n_tile) * p.kchunks + kt0) * 512;
-  auto issue = [&](int kt) {
-    const int s = kt % p.ring;
+  auto issue = [&](int kt, int s) {
     mbar_arrive_expect_tx(&bars->full[s], T_W + 512);
     tma_load_2d(smem + s * T_W, &tmap_w, (kt0 + kt) * TK, w_row, &bars->full[s]);
     bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
@@ -489,7 +488,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     mbar_init(&bars->acc_full, 1);
     bars->abort = 0;
     fence_barrier_init();
-    for (int kt = 0; kt < pre; ++kt) issue(kt);  // W needs nothing that the previous kernel writes
+    for (int kt = 0; kt < pre; ++kt) issue(kt, kt);  // W needs nothing that the previous kernel writes
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, F_TMEM);
@@ -504,13 +503,14 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     // ---------------- producer
     if (elect_one()) {
       int issued = pre;
-      for (int kt = pre; kt < nkt; ++kt) {
-        if (!mbar_wait(&bars->empty[kt % p.ring], ((kt / p.ring) & 1) ^ 1, p.status, 0x701)) {
+      Cursor at;  // the second lap refills a slot once the first lap's MMAs have completed
+      for (int kt = pre; kt < nkt; ++kt, at.next(p.ring)) {
+        if (!mbar_wait(&bars->empty[at.slot], at.phase, p.status, 0x701)) {
           bars->abort = 1;
           break;
         }
         if (*(volatile int*)&bars->abort) break;
-        issue(kt);
+        issue(kt, at.slot);
         ++issued;
       }
       for (int kt = max(0, issued - p.ring); kt < issued; ++kt)
@@ -522,16 +522,20 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       const uint32_t idesc = idesc_mxf8(TM, p.n_pad);
       bool ok = true;
       int passes = 0;  // passes seen complete
-      for (int kt = 0; kt < nkt; ++kt) {
+      Cursor at;
+      const uint64_t dw0 = smem_desc_sw128(smem), da0 = smem_desc_sw128(s_act);
+      const uint64_t dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
+      for (int kt = 0; kt < nkt; ++kt, at.next(p.ring)) {
         const int need = ((kt + 1) * 4 * p.rows + F_FILL - 1) / F_FILL;
-        for (; ok && passes < need; ++passes) ok = mbar_wait(&bars->ready[passes], 0, p.status, 0x703);
-        const int s = kt % p.ring;
-        if (ok) ok = mbar_wait(&bars->full[s], (kt / p.ring) & 1, p.status, 0x704);
-        if (!ok || *(volatile int*)&bars->abort) { ok = false; break; }
+        for (; ok && passes < need; ++passes)
+          ok = mbar_wait(&bars->ready[passes], 0, p.status, 0x703) && !*(volatile int*)&bars->abort;
+        const int s = at.slot;
+        if (ok) ok = mbar_wait(&bars->full[s], at.phase, p.status, 0x704);
+        if (!ok) break;
         tc_fence_after();
-        tmem_cp_sf(tmem + F_SFW, smem_desc_sf(s_sfw + s * 512));
-        tmem_cp_sf(tmem + F_SFA, smem_desc_sf(s_sfa + kt * 512));
-        const uint64_t dw = smem_desc_sw128(smem + s * T_W), da = smem_desc_sw128(s_act + kt * p.n_pad * TK);
+        tmem_cp_sf(tmem + F_SFW, dsw0 + (s * 512 >> 4));
+        tmem_cp_sf(tmem + F_SFA, dsa0 + (kt * 512 >> 4));
+        const uint64_t dw = dw0 + (s * T_W >> 4), da = da0 + (kt * p.n_pad * TK >> 4);
 #pragma unroll
         for (uint32_t kk = 0; kk < 4; ++kk)
           mma_mxf8(tmem, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + F_SFW) | (kk << 30),
@@ -720,14 +724,57 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, int live,
   if (t == 0) seg_tab[0] = carry_count;
 }
 
+// The pass before the grouped product: block 0 builds the segments, the others
+// lay the routed rows out in sorted order, a warp a row, quantising 16-bit rows
+// (kRaw) or copying MXFP8 rows.  Positions that no live slot fills keep what
+// the workspace held: their columns of the accumulators are dropped.  (Gathering
+// the rows in the product instead, by 4-row TMA gathers, took 65 cycles a
+// gather, 3100 a stage of 192 rows against 600 with boxes of sorted rows.)
+template <int kDtype, bool kRaw>
 __global__ void __launch_bounds__(SEG_THREADS)
-mxf8_segments_kernel(const int32_t* __restrict__ expert_ids, const int32_t* __restrict__ num_post_padded, int bs,
-                     int num_blocks, int num_experts, int nbmax, int32_t* __restrict__ seg_tab) {
+mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const uint8_t* __restrict__ a_scales,
+                        int64_t lds, const int32_t* __restrict__ sorted_ids, const int32_t* __restrict__ expert_ids,
+                        const int32_t* __restrict__ num_post_padded, int bs, int num_blocks, int num_experts,
+                        int nbmax, int top_k, int n_slots, int K, uint8_t* __restrict__ codes,
+                        uint8_t* __restrict__ scales, int64_t ldso, int32_t* __restrict__ seg_tab, float zero) {
   pdl_launch_dependents();
   pdl_wait();
-  const int npp = __ldg(num_post_padded);
+  const int npp = __ldcg(num_post_padded);
   const int live = npp <= 0 ? 0 : min(num_blocks, (npp - 1) / bs + 1);
-  build_segments(expert_ids, live, num_experts, nbmax, seg_tab);
+  if (blockIdx.x == 0) {
+    build_segments(expert_ids, live, num_experts, nbmax, seg_tab);
+    return;
+  }
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int64_t positions = static_cast<int64_t>(live) * bs;
+  const int gpr = K / 32;
+  for (int64_t pos = static_cast<int64_t>(blockIdx.x - 1) * warps + (threadIdx.x >> 5); pos < positions;
+       pos += static_cast<int64_t>(gridDim.x - 1) * warps) {
+    const int s = __ldcg(sorted_ids + pos);
+    if (s < 0 || s >= n_slots) continue;
+    const uint8_t* src = a + static_cast<int64_t>(s / top_k) * lda_bytes;
+    uint8_t* dst = codes + pos * K;
+    if (kRaw) {
+      for (int c0 = 0; c0 < 4 * gpr; c0 += 32) {  // 16-byte chunks of 8 elements, four lanes a group
+        const int c = c0 + lane;
+        const uint4 v = c < 4 * gpr ? __ldcg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+        uint32_t amax = absmax8(v);
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const int e = mx8_exp<kDtype>(amax);
+        if (c < 4 * gpr) {
+          *reinterpret_cast<uint2*>(dst + 8 * c) = mx8_chunk_codes<kDtype>(v, e, zero);
+          if ((c & 3) == 0) scales[pos * ldso + (c >> 2)] = static_cast<uint8_t>(e);
+        }
+      }
+      for (int g = gpr + lane; g < ldso; g += 32) scales[pos * ldso + g] = 0;
+    } else {
+      for (int c = lane; c < 2 * gpr; c += 32)
+        reinterpret_cast<uint4*>(dst)[c] = __ldcg(reinterpret_cast<const uint4*>(src) + c);
+      const uint4* from = reinterpret_cast<const uint4*>(a_scales + static_cast<int64_t>(s / top_k) * lds);
+      for (int c = lane; c < ldso / 16; c += 32) reinterpret_cast<uint4*>(scales + pos * ldso)[c] = __ldcg(from + c);
+    }
+  }
 }
 
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -763,7 +810,7 @@ int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, c
     if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
     attr_set[dev] = true;
   }
-  const size_t smem = 1024 + static_cast<size_t>(t_stages(p.nt)) * t_stage_bytes(p.nt) + sizeof(TBars);
+  const size_t smem = t_smem(p.nt);
   return launch_pdl(who, &mxf8_gemm_kernel<kDtype, kGrouped>, std::min<int64_t>(items, device_sm_count()), T_THREADS,
                     smem, s, tw, ta, p);
 }
@@ -836,6 +883,15 @@ int run_few(const char* who, const CUtensorMap& tw, FewArgs& p, const FewPlan& f
                : launch_few<QDQ_DTYPE_FP16, kGrouped, false>(who, tw, p, items, f.smem, s);
   return raw ? launch_few<QDQ_DTYPE_BF16, kGrouped, true>(who, tw, p, items, f.smem, s)
              : launch_few<QDQ_DTYPE_BF16, kGrouped, false>(who, tw, p, items, f.smem, s);
+}
+
+// Rows per item for `rows` wanted, in whole TMA boxes of 64, 32 or 16 rows: a
+// large box costs the producer fewer issues, a small one a ragged segment
+// fewer idle rows.
+void rows_per_item(GemmArgs& p, int64_t rows) {
+  const int want = static_cast<int>(std::min<int64_t>(rows, NT_MAX));
+  p.box = want > 96 ? 64 : want > 16 ? 32 : 16;
+  p.nt = (want + p.box - 1) / p.box * p.box;
 }
 
 int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
@@ -928,11 +984,12 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   p.K = static_cast<int>(K);
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
   p.top_k = 1;
-  p.nt = M >= NT_MAX ? NT_MAX : static_cast<int>((M + 15) / 16 * 16);
+  p.a_rows = p.M;
+  rows_per_item(p, M);
   p.status = status;
   CUtensorMap tw, ta;
   if (int st = make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128)) return st;
-  if (int st = make_tmap_u8_2d(&ta, a_codes, M, K, lda, TK, p.nt, 128)) return st;
+  if (int st = make_tmap_u8_2d(&ta, a_codes, M, K, lda, TK, p.box, 128)) return st;
   const int64_t items = ((M + p.nt - 1) / p.nt) * ((N + TM - 1) / TM);
   if (items >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
   return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, p, items, s)
@@ -971,8 +1028,8 @@ extern "C" int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void
 
 extern "C" int64_t fp8_moe_workspace_bytes(int64_t size_m, int64_t num_sorted, int moe_block_size, int64_t K) {
   if (size_m <= 0 || num_sorted <= 0 || moe_block_size <= 0 || K <= 0) return 0;
-  return up256(4 * (1 + 2 * (num_sorted / moe_block_size))) + up256(size_m * K) +
-         up256(size_m * qdq_mxfp8_scale_stride(K));
+  return up256(4 * (1 + 2 * (num_sorted / moe_block_size))) + up256(num_sorted * K) +
+         up256(num_sorted * qdq_mxfp8_scale_stride(K));
 }
 
 extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, const void* a_scales, int64_t ldac,
@@ -1041,29 +1098,32 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
     }
   }
   int32_t* seg_tab = static_cast<int32_t*>(workspace);
-  if (a) {
-    uint8_t* ws = static_cast<uint8_t*>(workspace) + up256(4 * (1 + 2 * num_blocks));
-    uint8_t* scales = ws + up256(size_m * K);
-    lds = qdq_mxfp8_scale_stride(K);
-    if (int st = qdq_mxfp8_rows(a, ws, scales, size_m, K, lda, K, lds, dtype, stream)) return st;
-    a_codes = ws;
-    a_scales = scales;
-    ldac = K;
-  }
+  uint8_t* codes = static_cast<uint8_t*>(workspace) + up256(4 * (1 + 2 * num_blocks));
+  uint8_t* scales = codes + up256(num_sorted * K);
+  const int64_t ldso = qdq_mxfp8_scale_stride(K);
   GemmArgs p = {};
   // Rows per item: the average expert's, rounded up to whole blocks, so that few rows leave the shared memory to
   // more stages of W in flight; never less than a block.
   const int64_t average = (num_sorted + num_experts - 1) / num_experts;
-  const int64_t rows = (average + moe_block_size - 1) / moe_block_size * moe_block_size;
-  p.nt = static_cast<int>((std::min<int64_t>(std::max<int64_t>(rows, moe_block_size), NT_MAX) + 15) / 16 * 16);
+  rows_per_item(p, (average + moe_block_size - 1) / moe_block_size * moe_block_size);
   const int nbmax = p.nt / moe_block_size;
-  if (int st = launch_pdl(who, &mxf8_segments_kernel, 1, SEG_THREADS, 0, s, expert_ids, num_tokens_post_padded,
-                          moe_block_size, static_cast<int>(num_blocks), static_cast<int>(num_experts), nbmax, seg_tab))
-    return st;
+  {
+    const int warps = SEG_THREADS / 32;
+    const int64_t grid = 1 + std::min<int64_t>((num_sorted + warps - 1) / warps, 2 * device_sm_count());
+    auto* fn = a == nullptr ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, false>
+               : dtype == QDQ_DTYPE_FP16 ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_FP16, true>
+                                         : &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, true>;
+    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, static_cast<const uint8_t*>(a ? a : a_codes),
+                            a ? lda * 2 : ldac, static_cast<const uint8_t*>(a_scales), lds, sorted_token_ids,
+                            expert_ids, num_tokens_post_padded, moe_block_size, num_blocks, num_experts, nbmax, top_k,
+                            n_slots, K, codes, scales, ldso, seg_tab, 0.0f))
+      return st;
+  }
   p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
   p.sf_per_expert = qdq_sf_tiled_bytes(N, K);
-  p.sfa = static_cast<const uint8_t*>(a_scales);
-  p.lds = lds;
+  p.sfa = scales;
+  p.lds = ldso;
+  p.a_rows = static_cast<int>(num_sorted);
   p.c = c;
   p.ldc = ldc;
   p.seg_tab = seg_tab;
@@ -1079,7 +1139,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.num_blocks = static_cast<int>(num_blocks);
   p.num_experts = static_cast<int>(num_experts);
   p.status = status;
-  if (int st = make_tmap_u8_2d(&ta, a_codes, size_m, K, ldac, TK, 1, 128)) return st;  // 4-row gathers: a box of one row
+  if (int st = make_tmap_u8_2d(&ta, codes, num_sorted, K, K, TK, p.box, 128)) return st;
   return dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, true>(who, tw, ta, p, num_blocks * n_tiles, s)
                                  : launch_gemm<QDQ_DTYPE_BF16, true>(who, tw, ta, p, num_blocks * n_tiles, s);
 }
