@@ -160,7 +160,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   uint8_t* s_sfw = smem + S * stage_bytes;
   uint8_t* s_sfa = s_sfw + S * 512;
   TBars* bars = reinterpret_cast<TBars*>(s_sfa + 4 * T_SCALE * sf_bytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = (p.N + TM - 1) / TM;
   const int num_m = kGrouped ? 1 : (p.M + p.nt - 1) / p.nt;
   const int num_kt = (p.K + TK - 1) / TK;
@@ -193,29 +193,29 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   tc_fence_after();
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);  // uniform
   const int num_items = kGrouped ? min(max(__ldcg(p.seg_tab), 0), p.num_blocks) * n_tiles : num_m * n_tiles;
 
   if (warp == 0) {
-    // ---------------- producer
-    if (elect_one()) {
-      Cursor at;
-      int issued = 0;
-      bool ok = true;
-      for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-        Item w;
-        if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
-        const int w_row = w.expert * p.N + w.n_tile * TM;
-        const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
-        const int boxes = (w.rows + p.box - 1) / p.box;
-        const uint32_t tx = T_W + 512 + boxes * p.box * TK;
-        bool ready = mbar_test(&bars->empty[at.slot], at.phase ^ 1u);
-        for (int kt = 0; kt < num_kt; ++kt, ++issued) {
-          const int s = at.slot;
-          if (!ready && !mbar_wait(&bars->empty[s], at.phase ^ 1u, p.status, 0x601)) { ok = false; break; }
-          at.next(S);
-          ready = mbar_test(&bars->empty[at.slot], at.phase ^ 1u);  // the next stage's, while this one is issued
-          uint8_t* st = smem + s * stage_bytes;
+    // ---------------- producer.  The whole warp walks the loop, so that its addresses stay in uniform registers;
+    // one lane issues.
+    const bool leader = elect_one();
+    Cursor at;
+    int issued = 0;
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+      Item w;
+      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+      const int w_row = w.expert * p.N + w.n_tile * TM;
+      const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
+      const int boxes = (w.rows + p.box - 1) / p.box;
+      const uint32_t tx = T_W + 512 + boxes * p.box * TK;
+      for (int kt = 0; kt < num_kt; ++kt, ++issued, at.next(S)) {
+        const int s = at.slot;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], at.phase ^ 1u, p.status, 0x601));
+        if (!ok) break;
+        uint8_t* st = smem + s * stage_bytes;
+        if (leader) {
           mbar_arrive_expect_tx(&bars->full[s], tx);
           tma_load_2d(st, &tmap_w, kt * TK, w_row, &bars->full[s]);
           bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
@@ -223,53 +223,65 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
             tma_load_2d(st + T_W + b * p.box * TK, &tmap_a, kt * TK, w.row0 + b * p.box, &bars->full[s]);
         }
       }
-      if (!ok) bars->abort = 1;
-      // every issued copy has landed before the CTA may exit
-      for (int j = max(0, issued - S); j < issued; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
     }
+    if (!ok) bars->abort = 1;
+    // every issued copy has landed before the CTA may exit
+    for (int j = max(0, issued - S); j < issued; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
   } else if (warp == 1) {
-    // ---------------- MMA issuer
-    if (elect_one()) {
-      Cursor at, sf_at, acc_at;
-      const uint64_t dw0 = smem_desc_sw128(smem), da0 = smem_desc_sw128(smem + T_W);
-      const uint64_t dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
-      bool ok = true;
-      for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-        Item w;
-        if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
-        const int n_mma = (w.rows + 15) / 16 * 16;
-        const uint32_t idesc = idesc_mxf8(TM, n_mma);
-        if (!mbar_wait(&bars->acc_empty[acc_at.slot], acc_at.phase ^ 1u, p.status, 0x603)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t acc = tmem + NT_MAX * acc_at.slot;
-        bool ready = mbar_test(&bars->full[at.slot], at.phase);
-        for (int kt = 0; kt < num_kt; ++kt) {
-          const int s = at.slot;
-          if ((kt & 3) == 0 && !mbar_wait(&bars->sf_full[sf_at.slot], sf_at.phase, p.status, 0x608)) { ok = false; break; }
-          if (!ready && !mbar_wait(&bars->full[s], at.phase, p.status, 0x604)) { ok = false; break; }
-          tc_fence_after();
-          at.next(S);
-          ready = mbar_test(&bars->full[at.slot], at.phase);  // the next stage's, while this one is issued
-          const uint64_t dsa = dsa0 + ((sf_at.slot * 4 + (kt & 3)) * sf_bytes >> 4);
-          tmem_cp_sf(tmem + T_SFW, dsw0 + (s * 512 >> 4));
-          tmem_cp_sf(tmem + T_SFA, dsa);
-          if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, dsa + (512 >> 4));
-          const uint64_t dw = dw0 + (s * stage_bytes >> 4), da = da0 + (s * stage_bytes >> 4);
+    // ---------------- MMA issuer (the whole warp walks, one lane issues).  Stages that are both full go out as a
+    // pair: at few rows the loop around a stage costs more than its MMAs.
+    const bool leader = elect_one();
+    Cursor at, sf_at, acc_at;
+    const uint64_t dw0 = smem_desc_sw128(smem), dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
+    bool ok = true;
+    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
+      Item w;
+      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+      const int n_mma = (w.rows + 15) / 16 * 16;
+      const uint32_t idesc = idesc_mxf8(TM, n_mma);
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc_at.slot], acc_at.phase ^ 1u, p.status, 0x603));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + NT_MAX * acc_at.slot;
+      auto stage = [&](int kt, int s) {
+        const uint64_t dsa = dsa0 + ((sf_at.slot * 4 + (kt & 3)) * sf_bytes >> 4);
+        tmem_cp_sf(tmem + T_SFW, dsw0 + (s * 512 >> 4));
+        tmem_cp_sf(tmem + T_SFA, dsa);
+        if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, dsa + (512 >> 4));
+        const uint64_t dw = dw0 + (s * stage_bytes >> 4), da = dw + (T_W >> 4);
 #pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk)  // K step kk reads scale byte kk of each row's four
-            mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + T_SFW) | (kk << 30),
-                     (tmem + T_SFA) | (kk << 30), (kt | kk) != 0);
-          tc_commit(&bars->empty[s]);
-          if ((kt & 3) == 3 || kt + 1 == num_kt) {
-            tc_commit(&bars->sf_empty[sf_at.slot]);
-            sf_at.next(T_SCALE);
-          }
-        }
+        for (uint32_t kk = 0; kk < 4; ++kk)  // K step kk reads scale byte kk of each row's four
+          mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + T_SFW) | (kk << 30),
+                   (tmem + T_SFA) | (kk << 30), (kt | kk) != 0);
+        tc_commit(&bars->empty[s]);
+      };
+      for (int kt = 0; kt < num_kt;) {
+        if ((kt & 3) == 0) ok = mbar_wait(&bars->sf_full[sf_at.slot], sf_at.phase, p.status, 0x608);
+        const Cursor one = at;
+        at.next(S);
+        const Cursor two = at;
+        const bool pair = ok && (kt & 1) == 0 && kt + 1 < num_kt &&
+                          __all_sync(0xffffffffu, mbar_test2(&bars->full[one.slot], one.phase, &bars->full[two.slot], two.phase));
+        if (!pair) ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->full[one.slot], one.phase, p.status, 0x604));
         if (!ok) break;
-        tc_commit(&bars->acc_full[acc_at.slot]);
-        acc_at.next(2);
+        tc_fence_after();
+        if (leader) {
+          stage(kt, one.slot);
+          if (pair) stage(kt + 1, two.slot);
+        }
+        if (pair) at.next(S);
+        kt += pair ? 2 : 1;
+        if ((kt & 3) == 0 || kt == num_kt) {
+          if (leader) tc_commit(&bars->sf_empty[sf_at.slot]);
+          sf_at.next(T_SCALE);
+        }
       }
-      if (!ok) bars->abort = 1;
+      if (!ok) break;
+      if (leader) tc_commit(&bars->acc_full[acc_at.slot]);
+      acc_at.next(2);
+    }
+    if (!ok) bars->abort = 1;
+    if (leader) {
       tc_commit(&bars->drain);
       mbar_wait(&bars->drain, 0, p.status, 0x605);
     }
@@ -385,41 +397,51 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (a decode step): one launch, bound by the bytes of W.
+// Few rows (a decode step, a short prompt): bound by the bytes of W and, below
+// that, by latency, so one short pipeline per CTA and no persistent walk.
 //
-// A cluster of `split` CTAs owns 128 rows of W and one set of at most 64
-// activation rows (dense: all of them; grouped: one block of one expert); its
-// CTAs take equal ranges of K, so that a narrow W still streams through most
-// SMs.  A CTA keeps its range of the activation resident in shared memory, as
-// swizzled codes and scale chunks made from 16-bit rows (kRaw, quantised here
-// with the rule of qdq_mxfp8) or copied from MXFP8 rows, while W comes through
-// a TMA ring that starts before the previous kernel on the stream has ended.
+// A cluster of `split` CTAs owns 128 rows of W and at most 64 activation rows
+// (dense: a block of rows; grouped: the live slots of one block of one
+// expert); its CTAs take equal ranges of K, so that a narrow W still streams
+// through most SMs.  W comes through a TMA ring that starts before the
+// previous kernel on the stream has ended (dense).  The activation comes
+//   kTiles   by TMA through the same ring, its scales written once for the
+//            CTA's whole range (dense MXFP8 rows);
+//   kQuant   from 16-bit rows, quantised here with the rule of qdq_mxfp8 into
+//            codes resident for the CTA's range (a handful of rows: one
+//            launch instead of two);
+//   kCopy    from MXFP8 rows by token index, resident likewise (grouped).
 // The partial sums meet in distributed shared memory: each CTA adds the
 // cluster's partials of its share of the W rows, always in rank order.
 //
-//   warp 0      TMA producer (W codes and scales)
-//   warp 1      MMA issuer (M = 128, N = n_pad, K = 32)
-//   warps 2-9   activation fill in passes of 256 groups, one barrier a pass,
-//               then the epilogue
+//   warp 0      TMA producer
+//   warp 1      MMA issuer (M = 128, N = rows rounded up to 16, K = 32)
+//   warps 2-9   activation fill in batches of 4 x 256 chunks of 8 elements,
+//               one barrier a batch, then the epilogue
 // ---------------------------------------------------------------------------
+enum { kTiles = 0, kQuant = 1, kCopy = 2 };
 constexpr int F_FILL = 256;
 constexpr int F_THREADS = 64 + F_FILL;
-constexpr int F_RING_MAX = 13, F_PASS_MAX = 16;
-constexpr int F_ROWS_MAX = 64;
-constexpr int F_ACT_MAX = 96 * 1024;      // resident activation bytes of a CTA
+constexpr int F_CHUNKS = TK / 8;          // 8-element chunks of a stage's row
+constexpr int F_UNROLL = 4, F_BATCH = F_UNROLL * F_FILL;
+constexpr int F_RING_MAX = 13, F_BATCH_MAX = 32;
+constexpr int F_ROWS = 64;                // activation rows of an item at the most
+constexpr int F_FILL_MAX = 96 * 1024;     // resident activation bytes of a CTA
 constexpr uint32_t F_TMEM = 128, F_SFW = 64, F_SFA = 68;
 
 struct __align__(8) FBars {
   uint64_t full[F_RING_MAX];
   uint64_t empty[F_RING_MAX];
-  uint64_t ready[F_PASS_MAX];  // the pass's groups are in shared memory
+  uint64_t ready[F_BATCH_MAX];  // the batch's groups (kTiles: all scales) are in shared memory
   uint64_t acc_full;
   uint32_t tmem_base;
   int abort;
+  int live;                     // grouped: live slots of the block
+  int slot[F_ROWS];             // and their numbers
 };
 
 struct FewArgs {
-  const void* a;               // 16-bit rows (kRaw) or codes
+  const void* a;               // 16-bit rows (kQuant) or codes (kCopy)
   int64_t lda;                 // elements / bytes
   const uint8_t* sfa;
   int64_t lds;
@@ -433,33 +455,38 @@ struct FewArgs {
   const int32_t* num_post_padded;
   const float* topk_w;
   int M, N, K, kchunks;        // M: dense rows, grouped slots
-  int rows, n_pad;             // rows of an item (dense M, grouped block size), rounded up to 16
+  int rows, n_pad;             // rows of an item (grouped: block size), rounded up to 16
   int top_k, num_experts;
-  int split, kt_per, ring;     // CTAs of a cluster, K-128 stages per CTA, W stages in the ring
+  int split, kt_per, ring;     // CTAs of a cluster, K-128 stages per CTA, stages in the ring
   float zero;
   int* status;
 };
 
-__host__ __device__ constexpr int f_act_bytes(int n_pad, int kt_per) { return kt_per * (n_pad * TK + 512); }
-
-template <int kDtype, bool kGrouped, bool kRaw>
+template <int kDtype, bool kGrouped, int kAct>
 __global__ void __launch_bounds__(F_THREADS, 1)
-mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ FewArgs p) {
+mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                     const __grid_constant__ FewArgs p) {
   using O = Out16<kDtype>;
   using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // W ring (also the partial sums once the MMAs are done) | activation codes | W scales | activation scales | barriers
-  uint8_t* s_act = smem + p.ring * T_W;
-  uint8_t* s_sfw = s_act + p.kt_per * p.n_pad * TK;
+  // ring (W codes, kTiles: activation codes; the partial sums once the MMAs are done) | resident codes |
+  // W scales | activation scales | barriers
+  const int tile_a = p.n_pad * TK;  // a stage's activation codes
+  const int stage_bytes = T_W + (kAct == kTiles ? tile_a : 0);
+  uint8_t* s_act = smem + p.ring * stage_bytes;
+  uint8_t* s_sfw = s_act + (kAct == kTiles ? 0 : p.kt_per * tile_a);
   uint8_t* s_sfa = s_sfw + p.ring * 512;
   FBars* bars = reinterpret_cast<FBars*>(s_sfa + p.kt_per * 512);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % p.split;
   const int item = static_cast<int>(blockIdx.x) / p.split;
   const int n_tiles = (p.N + TM - 1) / TM;
-  const int blk = kGrouped ? item / n_tiles : 0;
-  const int n_tile = item - blk * n_tiles;
+  // dense: the row blocks of one W tile side by side, so that they share it in L2
+  const int num_m = kGrouped ? 1 : (p.M + p.rows - 1) / p.rows;
+  const int n_tile = kGrouped ? item % n_tiles : item / num_m;
+  const int blk = kGrouped ? item / n_tiles : item - n_tile * num_m;
+  const int row0 = blk * p.rows;  // first row, or first sorted position
   const int num_kt = (p.K + TK - 1) / TK;
   const int kt0 = rank * p.kt_per, nkt = max(0, min(p.kt_per, num_kt - kt0));
 
@@ -469,14 +496,18 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     pdl_wait();  // the routing may come from the kernel before
     expert = __ldcg(p.expert_ids + blk);
     // the whole cluster shares the block, so it leaves as one
-    if (static_cast<int64_t>(blk) * p.rows >= __ldcg(p.num_post_padded) || expert < 0 || expert >= p.num_experts) return;
+    if (row0 >= __ldcg(p.num_post_padded) || expert < 0 || expert >= p.num_experts) return;
   }
   const int w_row = expert * p.N + n_tile * TM;
   const uint8_t* sfw = p.sfw + expert * p.sf_per_expert + (static_cast<int64_t>(n_tile) * p.kchunks + kt0) * 512;
-  auto issue = [&](int kt, int s) {
-    mbar_arrive_expect_tx(&bars->full[s], T_W + 512);
-    tma_load_2d(smem + s * T_W, &tmap_w, (kt0 + kt) * TK, w_row, &bars->full[s]);
+  auto issue_w = [&](int kt, int s) {
+    mbar_arrive_expect_tx(&bars->full[s], stage_bytes + 512);
+    tma_load_2d(smem + s * stage_bytes, &tmap_w, (kt0 + kt) * TK, w_row, &bars->full[s]);
     bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
+  };
+  auto issue_a = [&](int kt, int s) {
+    if (kAct == kTiles)
+      tma_load_2d(smem + s * stage_bytes + T_W, &tmap_a, (kt0 + kt) * TK, row0, &bars->full[s]);
   };
   const int pre = min(p.ring, nkt);
   if (threadIdx.x == 0) {
@@ -484,184 +515,216 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int i = 0; i < F_PASS_MAX; ++i) mbar_init(&bars->ready[i], F_FILL);
+    for (int i = 0; i < F_BATCH_MAX; ++i) mbar_init(&bars->ready[i], F_FILL);
     mbar_init(&bars->acc_full, 1);
     bars->abort = 0;
     fence_barrier_init();
-    for (int kt = 0; kt < pre; ++kt) issue(kt, kt);  // W needs nothing that the previous kernel writes
+    for (int kt = 0; kt < pre; ++kt) issue_w(kt, kt);  // W needs nothing that the previous kernel writes
   }
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, F_TMEM);
     tmem_relinquish();
   }
+  if (kGrouped && warp == 2) {  // the block's live slots, in order
+    int n = 0;
+    for (int r = lane; r < F_ROWS; r += 32) {
+      const int s = r < p.rows ? __ldcg(p.sorted_ids + row0 + r) : -1;
+      const bool ok = s >= 0 && s < p.M;
+      const unsigned bal = __ballot_sync(0xffffffffu, ok);
+      if (ok) bars->slot[n + __popc(bal & ((1u << lane) - 1u))] = s;
+      n += __popc(bal);
+    }
+    if (lane == 0) bars->live = n;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = bars->tmem_base;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);  // uniform
+  const int rows = kGrouped ? bars->live : min(p.rows, p.M - row0);
 
   if (warp == 0) {
-    // ---------------- producer
-    if (elect_one()) {
-      int issued = pre;
-      Cursor at;  // the second lap refills a slot once the first lap's MMAs have completed
-      for (int kt = pre; kt < nkt; ++kt, at.next(p.ring)) {
-        if (!mbar_wait(&bars->empty[at.slot], at.phase, p.status, 0x701)) {
-          bars->abort = 1;
-          break;
-        }
-        if (*(volatile int*)&bars->abort) break;
-        issue(kt, at.slot);
-        ++issued;
-      }
-      for (int kt = max(0, issued - p.ring); kt < issued; ++kt)
-        mbar_wait(&bars->full[kt % p.ring], (kt / p.ring) & 1, p.status, 0x702);
+    // ---------------- producer (the whole warp walks, one lane issues)
+    const bool leader = elect_one();
+    if (kAct == kTiles) {
+      pdl_wait();
+      if (leader)
+        for (int kt = 0; kt < pre; ++kt) issue_a(kt, kt);
     }
+    int issued = pre;
+    Cursor at;  // the second lap refills a slot once the first lap's MMAs have completed
+    bool ok = true;
+    for (int kt = pre; kt < nkt; ++kt, at.next(p.ring)) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[at.slot], at.phase, p.status, 0x701));
+      if (!ok) break;
+      if (leader) {
+        issue_w(kt, at.slot);
+        issue_a(kt, at.slot);
+      }
+      ++issued;
+    }
+    if (!ok) bars->abort = 1;
+    for (int kt = max(0, issued - p.ring); kt < issued; ++kt)
+      mbar_wait(&bars->full[kt % p.ring], (kt / p.ring) & 1, p.status, 0x702);
   } else if (warp == 1) {
     // ---------------- MMA issuer
-    if (elect_one()) {
-      const uint32_t idesc = idesc_mxf8(TM, p.n_pad);
-      bool ok = true;
-      int passes = 0;  // passes seen complete
-      Cursor at;
-      const uint64_t dw0 = smem_desc_sw128(smem), da0 = smem_desc_sw128(s_act);
-      const uint64_t dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
-      for (int kt = 0; kt < nkt; ++kt, at.next(p.ring)) {
-        const int need = ((kt + 1) * 4 * p.rows + F_FILL - 1) / F_FILL;
-        for (; ok && passes < need; ++passes)
-          ok = mbar_wait(&bars->ready[passes], 0, p.status, 0x703) && !*(volatile int*)&bars->abort;
-        const int s = at.slot;
-        if (ok) ok = mbar_wait(&bars->full[s], at.phase, p.status, 0x704);
-        if (!ok) break;
-        tc_fence_after();
-        tmem_cp_sf(tmem + F_SFW, dsw0 + (s * 512 >> 4));
-        tmem_cp_sf(tmem + F_SFA, dsa0 + (kt * 512 >> 4));
-        const uint64_t dw = dw0 + (s * T_W >> 4), da = da0 + (kt * p.n_pad * TK >> 4);
+    const bool leader = elect_one();
+    const uint32_t idesc = idesc_mxf8(TM, (max(rows, 1) + 15) / 16 * 16);
+    bool ok = true;
+    int batches = 0, covered = 0;  // batches seen complete, and the chunks in them
+    Cursor at;
+    const uint64_t dw0 = smem_desc_sw128(smem), da0 = smem_desc_sw128(kAct == kTiles ? smem + T_W : s_act);
+    const uint64_t dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
+    auto stage = [&](int kt, int s) {
+      tmem_cp_sf(tmem + F_SFW, dsw0 + (s * 512 >> 4));
+      tmem_cp_sf(tmem + F_SFA, dsa0 + (kt * 512 >> 4));
+      const uint64_t dw = dw0 + (s * stage_bytes >> 4);
+      const uint64_t da = da0 + ((kAct == kTiles ? s * stage_bytes : kt * tile_a) >> 4);
 #pragma unroll
-        for (uint32_t kk = 0; kk < 4; ++kk)
-          mma_mxf8(tmem, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + F_SFW) | (kk << 30),
-                   (tmem + F_SFA) | (kk << 30), (kt | kk) != 0);
-        tc_commit(&bars->empty[s]);
-      }
-      if (!ok) bars->abort = 1;
-      tc_commit(&bars->acc_full);  // also on abort: the epilogue waits for the issued MMAs
-    }
-  } else {
-    // ---------------- activation fill: group g of row r of stage kt, four neighbouring lanes a stage's row
-    if (!kGrouped) pdl_wait();
-    const int t = threadIdx.x - 64;
-    const int groups = nkt * 4 * p.rows, passes = (groups + F_FILL - 1) / F_FILL;
-    uint4 v[4];
-    uint32_t sb = 0;
-    int kt = 0, r = 0, g = 0;
-    bool live = false;
-    auto fetch = [&](int i) {
-      kt = i / (4 * p.rows);
-      const int j = i - kt * 4 * p.rows;
-      r = j >> 2;
-      g = j & 3;
-      live = false;
-      if (i >= groups) return;
-      int tok = r;
-      if (kGrouped) {
-        const int s = __ldcg(p.sorted_ids + static_cast<int64_t>(blk) * p.rows + r);
-        if (s < 0 || s >= p.M) return;
-        tok = s / p.top_k;
-      }
-      const int k = (kt0 + kt) * TK + g * 32;  // element of K
-      live = true;
-      sb = 0;
-      if (k >= p.K) {  // behind K: zero codes with scale 2^-127
-        v[0] = v[1] = v[2] = v[3] = make_uint4(0, 0, 0, 0);
-      } else if (kRaw) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a) + tok * p.lda + k);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = __ldcg(src + q);
-      } else {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.a) + tok * p.lda + k);
-        v[0] = __ldcg(src);
-        v[1] = __ldcg(src + 1);
-        sb = __ldcg(p.sfa + tok * p.lds + (k >> 5));
-      }
+      for (uint32_t kk = 0; kk < 4; ++kk)
+        mma_mxf8(tmem, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + F_SFW) | (kk << 30),
+                 (tmem + F_SFA) | (kk << 30), (kt | kk) != 0);
+      tc_commit(&bars->empty[s]);
     };
-    fetch(t);
-    for (int pass = 0; pass < passes; ++pass) {
-      if (live) {
-        uint4 c0 = v[0], c1 = v[1];
-        if (kRaw) {
-          const uint32_t amax = max(max(absmax8(v[0]), absmax8(v[1])), max(absmax8(v[2]), absmax8(v[3])));
-          const int e = mx8_exp<kDtype>(amax);
-          sb = static_cast<uint32_t>(e);
-          const uint2 q0 = mx8_chunk_codes<kDtype>(v[0], e, p.zero), q1 = mx8_chunk_codes<kDtype>(v[1], e, p.zero);
-          const uint2 q2 = mx8_chunk_codes<kDtype>(v[2], e, p.zero), q3 = mx8_chunk_codes<kDtype>(v[3], e, p.zero);
-          c0 = make_uint4(q0.x, q0.y, q1.x, q1.y);
-          c1 = make_uint4(q2.x, q2.y, q3.x, q3.y);
-        }
-        // 128-byte swizzle: 16-byte chunk c of row r sits at chunk c ^ (r % 8)
-        uint8_t* row = s_act + kt * p.n_pad * TK + r * TK;
-        *reinterpret_cast<uint4*>(row + (((2 * g) ^ (r & 7)) << 4)) = c0;
-        *reinterpret_cast<uint4*>(row + (((2 * g + 1) ^ (r & 7)) << 4)) = c1;
-        s_sfa[kt * 512 + (r & 31) * 16 + (r >> 5) * 4 + g] = static_cast<uint8_t>(sb);
+    for (int kt = 0; kt < nkt;) {
+      const int need = kAct == kTiles ? 1 : (kt + 1) * F_CHUNKS * rows;
+      for (; ok && covered < need; covered += F_BATCH) ok = mbar_wait(&bars->ready[batches++], 0, p.status, 0x703);
+      const Cursor one = at;
+      at.next(p.ring);
+      const Cursor two = at;
+      const bool pair = ok && kt + 1 < nkt && (kAct == kTiles || covered >= need + F_CHUNKS * rows) &&
+                        __all_sync(0xffffffffu, mbar_test2(&bars->full[one.slot], one.phase, &bars->full[two.slot], two.phase));
+      if (!pair) ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->full[one.slot], one.phase, p.status, 0x704));
+      if (!ok) break;
+      tc_fence_after();
+      if (leader) {
+        stage(kt, one.slot);
+        if (pair) stage(kt + 1, two.slot);
       }
-      if (pass + 1 < passes) fetch(t + (pass + 1) * F_FILL);
+      if (pair) at.next(p.ring);
+      kt += pair ? 2 : 1;
+    }
+    if (!ok) bars->abort = 1;
+    if (leader) tc_commit(&bars->acc_full);  // also on abort: the epilogue waits for the issued MMAs
+  } else if (kAct == kTiles) {
+    // ---------------- activation scales: a row's four bytes per stage, neighbouring lanes along the row (with
+    // neighbouring lanes down the rows, the SMs' reads of the same few lines queued for 3 us)
+    pdl_wait();
+    const int words = nkt * rows;
+    for (int i0 = threadIdx.x - 64; i0 < words; i0 += 2 * F_FILL) {
+      uint32_t v[2];
+      int at[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = i0 + u * F_FILL, r = i / nkt, kt = i - r * nkt;
+        at[u] = kt * 512 + (r & 31) * 16 + (r >> 5) * 4;
+        if (i < words) v[u] = __ldcg(reinterpret_cast<const uint32_t*>(p.sfa + (row0 + r) * p.lds + (kt0 + kt) * 4));
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (i0 + u * F_FILL < words) *reinterpret_cast<uint32_t*>(s_sfa + at[u]) = v[u];
+    }
+    fence_proxy_async_smem();
+    mbar_arrive(&bars->ready[0]);
+  } else {
+    // ---------------- activation fill: chunk j (8 elements) of a stage's row, four neighbouring lanes a scale group
+    if (!kGrouped) pdl_wait();
+    const int chunks = nkt * F_CHUNKS * rows, per_stage = F_CHUNKS * rows;
+    int batch = 0;
+    for (int i0 = threadIdx.x - 64; i0 < (chunks + F_FILL - 1) / F_FILL * F_FILL; i0 += F_BATCH, ++batch) {
+      uint4 v[F_UNROLL];
+      uint32_t sb[F_UNROLL];
+#pragma unroll
+      for (int u = 0; u < F_UNROLL; ++u) {
+        const int i = i0 + u * F_FILL, kt = i / per_stage, j = i - kt * per_stage, r = j / F_CHUNKS, c = j % F_CHUNKS;
+        const int k = (kt0 + kt) * TK + c * 8;  // element of K; behind K: zero codes with scale 2^-127
+        v[u] = make_uint4(0, 0, 0, 0);
+        sb[u] = 0;
+        if (i < chunks && k < p.K) {
+          const int64_t tok = kGrouped ? bars->slot[r] / p.top_k : row0 + r;
+          if (kAct == kQuant) {
+            v[u] = __ldcg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.a) + tok * p.lda + k));
+          } else {
+            const uint2 w = __ldcg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(p.a) + tok * p.lda + k));
+            v[u].x = w.x;
+            v[u].y = w.y;
+            sb[u] = __ldcg(p.sfa + tok * p.lds + (k >> 5));
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < F_UNROLL; ++u) {
+        const int i = i0 + u * F_FILL, kt = i / per_stage, j = i - kt * per_stage, r = j / F_CHUNKS, c = j % F_CHUNKS;
+        uint2 code = make_uint2(v[u].x, v[u].y);
+        if (kAct == kQuant) {
+          uint32_t amax = absmax8(v[u]);  // the lanes of a group walk together
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int e = mx8_exp<kDtype>(amax);
+          sb[u] = static_cast<uint32_t>(e);
+          code = mx8_chunk_codes<kDtype>(v[u], e, p.zero);
+        }
+        if (i < chunks) {
+          // 128-byte swizzle: 16-byte chunk h of row r sits at chunk h ^ (r % 8)
+          *reinterpret_cast<uint2*>(s_act + kt * tile_a + r * TK + (((c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8) = code;
+          if ((c & 3) == 0) s_sfa[kt * 512 + (r & 31) * 16 + (r >> 5) * 4 + (c >> 2)] = static_cast<uint8_t>(sb[u]);
+        }
+      }
       fence_proxy_async_smem();
-      mbar_arrive(&bars->ready[pass]);
+      mbar_arrive(&bars->ready[batch]);
     }
   }
 
-  // ---------------- epilogue (warps 2-9): TMEM lanes = W rows, columns = activation rows
+  // ---------------- epilogue (warps 2-9): TMEM lanes = W rows, columns = activation rows.  The sums go through
+  // shared memory, so that one short loop stores them in whole lines (an unrolled store per column cost 1.4 us of
+  // instruction fetches).
   float* part = reinterpret_cast<float*>(smem);
-  T* C = static_cast<T*>(p.c);
-  const int q = warp & 3, half = (warp - 2) >> 2;
   bool ok = true;
-  // output row of activation row r, -1: none
-  auto out_row = [&](int r) {
-    if (!kGrouped) return r < p.rows ? r : -1;
-    if (r >= p.rows) return -1;
-    const int s = __ldcg(p.sorted_ids + static_cast<int64_t>(blk) * p.rows + r);
-    return s < p.M ? s : -1;
-  };
-  auto store = [&](int s, int n, float v) {
-    if (s < 0 || n >= p.N) return;
-    if (kGrouped) v *= p.topk_w != nullptr ? __ldcg(p.topk_w + s) : 1.0f;
-    else if (p.bias != nullptr) v += O::load(static_cast<const T*>(p.bias) + n);
-    C[static_cast<int64_t>(s) * p.ldc + n] = O::one(v);
-  };
   if (warp >= 2) {
+    const int q = warp & 3, half = (warp - 2) >> 2;
     ok = mbar_wait(&bars->acc_full, 0, p.status, 0x705);
     ok = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
     tc_fence_after();
-    if (32 * half < p.rows) {
-      uint32_t acc[32];
-      tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + 32 * half, acc);
+    for (int c = 16 * half; c < rows; c += 32) {
+      uint32_t acc[16];
+      tmem_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + c, acc);
       tmem_ld_wait();
-      const int row = q * 32 + lane;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const int r = 32 * half + i;
-        if (r < p.rows) {
-          const float v = nkt > 0 ? __uint_as_float(acc[i]) : 0.f;
-          if (p.split > 1) part[r * TM + row] = v;
-          else if (ok) store(out_row(r), n_tile * TM + row, v);
-        }
+      for (int i = 0; i < 16; ++i)
+        if (c + i < rows) part[(c + i) * TM + q * 32 + lane] = nkt > 0 ? __uint_as_float(acc[i]) : 0.f;
+    }
+  }
+  __syncwarp();
+  if (p.split > 1) cluster_sync();  // every CTA's partials are in its shared memory
+  else __syncthreads();
+  if (warp >= 2 && ok) {
+    // thread: one of this CTA's W rows, every `step`-th activation row
+    const int shift = __ffs(TM / p.split) - 1, t = threadIdx.x - 64, step = F_FILL >> shift;
+    const int row = (rank << shift) + (t & ((1 << shift) - 1)), n = n_tile * TM + row;
+    T* C = static_cast<T*>(p.c) + n;
+    const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+#pragma unroll 2
+    for (int r = t >> shift; r < rows && n < p.N; r += step) {
+      float v;
+      if (p.split == 1) {
+        v = part[r * TM + row];
+      } else {
+        float x[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          if (c < p.split)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[c]) : "r"(cluster_addr(part + r * TM + row, c)));
+        v = x[0];
+#pragma unroll
+        for (int c = 1; c < 8; ++c)
+          if (c < p.split) v += x[c];
       }
+      const int64_t s = kGrouped ? bars->slot[r] : row0 + r;
+      if (kGrouped) v *= p.topk_w != nullptr ? __ldcg(p.topk_w + s) : 1.0f;
+      else v += bias;
+      C[s * p.ldc] = O::one(v);
     }
   }
   if (p.split > 1) {
-    __syncwarp();
-    cluster_sync();  // every CTA's partials are in its shared memory
-    if (warp >= 2 && ok) {
-      const int share = TM / p.split;  // W rows this CTA adds up
-      for (int i = threadIdx.x - 64; i < share * p.rows; i += F_FILL) {
-        const int r = i / share, row = rank * share + (i - r * share);
-        float v = 0.f;
-        for (int c = 0; c < p.split; ++c) {
-          float x;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(cluster_addr(part + r * TM + row, c)));
-          v += x;
-        }
-        store(out_row(r), n_tile * TM + row, v);
-      }
-    }
     __syncwarp();
     cluster_sync();  // no CTA leaves while another reads its partials
   }
@@ -816,36 +879,37 @@ int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, c
 }
 
 // How a few-rows launch splits: `split` CTAs of a cluster share an item's K so
-// that the items fill the SMs; 0: the rows do not fit (see F_ACT_MAX).
+// that the items fill the SMs; split 0: the launch does not fit.
 struct FewPlan {
   int split, kt_per, ring;
   size_t smem;
 };
-FewPlan few_plan(int64_t items, int rows, int64_t K) {
+FewPlan few_plan(int64_t items, int rows, int64_t K, int act) {
   FewPlan f = {0, 0, 0, 0};
-  if (rows < 1 || rows > F_ROWS_MAX) return f;
   const int num_kt = static_cast<int>((K + TK - 1) / TK), n_pad = (rows + 15) / 16 * 16;
   int split = 1;
   while (split < 8 && items * split * 2 <= device_sm_count() && num_kt >= split * 4) split *= 2;
   f.kt_per = (num_kt + split - 1) / split;
-  if (f_act_bytes(n_pad, f.kt_per) > F_ACT_MAX) return f;
-  if ((f.kt_per * 4 * rows + F_FILL - 1) / F_FILL > F_PASS_MAX) return f;
-  const int room = (kSmemMax - 1024 - static_cast<int>(sizeof(FBars)) - f_act_bytes(n_pad, f.kt_per)) / (T_W + 512);
+  const int64_t resident = static_cast<int64_t>(f.kt_per) * ((act == kTiles ? 0 : n_pad * TK) + 512);
+  if (resident > F_FILL_MAX || (act != kTiles && f.kt_per * F_CHUNKS * rows > F_BATCH_MAX * F_BATCH)) return f;
+  const int stage = T_W + (act == kTiles ? n_pad * TK : 0);
+  const int room = (kSmemMax - 1024 - static_cast<int>(sizeof(FBars)) - static_cast<int>(resident)) / (stage + 512);
   // the ring also holds the partial sums, 512 bytes an activation row
-  f.ring = std::max(std::min(std::min(room, F_RING_MAX), f.kt_per), (n_pad * TM * 4 + T_W - 1) / T_W);
+  f.ring = std::max(std::min(std::min(room, F_RING_MAX), f.kt_per), (n_pad * TM * 4 + stage - 1) / stage);
   if (f.ring > room) return f;
-  f.smem = 1024 + sizeof(FBars) + f_act_bytes(n_pad, f.kt_per) + static_cast<size_t>(f.ring) * (T_W + 512);
+  f.smem = 1024 + sizeof(FBars) + resident + static_cast<size_t>(f.ring) * (stage + 512);
   f.split = split;
   return f;
 }
 
-template <int kDtype, bool kGrouped, bool kRaw>
-int launch_few(const char* who, const CUtensorMap& tw, const FewArgs& p, int64_t items, size_t smem, cudaStream_t s) {
+template <int kDtype, bool kGrouped, int kAct>
+int launch_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, const FewArgs& p, int64_t items,
+               size_t smem, cudaStream_t s) {
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(&mxf8_few_rows_kernel<kDtype, kGrouped, kRaw>,
+    const cudaError_t e = cudaFuncSetAttribute(&mxf8_few_rows_kernel<kDtype, kGrouped, kAct>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
     attr_set[dev] = true;
@@ -864,25 +928,22 @@ int launch_few(const char* who, const CUtensorMap& tw, const FewArgs& p, int64_t
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mxf8_few_rows_kernel<kDtype, kGrouped, kRaw>, tw, p);
+  cfg.numAttrs = p.split > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mxf8_few_rows_kernel<kDtype, kGrouped, kAct>, tw, ta, p);
   if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
   return check_launch(who);
 }
 
-template <bool kGrouped>
-int run_few(const char* who, const CUtensorMap& tw, FewArgs& p, const FewPlan& f, int64_t items, int dtype, bool raw,
-            cudaStream_t s) {
+template <bool kGrouped, int kAct>
+int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewArgs& p, const FewPlan& f,
+            int64_t items, int dtype, cudaStream_t s) {
   p.split = f.split;
   p.kt_per = f.kt_per;
   p.ring = f.ring;
   p.n_pad = (p.rows + 15) / 16 * 16;
   p.zero = 0.0f;  // +0.0 as an operand the compiler cannot fold (see mx8_scaled)
-  if (dtype == QDQ_DTYPE_FP16)
-    return raw ? launch_few<QDQ_DTYPE_FP16, kGrouped, true>(who, tw, p, items, f.smem, s)
-               : launch_few<QDQ_DTYPE_FP16, kGrouped, false>(who, tw, p, items, f.smem, s);
-  return raw ? launch_few<QDQ_DTYPE_BF16, kGrouped, true>(who, tw, p, items, f.smem, s)
-             : launch_few<QDQ_DTYPE_BF16, kGrouped, false>(who, tw, p, items, f.smem, s);
+  return dtype == QDQ_DTYPE_FP16 ? launch_few<QDQ_DTYPE_FP16, kGrouped, kAct>(who, tw, ta, p, items, f.smem, s)
+                                 : launch_few<QDQ_DTYPE_BF16, kGrouped, kAct>(who, tw, ta, p, items, f.smem, s);
 }
 
 // Rows per item for `rows` wanted, in whole TMA boxes of 64, 32 or 16 rows: a
@@ -913,13 +974,18 @@ using namespace qdqb200;
 namespace qdqb200 {
 namespace {
 
-// The few-rows launch of a dense product, or false where its rows do not fit.
+// The few-rows launch of a dense product from MXFP8 rows (raw == false) or
+// 16-bit rows; false where the tiled kernel takes it.
 bool dense_few(const char* who, const void* a, int64_t lda, const void* a_scales, int64_t lds, bool raw,
                const void* w_codes, const void* w_sf_tiled, const void* bias, void* c, int64_t M, int64_t N, int64_t K,
                int64_t ldw, int64_t ldc, int dtype, cudaStream_t s, int* st) {
   const int64_t n_tiles = (N + TM - 1) / TM;
-  const FewPlan f = M <= F_ROWS_MAX ? few_plan(n_tiles, static_cast<int>(M), K) : FewPlan{0, 0, 0, 0};
-  if (f.split == 0) return false;
+  const int rows = static_cast<int>(std::min<int64_t>(M, F_ROWS));
+  const int64_t items = n_tiles * ((M + rows - 1) / rows);
+  if (items > device_sm_count()) return false;
+  const FewPlan f = few_plan(items, rows, K, raw ? kQuant : kTiles);
+  // 16-bit rows are quantised in the kernel while a CTA's share is one batch of its fill
+  if (f.split == 0 || (raw && (M > F_ROWS || f.kt_per * F_CHUNKS * M > F_BATCH))) return false;
   FewArgs p = {};
   p.a = a;
   p.lda = lda;
@@ -929,15 +995,19 @@ bool dense_few(const char* who, const void* a, int64_t lda, const void* a_scales
   p.bias = bias;
   p.c = c;
   p.ldc = ldc;
-  p.M = p.rows = static_cast<int>(M);
+  p.M = static_cast<int>(M);
+  p.rows = rows;
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
   p.top_k = 1;
   p.status = device_status_ptr();
-  CUtensorMap tw;
+  CUtensorMap tw, ta = {};
   *st = p.status == nullptr ? QDQ_ERR_CUDA : make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128);
-  if (*st == QDQ_OK) *st = run_few<false>(who, tw, p, f, n_tiles, dtype, raw, s);
+  if (*st == QDQ_OK && !raw) *st = make_tmap_u8_2d(&ta, a, M, K, lda, TK, (rows + 15) / 16 * 16, 128);
+  if (*st == QDQ_OK)
+    *st = raw ? run_few<false, kQuant>(who, tw, ta, p, f, items, dtype, s)
+              : run_few<false, kTiles>(who, tw, ta, p, f, items, dtype, s);
   return true;
 }
 
@@ -1071,7 +1141,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   const int64_t n_slots = size_m * top_k;
   // A decode step of few blocks: one launch without quantisation pass or segments, an item per block.
   if (num_blocks * n_tiles <= 2 * device_sm_count()) {
-    const FewPlan f = few_plan(num_blocks * n_tiles, moe_block_size, K);
+    const FewPlan f = few_plan(num_blocks * n_tiles, moe_block_size, K, a ? kQuant : kCopy);
     if (f.split != 0) {
       FewArgs p = {};
       p.a = a ? a : a_codes;
@@ -1094,7 +1164,9 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
       p.top_k = top_k;
       p.num_experts = static_cast<int>(num_experts);
       p.status = status;
-      return run_few<true>(who, tw, p, f, num_blocks * n_tiles, dtype, a != nullptr, s);
+      ta = {};
+      return a ? run_few<true, kQuant>(who, tw, ta, p, f, num_blocks * n_tiles, dtype, s)
+               : run_few<true, kCopy>(who, tw, ta, p, f, num_blocks * n_tiles, dtype, s);
     }
   }
   int32_t* seg_tab = static_cast<int32_t*>(workspace);
