@@ -84,6 +84,15 @@ struct Out16<QDQ_DTYPE_FP16> {
   __device__ static T one(float a) { return __float2half_rn(a); }
 };
 
+// E4M3 codes of a 16-byte chunk of a 32-group with scale exponent e.
+template <int kDtype>
+__device__ __forceinline__ uint2 chunk_codes(const uint4& v, int e, float zero) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t c[2];
+  mx8_codes<kDtype>(w, e, zero, c);
+  return make_uint2(c[0], c[1]);
+}
+
 struct GemmArgs {
   const uint8_t* sfw;          // tiled W scales
   int64_t sf_per_expert;
@@ -661,7 +670,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
           amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
           const int e = mx8_exp<kDtype>(amax);
           sb[u] = static_cast<uint32_t>(e);
-          code = mx8_chunk_codes<kDtype>(v[u], e, p.zero);
+          code = chunk_codes<kDtype>(v[u], e, p.zero);
         }
         if (i < chunks) {
           // 128-byte swizzle: 16-byte chunk h of row r sits at chunk h ^ (r % 8)
@@ -826,7 +835,7 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int e = mx8_exp<kDtype>(amax);
         if (c < 4 * gpr) {
-          *reinterpret_cast<uint2*>(dst + 8 * c) = mx8_chunk_codes<kDtype>(v, e, zero);
+          *reinterpret_cast<uint2*>(dst + 8 * c) = chunk_codes<kDtype>(v, e, zero);
           if ((c & 3) == 0) scales[pos * ldso + (c >> 2)] = static_cast<uint8_t>(e);
         }
       }

@@ -281,22 +281,67 @@ __device__ __forceinline__ float2 mx8_scaled(float a, float b, float inv, float 
   return t;
 }
 
-// E4M3 codes of eight elements (one 16-byte chunk) of a 32-group with scale
-// exponent e: the codes mxfp8_vec_kernel emits for the same group.
-template <int kDtype>
-__device__ __forceinline__ uint2 mx8_chunk_codes(const uint4& v, int e, float zero) {
+// E4M3 codes of a bf16 pair, w = x * inv with inv >= 2^-16 a power of two (as
+// a bf16 pair): the product is exact in bf16 and fma(x, inv, +0) makes a -0
+// quotient +0; magnitudes in [7, 8) * 2^-9 (bf16 0x3C60 .. 0x3C7F) lose their
+// low mantissa bits as in mx8_pair_f16.
+__device__ __forceinline__ uint32_t mx8_pair_bf16(uint32_t x, uint32_t inv2, uint32_t zero2) {
+  uint32_t t, eq, out;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(t) : "r"(x), "r"(inv2), "r"(zero2));
+  asm("{\n\t.reg .b32 m;\n\t"
+      "and.b32 m, %1, 0x7FE07FE0;\n\t"
+      "set.eq.u32.f16x2 %0, m, %2;\n\t}"  // equal bits: both are ordinary f16 numbers where they are equal
+      : "=r"(eq)
+      : "r"(t), "r"(0x3C603C60u));
+  t &= ~(eq & 0x001F001Fu);
+  asm("{\n\t.reg .b16 p;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 p, %2, %1;\n\t"
+      "cvt.u32.u16 %0, p;\n\t}"
+      : "=r"(out)
+      : "f"(bf16lo(t)), "f"(bf16hi(t)));
+  return out;
+}
+
+// E4M3 codes of the elements in kW words (two each) of a 32-group with scale
+// exponent e, four per output word: the codes mxfp8_vec_kernel emits.
+template <int kDtype, int kW>
+__device__ __forceinline__ void mx8_codes(const uint32_t (&w)[kW], int e, float zero, uint32_t (&code)[kW / 2]) {
   using F = Fmt<kDtype>;
   const float inv = pow2f(127 - e);
-  const bool fast = e <= 143;
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  uint32_t p[4];
+  uint32_t p[kW];
+  if (e <= 143) {
+    if (kDtype == QDQ_DTYPE_BF16) {
+      const uint32_t inv2 = pack_bf16x2(inv, inv), zero2 = __float_as_uint(zero);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 t = mx8_scaled(F::lo(w[j]), F::hi(w[j]), inv, zero, fast);
-    uint32_t h;
-    p[j] = fast ? mx8_pair_f16(pack_f16x2(t.x, t.y), h) : e4m3x2_roundtrip(mx8_sub_clamp(t.x), mx8_sub_clamp(t.y), h);
+      for (int j = 0; j < kW; ++j) p[j] = mx8_pair_bf16(w[j], inv2, zero2);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kW; ++j) {
+        const float2 t = mx8_scaled(F::lo(w[j]), F::hi(w[j]), inv, zero, true);
+        uint32_t h;
+        p[j] = mx8_pair_f16(pack_f16x2(t.x, t.y), h);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kW; ++j) {
+      const float2 t = mx8_scaled(F::lo(w[j]), F::hi(w[j]), inv, zero, false);
+      uint32_t h;
+      p[j] = e4m3x2_roundtrip(mx8_sub_clamp(t.x), mx8_sub_clamp(t.y), h);
+    }
   }
-  return make_uint2(p[0] | (p[1] << 16), p[2] | (p[3] << 16));
+#pragma unroll
+  for (int j = 0; j < kW / 2; ++j) code[j] = __byte_perm(p[2 * j], p[2 * j + 1], 0x5410);
+}
+
+// Maximum magnitude bits of the 16-bit elements in kW words; a NaN gives an
+// all-ones exponent, as an infinity does.
+template <int kDtype, int kW>
+__device__ __forceinline__ uint32_t absmax_words(const uint32_t (&w)[kW]) {
+  uint32_t m = w[0] & 0x7FFF7FFFu;
+#pragma unroll
+  for (int j = 1; j < kW; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+  return max(m & 0xFFFFu, m >> 16);
 }
 
 }  // namespace

@@ -16,8 +16,8 @@
 // loads 16 scales (512 elements of K) of a row at once and its last stage
 // finds 2^-127 rather than a stale NaN behind K.
 //
-// All three are one HBM pass: a lane owns 16-byte chunks (8 elements), the
-// four lanes of a group exchange their maxima by shuffles.
+// All three are one HBM pass: a lane owns units of 16 elements (two 16-byte
+// loads), the two lanes of a group exchange their maxima by a shuffle.
 #include <algorithm>
 #include <cstring>
 
@@ -30,95 +30,140 @@ namespace {
 using namespace sm100;
 
 constexpr uint32_t kAll = 0xFFFFFFFFu;
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;  // silu_mul [4096, 14336]: 49.4 us, at 256 threads 53.2, at 64 54.8
 
-// Scale exponent of the 32-group this lane's chunk belongs to (four
-// neighbouring lanes hold the group).
-template <int kDtype>
-__device__ __forceinline__ int group_exp(const uint4& y) {
-  uint32_t amax = absmax8(y);
-  amax = max(amax, __shfl_xor_sync(kAll, amax, 1));
-  amax = max(amax, __shfl_xor_sync(kAll, amax, 2));
-  return mx8_exp<kDtype>(amax);
+struct Unit {  // 16 elements of a row
+  uint4 a, b;
+};
+
+// One 32-byte access where every row starts on a 32-byte boundary (kWide),
+// two of 16 bytes elsewhere: the halves of a sector are then fetched apart.
+template <bool kWide>
+__device__ __forceinline__ Unit load_unit(const uint16_t* p) {
+  Unit u;
+  if (kWide) {
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(u.a.x), "=r"(u.a.y), "=r"(u.a.z), "=r"(u.a.w), "=r"(u.b.x), "=r"(u.b.y), "=r"(u.b.z), "=r"(u.b.w)
+                 : "l"(p));
+  } else {
+    const uint4* q = reinterpret_cast<const uint4*>(p);
+    u = {ld_stream(q), ld_stream(q + 1)};
+  }
+  return u;
+}
+template <bool kWide>
+__device__ __forceinline__ void store_unit(uint16_t* p, const Unit& u) {
+  if (kWide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u.a.x), "r"(u.a.y), "r"(u.a.z),
+                 "r"(u.a.w), "r"(u.b.x), "r"(u.b.y), "r"(u.b.z), "r"(u.b.w)
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(p)[0] = u.a;
+    reinterpret_cast<uint4*>(p)[1] = u.b;
+  }
+}
+__device__ __forceinline__ Unit zero_unit() { return {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)}; }
+__device__ __forceinline__ void words(const Unit& u, uint32_t (&w)[8]) {
+  w[0] = u.a.x, w[1] = u.a.y, w[2] = u.a.z, w[3] = u.a.w;
+  w[4] = u.b.x, w[5] = u.b.y, w[6] = u.b.z, w[7] = u.b.w;
+}
+__device__ __forceinline__ Unit unit_of(const uint32_t (&w)[8]) {
+  return {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
 
-// Codes and scale of one chunk; chunk `col` of a row of cpr chunks.  The lane
-// of the row's last group also clears the scale bytes behind K / 32.
-__device__ __forceinline__ void store_chunk(uint8_t* codes_row, uint8_t* scales_row, uint32_t col, uint32_t cpr,
-                                            uint2 code, int e) {
-  *reinterpret_cast<uint2*>(codes_row + col * 8u) = code;
-  if ((col & 3u) == 0) {
-    const uint32_t g = col >> 2, gpr = cpr >> 2;
-    scales_row[g] = static_cast<uint8_t>(e);
-    if (g + 1 == gpr)
-      for (uint32_t p = gpr; p < ((gpr + 15u) & ~15u); ++p) scales_row[p] = 0;
+// MXFP8 of unit `col` (of upr in the row): codes, and from the group's first
+// lane the scale; behind the last group also the zeros up to a multiple of 16
+// scales.  Every lane of the warp takes part in the shuffle.
+template <int kDtype>
+__device__ __forceinline__ void store_mxfp8(const uint32_t (&y)[8], uint8_t* codes_row, uint8_t* scales_row,
+                                            uint32_t col, uint32_t upr, bool live, float zero) {
+  uint32_t amax = absmax_words<kDtype>(y);
+  amax = max(amax, __shfl_xor_sync(kAll, amax, 1));
+  const int e = mx8_exp<kDtype>(amax);
+  if (!live) return;
+  uint32_t c[4];
+  mx8_codes<kDtype>(y, e, zero, c);
+  *reinterpret_cast<uint4*>(codes_row + col * 16u) = make_uint4(c[0], c[1], c[2], c[3]);
+  if ((col & 1u) == 0) {
+    scales_row[col >> 1] = static_cast<uint8_t>(e);
+    if (col + 2 == upr)
+      for (uint32_t p = upr >> 1; p < (((upr >> 1) + 15u) & ~15u); ++p) scales_row[p] = 0;
   }
 }
 
-// silu(g) * u without overflow of exp: t = exp(-|g|) <= 1.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// silu(g) * u: with t = exp(-|g|), silu(g) = g (g < 0 ? t : 1) / (1 + t), which
+// overflows nowhere.  t and 1 are carried times 2^24, so that ex2 (which
+// flushes subnormals) reaches down to |g| = 104, where silu is below 2^-140.
 __device__ __forceinline__ float silu_mul(float g, float u) {
-  const float t = __expf(-fabsf(g));
-  return g * __fdividef(g < 0.f ? t : 1.0f, 1.0f + t) * u;
+  const float t = ex2_approx(fmaf(-1.44269504088896341f, fabsf(g), 24.0f));
+  return g * ((g < 0.f ? t : 0x1p24f) * rcp_approx(t + 0x1p24f)) * u;
 }
 
 // ---------------------------------------------------------------------------
-// rows / silu_mul: a flat walk over the 16-byte chunks of all rows.
+// rows / silu_mul: `tpr` threads (a power of two, at least 2) of gridDim.y
+// CTAs walk a row, the next unit's loads in flight while one is converted.
+// Addresses are formed once a row: silu_mul issues 20 instructions an element,
+// near what the SMs can while HBM delivers it (as a flat walk with a division
+// and three row products per unit it took 27, and 55 us instead of 49 for
+// [4096, 14336], where HBM alone needs 45).
 // ---------------------------------------------------------------------------
-template <int kDtype, bool kSilu>
+template <int kDtype, bool kSilu, bool kWide>
 __global__ void __launch_bounds__(kRowThreads)
-rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                  uint32_t cpr, uint64_t total, int64_t ldx, int64_t ldc, int64_t lds, float zero) {
+rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t M,
+                  uint32_t upr, uint32_t tpr, int64_t ldx, int64_t ldc, int64_t lds, float zero) {
   using F = Fmt<kDtype>;
-  constexpr int kU = kSilu ? 2 : 4;  // chunks in flight per lane (silu_mul: two loads each)
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x * kU;
-  const bool narrow = total <= 0xFFFFFFFFull;
-  for (uint64_t base = (static_cast<uint64_t>(blockIdx.x) * blockDim.x + (threadIdx.x & ~31u)) * kU; base < total;
-       base += stride) {
-    uint4 v[kU], u[kU];
-    uint64_t row[kU];
-    uint32_t col[kU];
-#pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      const uint64_t c = base + static_cast<uint64_t>(i) * 32u + lane;
-      row[i] = narrow ? static_cast<uint32_t>(c) / cpr : c / cpr;
-      col[i] = static_cast<uint32_t>(c - row[i] * cpr);
-      v[i] = u[i] = make_uint4(0, 0, 0, 0);
-      if (c < total) {
-        const uint16_t* p = x + row[i] * ldx + col[i] * 8u;
-        v[i] = ld_stream(reinterpret_cast<const uint4*>(p));
-        if (kSilu) u[i] = ld_stream(reinterpret_cast<const uint4*>(p + cpr * 8u));
-      }
+  const uint32_t rpc = kRowThreads / tpr, t = threadIdx.x & (tpr - 1);
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * rpc + threadIdx.x / tpr;
+  const bool in_m = row < M;
+  const uint16_t* xr = x + row * ldx;
+  const uint16_t* ur = xr + upr * 16u;
+  uint8_t* cr = codes + row * ldc;
+  uint8_t* sr = scales + row * lds;
+  const uint32_t step = tpr * gridDim.y, first = tpr * blockIdx.y + t;
+  Unit v = zero_unit(), u = zero_unit();
+  if (in_m && first < upr) {
+    v = load_unit<kWide>(xr + first * 16u);
+    if (kSilu) u = load_unit<kWide>(ur + first * 16u);
+  }
+  for (uint32_t col0 = tpr * blockIdx.y; col0 < upr; col0 += step) {
+    const uint32_t col = col0 + t, next = col + step;
+    Unit vn = zero_unit(), un = zero_unit();
+    if (in_m && next < upr) {
+      vn = load_unit<kWide>(xr + next * 16u);
+      if (kSilu) un = load_unit<kWide>(ur + next * 16u);
     }
+    uint32_t y[8];
+    words(v, y);
+    if (kSilu) {
+      uint32_t u8[8];
+      words(u, u8);
 #pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      if (kSilu) {
-        uint32_t g4[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        const uint32_t u4[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          g4[j] = F::pack(silu_mul(F::lo(g4[j]), F::lo(u4[j])), silu_mul(F::hi(g4[j]), F::hi(u4[j])));
-        v[i] = make_uint4(g4[0], g4[1], g4[2], g4[3]);
-      }
-      const int e = group_exp<kDtype>(v[i]);
-      if (base + static_cast<uint64_t>(i) * 32u + lane < total)
-        store_chunk(codes + row[i] * ldc, scales + row[i] * lds, col[i], cpr, mx8_chunk_codes<kDtype>(v[i], e, zero), e);
+      for (int j = 0; j < 8; ++j)
+        y[j] = F::pack(silu_mul(F::lo(y[j]), F::lo(u8[j])), silu_mul(F::hi(y[j]), F::hi(u8[j])));
     }
+    store_mxfp8<kDtype>(y, cr, sr, col, upr, in_m && col < upr, zero);
+    v = vn;
+    u = un;
   }
 }
 
 // ---------------------------------------------------------------------------
-// rmsnorm: one row per warp (kWarpRow, up to 32 * kC chunks) or per CTA; the
-// row stays in registers (kC chunks per thread) between the sum of squares
+// rmsnorm: one row per warp (kWarpRow, up to 32 * kC units) or per CTA; the
+// row stays in registers (kC units per thread) between the sum of squares
 // and the output, so every input byte is read once.
 // ---------------------------------------------------------------------------
-template <int kDtype, int kC, bool kWarpRow>
+template <int kDtype, int kC, bool kWarpRow, bool kWide>
 __global__ void __launch_bounds__(kWarpRow ? kRowThreads : 1024)
 rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ res, const uint16_t* __restrict__ w,
                      uint16_t* __restrict__ h_out, uint16_t* __restrict__ y_out, uint8_t* __restrict__ codes,
-                     uint8_t* __restrict__ scales, int64_t M, uint32_t cpr, int64_t ldx, int64_t ldr, int64_t ldh,
+                     uint8_t* __restrict__ scales, int64_t M, uint32_t upr, int64_t ldx, int64_t ldr, int64_t ldh,
                      int64_t ldy, int64_t ldc, int64_t lds, float eps, float zero) {
   using F = Fmt<kDtype>;
   __shared__ float part[32];
@@ -129,41 +174,49 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
   const int64_t row0 = kWarpRow ? static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + warp : blockIdx.x;
   const int64_t rstep = kWarpRow ? static_cast<int64_t>(gridDim.x) * (kRowThreads / 32) : gridDim.x;
   for (int64_t row = row0; row < M; row += rstep) {
-    uint4 h[kC];
+    Unit h[kC];
     float ss = 0.f;
+    const uint16_t* xr = x + row * ldx;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const uint32_t col = t + i * step;
-      h[i] = col < cpr ? ld_stream(reinterpret_cast<const uint4*>(x + row * ldx + col * 8u)) : make_uint4(0, 0, 0, 0);
+      h[i] = col < upr ? load_unit<kWide>(xr + col * 16u) : zero_unit();
     }
     if (res != nullptr) {
-      uint4 r[kC];
+      const uint16_t* rr = res + row * ldr;
+      Unit r[kC];
 #pragma unroll
       for (int i = 0; i < kC; ++i) {
         const uint32_t col = t + i * step;
-        r[i] = col < cpr ? ld_stream(reinterpret_cast<const uint4*>(res + row * ldr + col * 8u)) : make_uint4(0, 0, 0, 0);
+        r[i] = col < upr ? load_unit<kWide>(rr + col * 16u) : zero_unit();
       }
 #pragma unroll
       for (int i = 0; i < kC; ++i) {
-        const uint32_t a4[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, r4[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
-        uint32_t o[4];
+        uint32_t a8[8], r8[8];
+        words(h[i], a8);
+        words(r[i], r8);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          o[j] = F::pack(__fadd_rn(F::lo(a4[j]), F::lo(r4[j])), __fadd_rn(F::hi(a4[j]), F::hi(r4[j])));
-        h[i] = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int j = 0; j < 8; ++j) {
+          const float2 s = add_f32x2(make_float2(F::lo(a8[j]), F::hi(a8[j])), make_float2(F::lo(r8[j]), F::hi(r8[j])));
+          a8[j] = F::pack(s.x, s.y);
+        }
+        h[i] = unit_of(a8);
         const uint32_t col = t + i * step;
-        if (col < cpr) *reinterpret_cast<uint4*>(h_out + row * ldh + col * 8u) = h[i];
+        if (col < upr) store_unit<kWide>(h_out + row * ldh + col * 16u, h[i]);
       }
     }
+    float2 sq = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
-      const uint32_t a4[4] = {h[i].x, h[i].y, h[i].z, h[i].w};
+      uint32_t a8[8];
+      words(h[i], a8);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = F::lo(a4[j]), b = F::hi(a4[j]);
-        ss = fmaf(a, a, fmaf(b, b, ss));
+      for (int j = 0; j < 8; ++j) {
+        const float2 a = make_float2(F::lo(a8[j]), F::hi(a8[j]));
+        sq = fma_f32x2(a, a, sq);
       }
     }
+    ss = sq.x + sq.y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
     if (!kWarpRow) {
@@ -174,37 +227,42 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
     }
-    const float rs = rsqrtf(ss / (static_cast<float>(cpr) * 8.0f) + eps);
+    const float rs = rsqrtf(ss / (static_cast<float>(upr) * 16.0f) + eps);
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
       const uint32_t col = t + i * step;
-      const uint4 wv = col < cpr ? __ldg(reinterpret_cast<const uint4*>(w + col * 8u)) : make_uint4(0, 0, 0, 0);
-      const uint32_t a4[4] = {h[i].x, h[i].y, h[i].z, h[i].w}, w4[4] = {wv.x, wv.y, wv.z, wv.w};
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        o[j] = F::pack(F::lo(a4[j]) * rs * F::lo(w4[j]), F::hi(a4[j]) * rs * F::hi(w4[j]));
-      const uint4 y = make_uint4(o[0], o[1], o[2], o[3]);
-      const int e = group_exp<kDtype>(y);
-      if (col < cpr) {
-        if (y_out != nullptr) *reinterpret_cast<uint4*>(y_out + row * ldy + col * 8u) = y;
-        store_chunk(codes + row * ldc, scales + row * lds, col, cpr, mx8_chunk_codes<kDtype>(y, e, zero), e);
+      Unit wv = zero_unit();
+      if (col < upr) {
+        const uint4* p = reinterpret_cast<const uint4*>(w + col * 16u);
+        wv = {__ldg(p), __ldg(p + 1)};
       }
+      uint32_t a8[8], w8[8];
+      words(h[i], a8);
+      words(wv, w8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 n = mul_f32x2(mul_f32x2(make_float2(F::lo(a8[j]), F::hi(a8[j])), make_float2(rs, rs)),
+                                   make_float2(F::lo(w8[j]), F::hi(w8[j])));
+        a8[j] = F::pack(n.x, n.y);
+      }
+      if (y_out != nullptr && col < upr) store_unit<kWide>(y_out + row * ldy + col * 16u, unit_of(a8));
+      store_mxfp8<kDtype>(a8, codes + row * ldc, scales + row * lds, col, upr, col < upr, zero);
     }
     if (!kWarpRow) __syncthreads();
   }
 }
 
-bool off16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+bool off(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
+bool off16(const void* p) { return off(p, 16); }
 
 // Launch with programmatic dependent launch: the kernel may start while the
 // previous one on the stream finishes; every thread passes
 // griddepcontrol.wait before it reads or writes global memory.
 template <typename... P, typename... A>
-int launch_pdl(const char* who, void (*fn)(P...), int64_t grid, int threads, cudaStream_t s, A... args) {
+int launch_pdl(const char* who, void (*fn)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -239,14 +297,23 @@ int rows_entry(const char* who, const void* x, void* codes, void* scales, int64_
                int64_t ldc, int64_t lds, int dtype, void* stream) {
   if (int st = check_rows(who, x, codes, scales, M, K, kSilu ? 2 * K : K, ldx, ldc, lds, dtype)) return st;
   if (M == 0 || K == 0) return QDQ_OK;
-  const uint32_t cpr = static_cast<uint32_t>(K / 8);
-  const uint64_t total = static_cast<uint64_t>(M) * cpr;
-  const uint64_t per = static_cast<uint64_t>(kRowThreads) * (kSilu ? 2 : 4);
-  const int64_t grid = static_cast<int64_t>(std::min<uint64_t>((total + per - 1) / per, 1u << 30));
-  auto fn = dtype == QDQ_DTYPE_FP16 ? &rows_mxfp8_kernel<QDQ_DTYPE_FP16, kSilu>
-                                    : &rows_mxfp8_kernel<QDQ_DTYPE_BF16, kSilu>;
-  return launch_pdl(who, fn, grid, kRowThreads, static_cast<cudaStream_t>(stream), static_cast<const uint16_t*>(x),
-                    static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), cpr, total, ldx, ldc, lds, 0.0f);
+  const uint32_t upr = static_cast<uint32_t>(K / 16);
+  // Threads a row: the most that keep 3/4 of themselves busy over the walk.
+  uint32_t tpr = 2;
+  for (uint32_t c = 4; c <= kRowThreads && c / 2 < upr; c *= 2)
+    if (4 * upr >= 3 * ((upr + c - 1) / c * c)) tpr = c;
+  const int64_t rpc = kRowThreads / tpr, grid = (M + rpc - 1) / rpc;
+  if (grid > (1ll << 31) - 1) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many rows", who);
+  // Few rows: a row's walk is split over CTAs, up to a few CTAs per SM (silu_mul [1, 14336]: 4.4 -> 2.6 us).
+  const int64_t walks = (upr + tpr - 1) / tpr, room = 4 * device_sm_count();
+  const int64_t split = std::max<int64_t>(1, std::min<int64_t>(walks, room / grid));
+  // K % 32 == 0, so silu_mul's second half starts as aligned as the first
+  const bool wide = !off(x, 32) && ldx % 16 == 0;
+  auto fn = dtype == QDQ_DTYPE_FP16
+                ? (wide ? &rows_mxfp8_kernel<QDQ_DTYPE_FP16, kSilu, true> : &rows_mxfp8_kernel<QDQ_DTYPE_FP16, kSilu, false>)
+                : (wide ? &rows_mxfp8_kernel<QDQ_DTYPE_BF16, kSilu, true> : &rows_mxfp8_kernel<QDQ_DTYPE_BF16, kSilu, false>);
+  return launch_pdl(who, fn, dim3(static_cast<unsigned>(grid), static_cast<unsigned>(split)), kRowThreads, static_cast<cudaStream_t>(stream), static_cast<const uint16_t*>(x),
+                    static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, upr, tpr, ldx, ldc, lds, 0.0f);
 }
 
 }  // namespace
@@ -284,24 +351,29 @@ extern "C" int qdq_rmsnorm_mxfp8(const void* x, const void* residual, const void
   if (off16(weight) || (residual && (off16(residual) || off16(residual_out) || ldr % 8 || ldh % 8)) ||
       (y && (off16(y) || ldy % 8)))
     return fail(QDQ_ERR_ALIGNMENT, "%s: rows must be 16-byte aligned", who);
-  const uint32_t cpr = static_cast<uint32_t>(K / 8);
+  const uint32_t upr = static_cast<uint32_t>(K / 16);
   const bool f16 = dtype == QDQ_DTYPE_FP16;
-  auto go = [&](auto fn_bf16, auto fn_f16, int threads, int64_t rows_per_cta) {
+  const bool wide = !(off(x, 32) || ldx % 16 || (residual && (off(residual, 32) || ldr % 16 || off(residual_out, 32) || ldh % 16)) ||
+                      (y && (off(y, 32) || ldy % 16)));
+  auto go = [&](auto bf16, auto f16w, auto bf16n, auto f16n, int threads, int64_t rows_per_cta) {
     const int64_t grid = std::min<int64_t>((M + rows_per_cta - 1) / rows_per_cta, 1 << 30);
-    return launch_pdl(who, f16 ? fn_f16 : fn_bf16, grid, threads, static_cast<cudaStream_t>(stream),
+    return launch_pdl(who, f16 ? (wide ? f16w : f16n) : (wide ? bf16 : bf16n), dim3(static_cast<unsigned>(grid)), threads, static_cast<cudaStream_t>(stream),
                       static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(residual),
                       static_cast<const uint16_t*>(weight), static_cast<uint16_t*>(residual_out),
-                      static_cast<uint16_t*>(y), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, cpr,
+                      static_cast<uint16_t*>(y), static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), M, upr,
                       ldx, ldr, ldh, ldy, ldc, lds, eps, 0.0f);
   };
 #define QDQ_NORM(C, WARP, THREADS, RPC) \
-  return go(&rmsnorm_mxfp8_kernel<QDQ_DTYPE_BF16, C, WARP>, &rmsnorm_mxfp8_kernel<QDQ_DTYPE_FP16, C, WARP>, THREADS, RPC)
-  if (cpr <= 32) QDQ_NORM(1, true, kRowThreads, kRowThreads / 32);
-  if (cpr <= 64) QDQ_NORM(2, true, kRowThreads, kRowThreads / 32);
-  if (cpr <= 128) QDQ_NORM(4, true, kRowThreads, kRowThreads / 32);
-  auto threads = [&](int c) { return static_cast<int>((cpr + 32 * c - 1) / (32 * c) * 32); };
-  if (cpr <= 1024) QDQ_NORM(2, false, threads(2), 1);
-  if (cpr <= 4096) QDQ_NORM(4, false, threads(4), 1);
-  QDQ_NORM(8, false, threads(8), 1);
+  return go(&rmsnorm_mxfp8_kernel<QDQ_DTYPE_BF16, C, WARP, true>, &rmsnorm_mxfp8_kernel<QDQ_DTYPE_FP16, C, WARP, true>, \
+            &rmsnorm_mxfp8_kernel<QDQ_DTYPE_BF16, C, WARP, false>, &rmsnorm_mxfp8_kernel<QDQ_DTYPE_FP16, C, WARP, false>, THREADS, RPC)
+  // Units per thread: one for few rows, whose latency is the sync's and the reduction's ([1, 4096] 2.0 us, with two
+  // 2.4; [777, 2880] 4.8 and 6.0), two where rows queue for the SMs and bytes in flight count ([16384, 8192] 137 us,
+  // with one 147).
+  if (upr <= 32) QDQ_NORM(1, true, kRowThreads, kRowThreads / 32);
+  if (upr <= 64) QDQ_NORM(2, true, kRowThreads, kRowThreads / 32);
+  auto threads = [&](int c) { return static_cast<int>((upr + 32 * c - 1) / (32 * c) * 32); };
+  if (upr <= 1024 && M <= 8 * device_sm_count()) QDQ_NORM(1, false, threads(1), 1);
+  if (upr <= 2048) QDQ_NORM(2, false, threads(2), 1);
+  QDQ_NORM(4, false, threads(4), 1);
 #undef QDQ_NORM
 }
