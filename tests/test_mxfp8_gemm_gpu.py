@@ -249,3 +249,71 @@ def test_a_gated_expert_layer_stage_by_stage(cuda_device, m, bs):
     out = h + down.view(m, top_k, hidden).sum(1)
     assert out.shape == (m, hidden) and out.isfinite().all()
     _ok()
+
+
+def test_refusals_name_the_argument(cuda_device):
+    """Malformed calls are refused before any launch, as the other operators refuse them."""
+    import dataclasses
+    from vllm_qdq_plugin.gemm import (mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight)
+    from vllm_qdq_plugin.qdq import Mxfp8Rows, mxfp8_rows, rmsnorm_mxfp8, silu_mul_mxfp8
+    dev = cuda_device
+    x = activation(8, 64, torch.bfloat16, 1, dev)
+    g = torch.ones(64, dtype=torch.bfloat16, device=dev)
+    rows = mxfp8_rows(x)
+    w = prepare_mxfp8_weight(*random_weight(32, 64, seed=1, dev=dev))
+    wm = prepare_mxfp8_moe_weight(*random_weight(2, 32, 64, seed=1, dev=dev))
+    _, sid, eid, ntp, tw = routing(8, 2, 1, 16, 1, dev)
+    bad = [
+        lambda: mxfp8_rows(x.float()), lambda: mxfp8_rows(x[0]), lambda: mxfp8_rows(x[:, :48]),
+        lambda: silu_mul_mxfp8(x[:, :63]), lambda: silu_mul_mxfp8(x[:, :32]),
+        lambda: rmsnorm_mxfp8(x, g[:32]), lambda: rmsnorm_mxfp8(x, g.float()), lambda: rmsnorm_mxfp8(x, g.cpu()),
+        lambda: rmsnorm_mxfp8(x, g, x[:4]), lambda: rmsnorm_mxfp8(x, g, x.half()), lambda: rmsnorm_mxfp8(x, g, x.cpu()),
+        lambda: rmsnorm_mxfp8(x, g, eps=-1.0),
+        lambda: rmsnorm_mxfp8(torch.zeros(1, 65568, dtype=torch.bfloat16, device=dev),
+                              torch.zeros(65568, dtype=torch.bfloat16, device=dev)),
+        lambda: Mxfp8Rows.from_codes(rows.codes, rows.scales[:, :1]), lambda: Mxfp8Rows.from_codes(rows.codes.view(torch.int8), rows.scales),
+        lambda: Mxfp8Rows.from_codes(rows.codes, rows.scales, torch.float32),
+        lambda: mxfp8_linear(x.float(), w), lambda: mxfp8_linear(x[:, :32], w), lambda: mxfp8_linear(x, w, g),
+        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.scales, rows.dtype), w),
+        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.stored[:4], rows.dtype), w),
+        lambda: mxfp8_linear(x, dataclasses.replace(w, codes=w.codes.cpu())),
+        lambda: prepare_mxfp8_weight(w.codes, rows.scales), lambda: prepare_mxfp8_moe_weight(w.codes, rows.scales),
+        lambda: mxfp8_moe_linear(x, wm, sid.long(), eid, ntp, tw, 16, 1, False),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid[:1], ntp, tw, 8, 1, False),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, None, 16, 1, True),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw[:3], 16, 1, True),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 65, 1, False),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 0, False),
+        lambda: mxfp8_moe_linear(x, wm, sid.cpu(), eid, ntp, tw, 16, 1, False),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 1, False, out=torch.empty(8, 32, device=dev)),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 1, False, out=torch.empty_like(x)),
+        lambda: mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 1, False,
+                                 out=torch.empty(32, 8, dtype=torch.bfloat16, device=dev).t()),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises((AssertionError, RuntimeError)):
+            call()
+            pytest.fail(f"call {i} was not refused")
+    with pytest.raises(AssertionError, match="2D"):
+        mxfp8_rows(x[0])
+    with pytest.raises(AssertionError, match="weight"):
+        rmsnorm_mxfp8(x, g[:32])
+    assert mxfp8_linear(x, w).isfinite().all()
+    _ok()
+
+
+def test_operators_trace_under_compile(cuda_device):
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import rmsnorm_mxfp8, silu_mul_mxfp8
+    x = activation(8, 64, torch.bfloat16, 1, cuda_device)
+    g = torch.ones(64, dtype=torch.bfloat16, device=cuda_device)
+    w = prepare_mxfp8_weight(*random_weight(128, 64, seed=1, dev=cuda_device))
+
+    def layer(x, r):
+        rows, h, _ = rmsnorm_mxfp8(x, g, r)
+        act = silu_mul_mxfp8(mxfp8_linear(rows, w))
+        return act.codes, act.stored, h
+
+    want = layer(x, x)
+    got = torch.compile(layer, backend="eager", fullgraph=True)(x, x)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -10,9 +10,6 @@ from vllm_qdq_plugin import _native
 BF16 = torch.bfloat16
 
 
-def _meta(*shape, dtype=BF16):
-    return torch.empty(*shape, dtype=dtype, device="meta")
-
 
 def test_cpu_tensors_are_refused():
     from vllm_qdq_plugin.gemm import Mxfp8MoeWeight, Mxfp8Weight, mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_weight
@@ -26,6 +23,17 @@ def test_cpu_tensors_are_refused():
                  lambda: Mxfp8Rows.from_codes(codes, scales), lambda: prepare_mxfp8_weight(codes, scales),
                  lambda: mxfp8_linear(x, weight),
                  lambda: mxfp8_moe_linear(x, moe, i32, i32, i32, None, 16, 1, False)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_errors_of_the_native_ops_reach_python():
+    """An error raised inside the C++ library is a Python exception, not the end of the process."""
+    from vllm_qdq_plugin import _build, qdq  # noqa: F401  (defines the schemas)
+    _native.lib()
+    torch.ops.load_library(str(_build.TORCH_OPS_PATH))
+    x = torch.zeros(4, 64, dtype=BF16)
+    for call in (lambda: torch.ops.qdq_b200.mxfp8_rows(x), lambda: torch.ops.qdq_b200.rmsnorm_mxfp8(x, x[0], x, 1e-6, True)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
 
@@ -150,6 +158,9 @@ def test_fake_kernels_give_the_shapes():
         assert torch.ops.qdq_b200.mxfp8_linear(x, w, sf, None).shape == (5, 7)
         y = torch.ops.qdq_b200.mxfp8_linear_rows(codes, scales, w, sf, None, False)
         assert y.shape == (5, 7) and y.dtype == torch.bfloat16
+        ids = torch.empty(32, dtype=torch.int32, device="cuda")
+        y = torch.ops.qdq_b200.mxfp8_moe_linear(x, None, w[None], sf, ids, ids, ids, None, 16, 2, True)
+        assert y.shape == (10, 7) and y.dtype == torch.float16
 
 
 def test_scale_stride_is_the_c_abis():

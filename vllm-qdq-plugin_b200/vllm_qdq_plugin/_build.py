@@ -71,7 +71,9 @@ def _torch_ops_commands(obj: Path, out: Path) -> tuple[list[str], list[str]]:
     includes = [f"-I{INCLUDE_DIR}", *(f"-isystem{p}" for p in cpp_extension.include_paths()), f"-isystem{cuda / 'include'}"]
     compile_cmd = [cxx, "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                    *includes, "-c", "-o", str(obj), str(TORCH_OPS_SOURCE)]
-    link_cmd = [cxx, "-shared", "-o", str(out), str(obj), f"-L{LIB_DIR}", "-lqdq_b200",
+    # The shared libstdc++ by name: a toolchain that links a static one in would give this library its own exception
+    # machinery, and an error it raises would end the process instead of reaching Python.
+    link_cmd = [cxx, "-shared", "-nostdlib++", "-o", str(out), str(obj), "-l:libstdc++.so.6", f"-L{LIB_DIR}", "-lqdq_b200",
                 *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
                 "-Wl,-rpath,$ORIGIN"]
     return compile_cmd, link_cmd

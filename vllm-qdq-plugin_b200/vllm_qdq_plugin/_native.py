@@ -118,10 +118,11 @@ def lib() -> ctypes.CDLL:
 _OPS_LOADED = False
 
 
-def load_ops() -> None:
-    """Load (building first if missing or stale) the torch.library kernels of csrc/torch_ops.cpp."""
+def load_ops(x: torch.Tensor) -> None:
+    """Load (building first if missing or stale) the torch.library kernels of csrc/torch_ops.cpp for the CUDA tensor x."""
     global _OPS_LOADED
     if not _OPS_LOADED:
+        require_cuda(x)
         lib()
         with _LOCK:
             if not _OPS_LOADED:

@@ -484,8 +484,11 @@ def prepare_mxfp8_moe_weight(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp8
     sf = torch.empty((e * per,), dtype=torch.uint8, device=codes.device)
     with _native.on_device(codes.device):
         stream = _native.stream_ptr(codes.device)
-        for i in range(e if n else 0):
-            _native.call("qdq_sf_tile", scales[i].data_ptr(), sf[i * per:].data_ptr(), n, k, k // 32, 32, stream)
+        if n % 128 == 0:  # whole row blocks: the experts' layouts follow one another
+            _native.call("qdq_sf_tile", scales.data_ptr(), sf.data_ptr(), e * n, k, k // 32, 32, stream)
+        else:
+            for i in range(e):
+                _native.call("qdq_sf_tile", scales[i].data_ptr(), sf[i * per:].data_ptr(), n, k, k // 32, 32, stream)
     return Mxfp8MoeWeight(codes=codes, sf_tiled=sf, e=e, n=n, k=k)
 
 
@@ -494,14 +497,14 @@ _LIB = torch.library.Library("qdq_b200", "FRAGMENT")
 _LIB.define("mxfp8_linear(Tensor a, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias) -> Tensor")
 _LIB.define("mxfp8_linear_rows(Tensor codes, Tensor scales, Tensor w_codes, Tensor w_sf_tiled, Tensor? bias, "
             "bool out_fp16) -> Tensor")
-_LIB.define("mxfp8_moe_linear(Tensor a, Tensor? a_scales, Tensor w_codes, Tensor w_sf_tiled, Tensor sorted_token_ids, "
-            "Tensor expert_ids, Tensor num_tokens_post_padded, Tensor? topk_weights, int moe_block_size, int top_k, "
-            "Tensor(a!) out) -> ()")
-
-
+_MOE_ARGS = ("Tensor a, Tensor? a_scales, Tensor w_codes, Tensor w_sf_tiled, Tensor sorted_token_ids, Tensor expert_ids, "
+             "Tensor num_tokens_post_padded, Tensor? topk_weights, int moe_block_size, int top_k")
+_LIB.define(f"mxfp8_moe_linear({_MOE_ARGS}, bool out_fp16) -> Tensor")
+_LIB.define(f"mxfp8_moe_linear_out({_MOE_ARGS}, Tensor(a!) out) -> ()")
 _mxfp8_linear_op = torch.ops.qdq_b200.mxfp8_linear.default
 _mxfp8_linear_rows_op = torch.ops.qdq_b200.mxfp8_linear_rows.default
 _mxfp8_moe_linear_op = torch.ops.qdq_b200.mxfp8_moe_linear.default
+_mxfp8_moe_linear_out_op = torch.ops.qdq_b200.mxfp8_moe_linear_out.default
 
 
 @torch.library.register_fake("qdq_b200::mxfp8_linear")
@@ -516,24 +519,28 @@ def _(codes, scales, w_codes, w_sf_tiled, bias, out_fp16):
 
 @torch.library.register_fake("qdq_b200::mxfp8_moe_linear")
 def _(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded, topk_weights,
+      moe_block_size, top_k, out_fp16):
+    return a.new_empty((a.shape[0] * top_k, w_codes.shape[1]), dtype=torch.float16 if out_fp16 else torch.bfloat16)
+
+
+@torch.library.register_fake("qdq_b200::mxfp8_moe_linear_out")
+def _(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens_post_padded, topk_weights,
       moe_block_size, top_k, out):
     return None
 
 
+# Where a call is refused (by the C++ ops, before any launch) or has no CUDA
+# tensor to dispatch on, these give the errors of the other operators.
 def _check_mxfp8_rows(name: str, a: torch.Tensor | Mxfp8Rows, k: int) -> None:
     if isinstance(a, Mxfp8Rows):
         _native.require_cuda(a.codes, a.stored)
-        m = a.codes.shape[0]
         assert a.codes.dim() == 2 and a.codes.dtype == torch.uint8 and a.stored.dtype == torch.uint8 and (
-            tuple(a.stored.shape) == (m, scale_stride(a.codes.shape[1]))), f"{name}: malformed MXFP8 rows"
-        assert a.codes.stride(1) == 1 and a.stored.stride(1) == 1, f"{name}: MXFP8 rows must be dense along K"
-        _native.same_device(a.codes.device, a.stored)
+            tuple(a.stored.shape) == (a.codes.shape[0], scale_stride(a.codes.shape[1]))), f"{name}: malformed MXFP8 rows"
     else:
         assert a.dim() == 2 and a.dtype in (torch.bfloat16, torch.float16), (
             f"{name}: the activation must be 2-D bf16/fp16 or MXFP8 rows")
         _native.require_cuda(a)
     assert a.shape[1] == k, (tuple(a.shape), k)
-    _native.load_ops()
 
 
 def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -543,16 +550,18 @@ def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.T
     rows that a norm or gate before it left.  Output dtype = a.dtype.  The
     product equals that of the dequantised operands up to fp32 summation order.
     """
-    _check_mxfp8_rows("mxfp8_linear", a, weight.k)
     if bias is None:
         bias = weight.bias
-    if bias is not None:
-        assert bias.dim() == 1 and bias.shape[0] == weight.n, (tuple(bias.shape), weight.n)
-        bias = bias.to(a.dtype).contiguous()
-    _native.same_device(a.device, weight.codes, bias)
-    if isinstance(a, Mxfp8Rows):
-        return _mxfp8_linear_rows_op(a.codes, a.stored, weight.codes, weight.sf_tiled, bias, a.dtype == torch.float16)
-    return _mxfp8_linear_op(a, weight.codes, weight.sf_tiled, bias)
+    try:
+        if isinstance(a, Mxfp8Rows):
+            _native.load_ops(a.codes)
+            return _mxfp8_linear_rows_op(a.codes, a.stored, weight.codes, weight.sf_tiled, bias, a.dtype == torch.float16)
+        _native.load_ops(a)
+        return _mxfp8_linear_op(a, weight.codes, weight.sf_tiled, bias)
+    except RuntimeError:
+        _check_mxfp8_rows("mxfp8_linear", a, weight.k)
+        assert bias is None or tuple(bias.shape) == (weight.n,), (tuple(bias.shape), weight.n)
+        raise
 
 
 def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted_token_ids: torch.Tensor,
@@ -565,24 +574,21 @@ def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted
 
     a: [M, K] bf16/fp16, or MXFP8 rows; out: [M * top_k, N] of a's dtype (allocated when None; rows of
     slots that are not routed keep their contents).  moe_block_size in [1, 64]."""
-    _check_mxfp8_rows("mxfp8_moe_linear", a, weight.k)
-    slots = a.shape[0] * top_k
-    assert top_k >= 1 and 1 <= moe_block_size <= 64, (top_k, moe_block_size)
-    for t in (sorted_token_ids, expert_ids, num_tokens_post_padded):
-        assert t.dtype == torch.int32 and t.is_contiguous(), "routing tensors are dense int32"
-    assert num_tokens_post_padded.numel() >= 1
-    assert expert_ids.numel() >= sorted_token_ids.numel() // moe_block_size, "expert_ids: one entry per block"
-    tw = None
-    if mul_topk_weights:
-        assert topk_weights is not None and topk_weights.numel() == slots, "topk_weights: one per slot"
-        tw = topk_weights.reshape(-1).float().contiguous()
-    if out is None:
-        out = torch.empty((slots, weight.n), dtype=a.dtype, device=a.device)
-    else:
-        assert tuple(out.shape) == (slots, weight.n) and out.dtype == a.dtype and (weight.n <= 1 or out.stride(1) == 1), (
-            "out must be [M * top_k, N] of the activation's dtype with dense rows")
-    _native.same_device(a.device, weight.codes, sorted_token_ids, expert_ids, num_tokens_post_padded, tw, out)
     rows = isinstance(a, Mxfp8Rows)
-    _mxfp8_moe_linear_op(a.codes if rows else a, a.stored if rows else None, weight.codes, weight.sf_tiled,
-                         sorted_token_ids, expert_ids, num_tokens_post_padded, tw, moe_block_size, top_k, out)
-    return out
+    codes, scales = (a.codes, a.stored) if rows else (a, None)
+    assert not mul_topk_weights or topk_weights is not None, "mul_topk_weights needs topk_weights"
+    tw = topk_weights if mul_topk_weights else None
+    assert out is None or out.dtype == a.dtype, (out.dtype, a.dtype)
+    try:
+        _native.load_ops(codes)
+        if out is None:
+            return _mxfp8_moe_linear_op(codes, scales, weight.codes, weight.sf_tiled, sorted_token_ids, expert_ids,
+                                        num_tokens_post_padded, tw, moe_block_size, top_k, a.dtype == torch.float16)
+        _mxfp8_moe_linear_out_op(codes, scales, weight.codes, weight.sf_tiled, sorted_token_ids, expert_ids,
+                                 num_tokens_post_padded, tw, moe_block_size, top_k, out)
+        return out
+    except RuntimeError:
+        _check_mxfp8_rows("mxfp8_moe_linear", a, weight.k)
+        for t in (sorted_token_ids, expert_ids, num_tokens_post_padded):
+            assert t.dtype == torch.int32 and t.is_contiguous(), "routing tensors are dense int32"
+        raise

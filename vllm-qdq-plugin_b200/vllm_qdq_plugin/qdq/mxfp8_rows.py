@@ -53,7 +53,7 @@ class Mxfp8Rows:
     def scales(self) -> torch.Tensor:
         """E8M0 scales [M, K / 32] (a view)."""
         n = self.codes.shape[1] // 32
-        return self.stored if self.stored.shape[1] == n else self.stored[:, :n]
+        return self.stored if self.stored.shape[1] == n else self.stored.narrow(1, 0, n)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> "Mxfp8Rows":
@@ -112,13 +112,19 @@ def _check(name: str, x: torch.Tensor, k: int) -> None:
     assert x.dtype in _DTYPES, f"{name} only supports fp16/bf16 tensors, but got {x.dtype}"
     assert k > 0 and k % 32 == 0, f"{name}: K={k} must be a positive multiple of 32"
     _native.require_cuda(x)
-    _native.load_ops()
 
 
+# The C++ ops refuse what is malformed before any launch.  The checks here give
+# the errors of the other operators (AssertionError for shapes and types); they
+# run only where a call was refused, or has no CUDA tensor to dispatch on.
 def mxfp8_rows(x: torch.Tensor) -> Mxfp8Rows:
     """MXFP8 rows of x [M, K] bf16/fp16 (CUDA, K % 32 == 0): the codes and scales of `mxfp8_quantize`."""
-    _check("mxfp8_rows", x, x.shape[-1])
-    return Mxfp8Rows(*_rows_op(x), x.dtype)
+    try:
+        _native.load_ops(x)
+        return Mxfp8Rows(*_rows_op(x), x.dtype)
+    except RuntimeError:
+        _check("mxfp8_rows", x, x.shape[-1])
+        raise
 
 
 def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
@@ -129,10 +135,12 @@ def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
 
     The product is formed in fp32 and rounded to x's dtype before it is quantised.
     """
-    k = x.shape[-1] // 2
-    _check("silu_mul_mxfp8", x, k)
-    assert x.shape[1] == 2 * k, f"silu_mul_mxfp8: {x.shape[1]} columns are not two halves"
-    return Mxfp8Rows(*_silu_mul_op(x), x.dtype)
+    try:
+        _native.load_ops(x)
+        return Mxfp8Rows(*_silu_mul_op(x), x.dtype)
+    except RuntimeError:
+        _check("silu_mul_mxfp8", x, x.shape[-1] // 2)
+        raise
 
 
 def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -152,15 +160,18 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     Returns:
         (MXFP8 rows of y, h or None without a residual, y or None).
     """
-    _check("rmsnorm_mxfp8", x, x.shape[-1])
-    k = x.shape[1]
-    assert k <= RMSNORM_MAX_K, f"rmsnorm_mxfp8: K={k} is above {RMSNORM_MAX_K}"
-    assert weight.dim() == 1 and weight.shape[0] == k and weight.dtype == x.dtype and weight.stride(0) == 1, (
-        f"rmsnorm_mxfp8: weight must be a dense [{k}] tensor of {x.dtype}")
-    assert residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), (
-        "rmsnorm_mxfp8: residual must have x's shape and dtype")
-    assert eps >= 0, f"rmsnorm_mxfp8: eps={eps} must not be negative"
-    _native.same_device(x.device, weight, residual)
-    out = _rmsnorm_op(x, weight, residual, eps, norm_out)
+    try:
+        _native.load_ops(x)
+        out = _rmsnorm_op(x, weight, residual, eps, norm_out)
+    except RuntimeError:
+        _check("rmsnorm_mxfp8", x, x.shape[-1])
+        k = x.shape[1]
+        assert k <= RMSNORM_MAX_K, f"rmsnorm_mxfp8: K={k} is above {RMSNORM_MAX_K}"
+        assert weight.dim() == 1 and weight.shape[0] == k and weight.dtype == x.dtype, (
+            f"rmsnorm_mxfp8: weight must be a [{k}] tensor of {x.dtype}")
+        assert residual is None or (residual.shape == x.shape and residual.dtype == x.dtype), (
+            "rmsnorm_mxfp8: residual must have x's shape and dtype")
+        assert eps >= 0, f"rmsnorm_mxfp8: eps={eps} must not be negative"
+        raise
     return (Mxfp8Rows(out[0], out[1], x.dtype), out[2] if residual is not None else None,
             out[-1] if norm_out else None)
