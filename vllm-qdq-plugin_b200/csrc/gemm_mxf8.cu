@@ -47,14 +47,16 @@ constexpr int T_EPI = 8;             // epilogue warps
 constexpr int T_SCALE = 4;           // scale warps = quads of stages in the scale ring
 constexpr int T_THREADS = 32 * (2 + T_SCALE + T_EPI);
 constexpr uint32_t T_TMEM = 512, T_SFW = 2 * NT_MAX, T_SFA = T_SFW + 4;
+constexpr uint32_t T_SF_COLS = 12;   // four sets of scale columns in turn: a stage's copies overlap the MMAs before it
 
-__host__ __device__ constexpr int t_stage_bytes(int nt) { return T_W + nt * TK + 512; }  // codes, W scales
-__host__ __device__ constexpr int t_sf_bytes(int nt) { return nt > 128 ? 1024 : 512; }     // a stage's activation scales
+__host__ __device__ constexpr int t_stage_bytes(int nt) { return T_W + nt * TK; }       // codes
+__host__ __device__ constexpr int t_sf_bytes(int nt) { return nt > 128 ? 1024 : 512; }  // a stage's activation scales
+__host__ __device__ constexpr int t_quads_bytes(int nt) { return 4 * T_SCALE * (t_sf_bytes(nt) + 512); }
 
 struct __align__(8) TBars {
   uint64_t full[T_STAGES_MAX];   // codes and W scales landed (1 arrival + tx)
   uint64_t empty[T_STAGES_MAX];  // the stage's MMAs completed
-  uint64_t sf_full[T_SCALE];     // a quad's activation scales are written
+  uint64_t sf_full[T_SCALE];     // a quad's activation scales are written, its W scales landed (2 arrivals + tx)
   uint64_t sf_empty[T_SCALE];    // the quad's MMAs completed
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
@@ -64,11 +66,11 @@ struct __align__(8) TBars {
 };
 constexpr int kSmemMax = 227 * 1024;
 __host__ __device__ constexpr int t_stages(int nt) {
-  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars)) - 4 * T_SCALE * t_sf_bytes(nt)) / t_stage_bytes(nt);
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars)) - t_quads_bytes(nt)) / t_stage_bytes(nt);
   return n < T_STAGES_MAX ? n : T_STAGES_MAX;
 }
 __host__ __device__ constexpr int t_smem(int nt) {
-  return 1024 + t_stages(nt) * t_stage_bytes(nt) + 4 * T_SCALE * t_sf_bytes(nt) + static_cast<int>(sizeof(TBars));
+  return 1024 + t_stages(nt) * t_stage_bytes(nt) + t_quads_bytes(nt) + static_cast<int>(sizeof(TBars));
 }
 
 template <int kDtype>
@@ -101,7 +103,7 @@ struct GemmArgs {
   const void* bias;            // dense
   void* c;
   int64_t ldc;
-  const int32_t* seg_tab;      // grouped: [count, (first block, blocks) ...]
+  const int32_t* seg_tab;      // grouped: [count, -, -, -], then (first position, rows, expert, -) per segment
   const int32_t* sorted_ids;
   const int32_t* expert_ids;
   const float* topk_w;         // nullptr: no scaling
@@ -128,33 +130,52 @@ struct Cursor {
 
 struct Item {
   int row0;     // first activation row (dense) or first sorted position (grouped)
-  int rows;     // rows of the segment
+  int rows;     // rows of the segment; 0: nothing to do
   int n_tile;
   int expert;
 };
 
-// Work item i, decoded alike by every role; false: nothing to do (grouped
-// only: a malformed segment).  Dense: tiles of one W panel run side by side,
-// so the CTAs in flight share it in L2.  Grouped: segment-major, so that each
-// expert's W streams from HBM once while its rows stay in L2.
+// Walks a CTA's work items; every role decodes them alike.  Dense: tiles of
+// one W panel run side by side, so the CTAs in flight share it in L2.
+// Grouped: segment-major, so that each expert's W streams from HBM once while
+// its rows stay in L2; the next item's segment entry is fetched while the
+// present item runs (read when it was needed, it held the ring up for 1 us an
+// item).
 template <bool kGrouped>
-__device__ __forceinline__ bool item_of(const GemmArgs& p, int i, int n_tiles, int num_m, Item& it) {
-  if (!kGrouped) {
-    it.n_tile = i / num_m;
-    it.row0 = (i - it.n_tile * num_m) * p.nt;
-    it.rows = min(p.nt, p.M - it.row0);
-    it.expert = 0;
+struct Walk {
+  const GemmArgs& p;
+  const int n_tiles, num_m, items, step;
+  int i;
+  int4 next;
+
+  __device__ __forceinline__ Walk(const GemmArgs& args, int first, int stride, int tiles)
+      : p(args), n_tiles(tiles), num_m(kGrouped ? 1 : (args.M + args.nt - 1) / args.nt),
+        items(kGrouped ? min(max(__ldcg(args.seg_tab), 0), args.num_blocks) * tiles : num_m * tiles), step(stride),
+        i(first - stride) {
+    fetch(first);
+  }
+  __device__ __forceinline__ void fetch(int j) {
+    if (kGrouped && j < items) next = __ldcg(reinterpret_cast<const int4*>(p.seg_tab + 4) + j / n_tiles);
+  }
+  __device__ __forceinline__ bool advance(Item& it) {
+    i += step;
+    if (i >= items) return false;
+    if (kGrouped) {
+      it = {next.x, next.y, i % n_tiles, next.z};
+      // a malformed entry is nothing to do
+      if (it.row0 < 0 || it.rows < 0 || it.rows > p.nt || it.row0 + it.rows > p.a_rows || it.expert < 0 ||
+          it.expert >= p.num_experts)
+        it.rows = 0;
+      fetch(i + step);
+    } else {
+      it.n_tile = i / num_m;
+      it.row0 = (i - it.n_tile * num_m) * p.nt;
+      it.rows = min(p.nt, p.M - it.row0);
+      it.expert = 0;
+    }
     return true;
   }
-  const int seg = i / n_tiles;
-  it.n_tile = i - seg * n_tiles;
-  const int blk0 = __ldcg(p.seg_tab + 1 + 2 * seg), nb = __ldcg(p.seg_tab + 2 + 2 * seg);
-  if (blk0 < 0 || nb < 1 || blk0 + nb > p.num_blocks || nb * p.bs > p.nt) return false;
-  it.expert = __ldcg(p.expert_ids + blk0);
-  it.row0 = blk0 * p.bs;
-  it.rows = nb * p.bs;
-  return it.expert >= 0 && it.expert < p.num_experts;
-}
+};
 
 template <int kDtype, bool kGrouped>
 __global__ void __launch_bounds__(T_THREADS, 1)
@@ -164,14 +185,13 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // code stages | W scale stages | quads of activation scales | barriers
+  // code stages | quads of W scales | quads of activation scales | barriers
   const int S = t_stages(p.nt), stage_bytes = T_W + p.nt * TK, sf_bytes = t_sf_bytes(p.nt);
   uint8_t* s_sfw = smem + S * stage_bytes;
-  uint8_t* s_sfa = s_sfw + S * 512;
+  uint8_t* s_sfa = s_sfw + 4 * T_SCALE * 512;
   TBars* bars = reinterpret_cast<TBars*>(s_sfa + 4 * T_SCALE * sf_bytes);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = (p.N + TM - 1) / TM;
-  const int num_m = kGrouped ? 1 : (p.M + p.nt - 1) / p.nt;
   const int num_kt = (p.K + TK - 1) / TK;
 
   if (threadIdx.x == 0) {
@@ -180,7 +200,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       mbar_init(&bars->empty[s], 1);
     }
     for (int b = 0; b < T_SCALE; ++b) {
-      mbar_init(&bars->sf_full[b], 1);
+      mbar_init(&bars->sf_full[b], 2);
       mbar_init(&bars->sf_empty[b], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -203,31 +223,41 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   pdl_launch_dependents();
   pdl_wait();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);  // uniform
-  const int num_items = kGrouped ? min(max(__ldcg(p.seg_tab), 0), p.num_blocks) * n_tiles : num_m * n_tiles;
+  Walk<kGrouped> walk(p, blockIdx.x, gridDim.x, n_tiles);
+  Item w;
 
   if (warp == 0) {
     // ---------------- producer.  The whole warp walks the loop, so that its addresses stay in uniform registers;
     // one lane issues.
     const bool leader = elect_one();
-    Cursor at;
-    int issued = 0;
+    Cursor at, sf_at;
+    int issued = 0, quads = 0;
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-      Item w;
-      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+    while (ok && walk.advance(w)) {
+      if (w.rows == 0) continue;
       const int w_row = w.expert * p.N + w.n_tile * TM;
       const uint8_t* sfw = p.sfw + w.expert * p.sf_per_expert + static_cast<int64_t>(w.n_tile) * p.kchunks * 512;
       const int boxes = (w.rows + p.box - 1) / p.box;
-      const uint32_t tx = T_W + 512 + boxes * p.box * TK;
+      const uint32_t tx = T_W + boxes * p.box * TK;
       for (int kt = 0; kt < num_kt; ++kt, ++issued, at.next(S)) {
         const int s = at.slot;
+        if ((kt & 3) == 0) {  // W scales, four stages at once
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->sf_empty[sf_at.slot], sf_at.phase ^ 1u, p.status, 0x609));
+          if (!ok) break;
+          if (leader) {
+            const uint32_t bytes = 512u * min(4, num_kt - kt);
+            mbar_arrive_expect_tx(&bars->sf_full[sf_at.slot], bytes);
+            bulk_load(s_sfw + sf_at.slot * 2048, sfw + static_cast<int64_t>(kt) * 512, bytes, &bars->sf_full[sf_at.slot]);
+          }
+          sf_at.next(T_SCALE);
+          ++quads;
+        }
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], at.phase ^ 1u, p.status, 0x601));
         if (!ok) break;
         uint8_t* st = smem + s * stage_bytes;
         if (leader) {
           mbar_arrive_expect_tx(&bars->full[s], tx);
           tma_load_2d(st, &tmap_w, kt * TK, w_row, &bars->full[s]);
-          bulk_load(s_sfw + s * 512, sfw + static_cast<int64_t>(kt) * 512, 512, &bars->full[s]);
           for (int b = 0; b < boxes; ++b)
             tma_load_2d(st + T_W + b * p.box * TK, &tmap_a, kt * TK, w.row0 + b * p.box, &bars->full[s]);
         }
@@ -236,6 +266,8 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     if (!ok) bars->abort = 1;
     // every issued copy has landed before the CTA may exit
     for (int j = max(0, issued - S); j < issued; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x602);
+    for (int j = max(0, quads - T_SCALE); j < quads; ++j)
+      mbar_wait(&bars->sf_full[j % T_SCALE], (j / T_SCALE) & 1, p.status, 0x60a);
   } else if (warp == 1) {
     // ---------------- MMA issuer (the whole warp walks, one lane issues).  Stages that are both full go out as a
     // pair: at few rows the loop around a stage costs more than its MMAs.
@@ -243,9 +275,8 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     Cursor at, sf_at, acc_at;
     const uint64_t dw0 = smem_desc_sw128(smem), dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-      Item w;
-      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+    while (ok && walk.advance(w)) {
+      if (w.rows == 0) continue;
       const int n_mma = (w.rows + 15) / 16 * 16;
       const uint32_t idesc = idesc_mxf8(TM, n_mma);
       ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc_at.slot], acc_at.phase ^ 1u, p.status, 0x603));
@@ -254,14 +285,15 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       const uint32_t acc = tmem + NT_MAX * acc_at.slot;
       auto stage = [&](int kt, int s) {
         const uint64_t dsa = dsa0 + ((sf_at.slot * 4 + (kt & 3)) * sf_bytes >> 4);
-        tmem_cp_sf(tmem + T_SFW, dsw0 + (s * 512 >> 4));
-        tmem_cp_sf(tmem + T_SFA, dsa);
-        if (n_mma > 128) tmem_cp_sf(tmem + T_SFA + 4, dsa + (512 >> 4));
+        const uint32_t sf = tmem + T_SF_COLS * (kt & 3);
+        tmem_cp_sf(sf + T_SFW, dsw0 + ((sf_at.slot * 4 + (kt & 3)) * 512 >> 4));
+        tmem_cp_sf(sf + T_SFA, dsa);
+        if (n_mma > 128) tmem_cp_sf(sf + T_SFA + 4, dsa + (512 >> 4));
         const uint64_t dw = dw0 + (s * stage_bytes >> 4), da = dw + (T_W >> 4);
 #pragma unroll
         for (uint32_t kk = 0; kk < 4; ++kk)  // K step kk reads scale byte kk of each row's four
-          mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (tmem + T_SFW) | (kk << 30),
-                   (tmem + T_SFA) | (kk << 30), (kt | kk) != 0);
+          mma_mxf8(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (sf + T_SFW) | (kk << 30),
+                   (sf + T_SFA) | (kk << 30), (kt | kk) != 0);
         tc_commit(&bars->empty[s]);
       };
       for (int kt = 0; kt < num_kt;) {
@@ -301,9 +333,8 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     const int quads = (num_kt + 3) / 4;
     int quad = 0;  // first quad of the item, counted over the CTA's items
     bool ok = true;
-    for (int i = blockIdx.x; ok && i < num_items; i += gridDim.x) {
-      Item w;
-      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+    while (ok && walk.advance(w)) {
+      if (w.rows == 0) continue;
       const int n_mma = (w.rows + 15) / 16 * 16;
       const uint8_t* src[kR];
 #pragma unroll
@@ -343,9 +374,8 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     T* C = static_cast<T*>(p.c);
     bool ok = true;
     int j = 0;
-    for (int i = blockIdx.x; i < num_items; i += gridDim.x) {
-      Item w;
-      if (!item_of<kGrouped>(p, i, n_tiles, num_m, w)) continue;
+    while (walk.advance(w)) {
+      if (w.rows == 0) continue;
       const int nchunks = (w.rows + 31) / 32;
       // output rows of this warp's columns, fetched while the MMAs run: lane l holds that of column 32 c + l
       int slot[kCh];
@@ -752,7 +782,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // ---------------------------------------------------------------------------
 constexpr int SEG_THREADS = 1024;
 
-__device__ void build_segments(const int32_t* __restrict__ expert_ids, int live, int num_experts, int nbmax,
+__device__ void build_segments(const int32_t* __restrict__ expert_ids, int live, int bs, int num_experts, int nbmax,
                                int32_t* __restrict__ seg_tab) {
   __shared__ int s_start[32], s_count[32];
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5, nw = blockDim.x >> 5;
@@ -786,8 +816,7 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, int live,
     if (seg) {
       int nb = 1;
       while (nb < nbmax && b + nb < live && __ldg(expert_ids + b + nb) == e) ++nb;
-      seg_tab[1 + 2 * at] = b;
-      seg_tab[2 + 2 * at] = nb;
+      reinterpret_cast<int4*>(seg_tab + 4)[at] = make_int4(b * bs, nb * bs, e, 0);
     }
     carry_start = last;
     carry_count += all;
@@ -814,7 +843,7 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
   const int npp = __ldcg(num_post_padded);
   const int live = npp <= 0 ? 0 : min(num_blocks, (npp - 1) / bs + 1);
   if (blockIdx.x == 0) {
-    build_segments(expert_ids, live, num_experts, nbmax, seg_tab);
+    build_segments(expert_ids, live, bs, num_experts, nbmax, seg_tab);
     return;
   }
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -956,12 +985,13 @@ int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewAr
 }
 
 // Rows per item for `rows` wanted, in whole TMA boxes of 64, 32 or 16 rows: a
-// large box costs the producer fewer issues, a small one a ragged segment
-// fewer idle rows.
-void rows_per_item(GemmArgs& p, int64_t rows) {
+// large box costs the producer fewer issues (60 cycles each), a small one a
+// ragged segment fewer idle rows.
+void rows_per_item(GemmArgs& p, int64_t rows, bool grouped) {
   const int want = static_cast<int>(std::min<int64_t>(rows, NT_MAX));
   p.box = want > 96 ? 64 : want > 16 ? 32 : 16;
   p.nt = (want + p.box - 1) / p.box * p.box;
+  if (!grouped) p.box = p.nt;  // one tile's rows in one box
 }
 
 int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
@@ -1064,7 +1094,7 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
   p.top_k = 1;
   p.a_rows = p.M;
-  rows_per_item(p, M);
+  rows_per_item(p, M, false);
   p.status = status;
   CUtensorMap tw, ta;
   if (int st = make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128)) return st;
@@ -1107,7 +1137,7 @@ extern "C" int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void
 
 extern "C" int64_t fp8_moe_workspace_bytes(int64_t size_m, int64_t num_sorted, int moe_block_size, int64_t K) {
   if (size_m <= 0 || num_sorted <= 0 || moe_block_size <= 0 || K <= 0) return 0;
-  return up256(4 * (1 + 2 * (num_sorted / moe_block_size))) + up256(num_sorted * K) +
+  return up256(16 * (1 + num_sorted / moe_block_size)) + up256(num_sorted * K) +
          up256(num_sorted * qdq_mxfp8_scale_stride(K));
 }
 
@@ -1179,14 +1209,14 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
     }
   }
   int32_t* seg_tab = static_cast<int32_t*>(workspace);
-  uint8_t* codes = static_cast<uint8_t*>(workspace) + up256(4 * (1 + 2 * num_blocks));
+  uint8_t* codes = static_cast<uint8_t*>(workspace) + up256(16 * (1 + num_blocks));
   uint8_t* scales = codes + up256(num_sorted * K);
   const int64_t ldso = qdq_mxfp8_scale_stride(K);
   GemmArgs p = {};
   // Rows per item: the average expert's, rounded up to whole blocks, so that few rows leave the shared memory to
   // more stages of W in flight; never less than a block.
   const int64_t average = (num_sorted + num_experts - 1) / num_experts;
-  rows_per_item(p, (average + moe_block_size - 1) / moe_block_size * moe_block_size);
+  rows_per_item(p, (average + moe_block_size - 1) / moe_block_size * moe_block_size, true);
   const int nbmax = p.nt / moe_block_size;
   {
     const int warps = SEG_THREADS / 32;
