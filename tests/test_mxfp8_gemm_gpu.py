@@ -27,7 +27,8 @@ def _rows_values(rows):
 @pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 32), (1, 4096, 4096), (2, 300, 96), (16, 512, 1024),
                                    (17, 129, 544), (33, 640, 512), (64, 1024, 2080), (65, 200, 288), (100, 1001, 2880),
                                    (128, 256, 256), (129, 257, 352), (192, 384, 512), (193, 384, 512),
-                                   (333, 768, 2048), (1000, 136, 160), (257, 2050, 4128)])
+                                   (333, 768, 2048), (1000, 136, 160), (257, 2050, 4128),
+                                   (1500, 2560, 544), (2100, 1281, 288), (700, 5002, 320), (4111, 640, 128)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_linear_against_64_bits(cuda_device, m, n, k, dtype):
     from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
@@ -107,7 +108,10 @@ def test_linear_empty(cuda_device):
                                                   (150, 4, 2, 48, 257, 512, False),
                                                   (90, 5, 2, 1, 130, 96, True),
                                                   (50, 3, 1, 13, 128, 320, False),
-                                                  (61, 128, 4, 16, 128, 256, True)])
+                                                  (61, 128, 4, 16, 128, 256, True),
+                                                  (600, 3, 2, 64, 2304, 288, True),
+                                                  (200, 16, 2, 16, 2305, 544, False),
+                                                  (900, 2, 1, 48, 4352, 96, True)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_moe_against_64_bits(cuda_device, m, e, top_k, bs, n, k, mul, dtype):
     """Every routed slot's row; one block per expert, long runs cut into segments, layouts whose runs cross the

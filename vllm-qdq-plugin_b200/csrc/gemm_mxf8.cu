@@ -78,12 +78,14 @@ struct Out16 {
   using T = __nv_bfloat16;
   __device__ static float load(const T* p) { return __bfloat162float(*p); }
   __device__ static T one(float a) { return __float2bfloat16_rn(a); }
+  __device__ static uint32_t two(float a, float b) { return pack_bf16x2(a, b); }
 };
 template <>
 struct Out16<QDQ_DTYPE_FP16> {
   using T = __half;
   __device__ static float load(const T* p) { return __half2float(*p); }
   __device__ static T one(float a) { return __float2half_rn(a); }
+  __device__ static uint32_t two(float a, float b) { return pack_f16x2(a, b); }
 };
 
 // E4M3 codes of a 16-byte chunk of a 32-group with scale exponent e.
@@ -111,6 +113,7 @@ struct GemmArgs {
   int top_k, bs, num_blocks, num_experts;
   int a_rows;                  // rows of the activation codes (grouped: sorted positions)
   int nt, box;                 // activation rows per item, and per TMA box
+  int pairs;                   // C takes 4-byte stores of two columns
   int* status;
 };
 
@@ -176,6 +179,62 @@ struct Walk {
     return true;
   }
 };
+
+// Output row of each of an item's columns (-1: none) and its factor, held by
+// lane l for column 32 c + l.
+template <bool kGrouped>
+__device__ __forceinline__ void column_rows(const GemmArgs& p, const Item& w, int c, int lane, int& slot, float& wt) {
+  const int col = 32 * c + lane;
+  slot = -1;
+  wt = 1.0f;
+  if (col < w.rows) slot = kGrouped ? __ldcg(p.sorted_ids + w.row0 + col) : w.row0 + col;
+  if (slot >= p.M) slot = -1;
+  if (kGrouped && p.topk_w != nullptr && slot >= 0) wt = __ldcg(p.topk_w + slot);
+}
+
+// Stores 32 accumulator columns (activation rows) of this lane's W row n.
+// Neighbouring lanes hold neighbouring n: they exchange halves, so that a lane
+// stores two n of one row at once, the even lanes of the even rows, the odd
+// lanes of the odd ones.  All exchanges come before the stores (in turn with
+// them, each store waited for its row's shuffle: 18 k cycles an item of 240
+// rows where the MMAs take 15 k).
+template <int kDtype, bool kGrouped>
+__device__ __forceinline__ void store_columns(const GemmArgs& p, const uint32_t (&r)[32], int n, int lane, int slot,
+                                              float wt, float bias) {
+  using O = Out16<kDtype>;
+  using T = typename O::T;
+  T* C = static_cast<T*>(p.c);
+  if (p.pairs) {
+    const int odd = lane & 1;
+    uint32_t v[16];
+    int row[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float a = __uint_as_float(r[2 * i]) + bias, b = __uint_as_float(r[2 * i + 1]) + bias;
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
+      float lo = odd ? other : a, hi = odd ? b : other;
+      if (kGrouped) {
+        const float f = __shfl_sync(0xffffffffu, wt, 2 * i + odd);
+        lo *= f;
+        hi *= f;
+      }
+      row[i] = __shfl_sync(0xffffffffu, slot, 2 * i + odd);
+      v[i] = O::two(lo, hi);
+    }
+    if (n < p.N) {  // N is even: both n of a pair are inside, or neither
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (row[i] >= 0) *reinterpret_cast<uint32_t*>(C + static_cast<int64_t>(row[i]) * p.ldc + (n & ~1)) = v[i];
+    }
+  } else {
+#pragma unroll
+    for (int l = 0; l < 32; ++l) {
+      const int s = __shfl_sync(0xffffffffu, slot, l);
+      const float f = __shfl_sync(0xffffffffu, wt, l);
+      if (s >= 0 && n < p.N) C[static_cast<int64_t>(s) * p.ldc + n] = O::one(__uint_as_float(r[l]) * f + bias);
+    }
+  }
+}
 
 template <int kDtype, bool kGrouped>
 __global__ void __launch_bounds__(T_THREADS, 1)
@@ -371,27 +430,18 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     // ---------------- epilogue: warp reads TMEM lanes 32 (warp % 4).., column chunks half, half + 2, ...
     const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
     constexpr int kCh = (NT_MAX / 32 + 1) / 2;
-    T* C = static_cast<T*>(p.c);
     bool ok = true;
     int j = 0;
     while (walk.advance(w)) {
       if (w.rows == 0) continue;
       const int nchunks = (w.rows + 31) / 32;
-      // output rows of this warp's columns, fetched while the MMAs run: lane l holds that of column 32 c + l
+      // output rows of this warp's columns, fetched while the MMAs run
       int slot[kCh];
       float wt[kCh];
 #pragma unroll
-      for (int u = 0; u < kCh; ++u) {
-        const int col = 32 * (half + 2 * u) + lane;
-        int s = -1;
-        if (col < w.rows) s = kGrouped ? __ldcg(p.sorted_ids + w.row0 + col) : w.row0 + col;
-        if (s >= p.M) s = -1;
-        slot[u] = s;
-        wt[u] = (kGrouped && p.topk_w != nullptr && s >= 0) ? __ldcg(p.topk_w + s) : 1.0f;
-      }
+      for (int u = 0; u < kCh; ++u) column_rows<kGrouped>(p, w, half + 2 * u, lane, slot[u], wt[u]);
       const int n = w.n_tile * TM + q * 32 + lane;
-      const bool in_n = n < p.N;
-      const float bias = (!kGrouped && p.bias != nullptr && in_n) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+      const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
       const int buf = j & 1;
       if (ok) ok = mbar_wait(&bars->acc_full[buf], (j >> 1) & 1, p.status, 0x607);
       ok = __all_sync(0xffffffffu, ok);
@@ -414,14 +464,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           mbar_arrive(&bars->acc_empty[buf]);
         }
         if (!store) continue;
-#pragma unroll
-        for (int l = 0; l < 32; ++l) {
-          const int s = __shfl_sync(0xffffffffu, slot[u], l);
-          float v = __uint_as_float(r[l]);
-          if (kGrouped) v *= __shfl_sync(0xffffffffu, wt[u], l);
-          else v += bias;
-          if (s >= 0 && in_n) C[static_cast<int64_t>(s) * p.ldc + n] = O::one(v);
-        }
+        store_columns<kDtype, kGrouped>(p, r, n, lane, slot[u], wt[u], bias);
       }
       ++j;
     }
@@ -432,6 +475,287 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, T_TMEM);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the same walk by pairs of CTAs (tcgen05 cta_group::2).
+//
+// What bounds the kernel above at many rows is operand delivery: an SM takes
+// in about 80 bytes a cycle, and a 128 x 192 item needs 106 to keep its MMAs
+// going.  A pair shares one 256 x NT item: each CTA holds 128 rows of W and
+// half of the activation rows, and its MMAs read the other half from its
+// peer's shared memory, so an SM takes in 66 bytes a cycle at NT = 240.
+// Two accumulators of 240 columns and two sets of scale columns fill TMEM.
+//
+// Roles as above, in both CTAs, with these differences: TMA completes on the
+// leader's (rank 0) barriers, the leader alone issues MMAs and its commits
+// arrive in both CTAs; each CTA writes the scales of all the item's rows to
+// its own shared memory, which its half of the MMA reads.
+// ---------------------------------------------------------------------------
+constexpr int P_NT_MAX = 240;
+constexpr int P_STAGES_MAX = 11;
+constexpr uint32_t P_SFW = 2 * P_NT_MAX, P_SFA = P_SFW + 4, P_SF_COLS = 12, P_SF_SETS = 2;
+static_assert(P_SFW + P_SF_SETS * P_SF_COLS <= 512, "pair TMEM columns");
+
+struct __align__(8) PBars {
+  uint64_t full[P_STAGES_MAX];   // leader: both CTAs' codes landed (1 arrival + tx)
+  uint64_t empty[P_STAGES_MAX];  // each CTA: the pair's MMAs on the stage completed
+  uint64_t sf_full[T_SCALE];     // leader: both CTAs' scales of the quad are in place (3 arrivals + tx)
+  uint64_t sf_empty[T_SCALE];    // each CTA
+  uint64_t acc_full[2];          // each CTA
+  uint64_t acc_empty[2];         // leader: both CTAs' epilogue warps have read the accumulator
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+__host__ __device__ constexpr int p_stage_bytes(int tok) { return T_W + tok * TK; }  // tok: token rows held by a CTA
+constexpr int P_QUADS = 4 * T_SCALE * (1024 + 512);
+__host__ __device__ constexpr int p_stages(int tok) {
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(PBars)) - P_QUADS) / p_stage_bytes(tok);
+  return n < P_STAGES_MAX ? n : P_STAGES_MAX;
+}
+__host__ __device__ constexpr int p_smem(int tok) {
+  return 1024 + p_stages(tok) * p_stage_bytes(tok) + P_QUADS + static_cast<int>(sizeof(PBars));
+}
+
+template <int kDtype, bool kGrouped>
+__global__ void __launch_bounds__(T_THREADS, 1)
+mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
+                 const __grid_constant__ CUtensorMap tmap_sfw, const __grid_constant__ GemmArgs p) {
+  using O = Out16<kDtype>;
+  using T = typename O::T;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // code stages | quads of W scales | quads of activation scales | barriers
+  const int tok_rows = (p.nt / 2 + p.box - 1) / p.box * p.box;
+  const int S = p_stages(tok_rows), stage_bytes = p_stage_bytes(tok_rows);
+  uint8_t* s_sfw = smem + S * stage_bytes;
+  uint8_t* s_sfa = s_sfw + 4 * T_SCALE * 512;
+  PBars* bars = reinterpret_cast<PBars*>(s_sfa + 4 * T_SCALE * 1024);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int n_tiles = (p.N + 2 * TM - 1) / (2 * TM);
+  const int num_kt = (p.K + TK - 1) / TK;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int b = 0; b < T_SCALE; ++b) {
+      mbar_init(&bars->sf_full[b], 3);
+      mbar_init(&bars->sf_empty[b], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&bars->acc_full[b], 1);
+      mbar_init(&bars->acc_empty[b], 2 * T_EPI);
+    }
+    mbar_init(&bars->drain, 1);
+    bars->abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_sfw);
+  }
+  if (warp == 0) {
+    tmem_alloc_pair(&bars->tmem_base, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();  // both CTAs' barriers are initialised and the TMEM is allocated
+  tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);
+  Walk<kGrouped> walk(p, blockIdx.x >> 1, gridDim.x >> 1, n_tiles);
+  Item w;
+
+  if (warp == 0) {
+    // ---------------- producer (both CTAs): own W rows and own half of the activation rows
+    const bool leader = elect_one();
+    Cursor at, sf_at;
+    int issued = 0, quads = 0;
+    bool ok = true;
+    while (ok && walk.advance(w)) {
+      if (w.rows == 0) continue;
+      const int half = (w.rows + 15) / 16 * 8;  // half of the MMA's N
+      const int w_row = w.expert * p.N + w.n_tile * 2 * TM + static_cast<int>(rank) * TM;
+      const int a_row = w.row0 + static_cast<int>(rank) * half;
+      const int sf_row = w.expert * static_cast<int>(p.sf_per_expert / 512) + (2 * w.n_tile + static_cast<int>(rank)) * p.kchunks;
+      const int boxes = (half + p.box - 1) / p.box;
+      for (int kt = 0; kt < num_kt; ++kt, ++issued, at.next(S)) {
+        const int s = at.slot;
+        if ((kt & 3) == 0) {  // W scales, four stages at once
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->sf_empty[sf_at.slot], sf_at.phase ^ 1u, p.status, 0x801));
+          if (!ok) break;
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(&bars->sf_full[sf_at.slot], 2 * 2048);
+            tma_load_2d_pair(s_sfw + sf_at.slot * 2048, &tmap_sfw, 0, sf_row + kt, cluster_addr(&bars->sf_full[sf_at.slot], 0));
+          }
+          sf_at.next(T_SCALE);
+          ++quads;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->empty[s], at.phase ^ 1u, p.status, 0x802));
+        if (!ok) break;
+        uint8_t* st = smem + s * stage_bytes;
+        if (leader) {
+          const uint32_t full0 = cluster_addr(&bars->full[s], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * (T_W + boxes * p.box * TK));
+          tma_load_2d_pair(st, &tmap_w, kt * TK, w_row, full0);
+          for (int b = 0; b < boxes; ++b)
+            tma_load_2d_pair(st + T_W + b * p.box * TK, &tmap_a, kt * TK, a_row + b * p.box, full0);
+        }
+      }
+    }
+    if (!ok) bars->abort = 1;
+    // The leader's barriers cover the pair's copies still in flight.
+    if (rank == 0) {
+      for (int j = max(0, issued - S); j < issued; ++j) mbar_wait(&bars->full[j % S], (j / S) & 1, p.status, 0x803);
+      for (int j = max(0, quads - T_SCALE); j < quads; ++j)
+        mbar_wait(&bars->sf_full[j % T_SCALE], (j / T_SCALE) & 1, p.status, 0x804);
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader)
+    if (rank == 0) {
+      const bool leader = elect_one();
+      Cursor at, sf_at, acc_at;
+      const uint64_t dw0 = smem_desc_sw128(smem), dsw0 = smem_desc_sf(s_sfw), dsa0 = smem_desc_sf(s_sfa);
+      bool ok = true;
+      while (ok && walk.advance(w)) {
+        if (w.rows == 0) continue;
+        const int n_mma = (w.rows + 15) / 16 * 16;
+        const uint32_t idesc = idesc_mxf8(2 * TM, n_mma);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_empty[acc_at.slot], acc_at.phase ^ 1u, p.status, 0x805));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + P_NT_MAX * acc_at.slot;
+        for (int kt = 0; kt < num_kt; ++kt, at.next(S)) {
+          const int s = at.slot;
+          if ((kt & 3) == 0) ok = mbar_wait_cluster(&bars->sf_full[sf_at.slot], sf_at.phase, p.status, 0x806);
+          ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->full[s], at.phase, p.status, 0x807));
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+            const uint64_t dsa = dsa0 + ((sf_at.slot * 4 + (kt & 3)) * 1024 >> 4);
+            const uint32_t sf = tmem + P_SF_COLS * (kt & (P_SF_SETS - 1));
+            tmem_cp_sf_pair(sf + P_SFW, dsw0 + ((sf_at.slot * 4 + (kt & 3)) * 512 >> 4));
+            tmem_cp_sf_pair(sf + P_SFA, dsa);
+            if (n_mma > 128) tmem_cp_sf_pair(sf + P_SFA + 4, dsa + (512 >> 4));
+            const uint64_t dw = dw0 + (s * stage_bytes >> 4), da = dw + (T_W >> 4);
+#pragma unroll
+            for (uint32_t kk = 0; kk < 4; ++kk)
+              mma_mxf8_pair(acc, dw + 2 * kk, da + 2 * kk, idesc_with_sf_ids(idesc, kk, kk), (sf + P_SFW) | (kk << 30),
+                            (sf + P_SFA) | (kk << 30), (kt | kk) != 0);
+            tc_commit_pair(&bars->empty[s]);
+            if ((kt & 3) == 3 || kt + 1 == num_kt) tc_commit_pair(&bars->sf_empty[sf_at.slot]);
+          }
+          if ((kt & 3) == 3 || kt + 1 == num_kt) sf_at.next(T_SCALE);
+        }
+        if (!ok) break;
+        if (leader) tc_commit_pair(&bars->acc_full[acc_at.slot]);
+        acc_at.next(2);
+      }
+      if (!ok) bars->abort = 1;
+      if (leader) {
+        tc_commit_pair_local(&bars->drain);  // tracks the pair's tcgen05 ops
+        mbar_wait(&bars->drain, 0, p.status, 0x808);
+      }
+    }
+  } else if (warp < 2 + T_SCALE) {
+    // ---------------- activation scales of all the item's rows, in both CTAs
+    constexpr int kR = (P_NT_MAX + 31) / 32;  // rows per lane
+    const int u = warp - 2;
+    const int quads = (num_kt + 3) / 4;
+    const uint32_t full0 = cluster_addr(&bars->sf_full[u], 0);
+    int quad = 0;
+    bool ok = true;
+    while (ok && walk.advance(w)) {
+      if (w.rows == 0) continue;
+      const int n_mma = (w.rows + 15) / 16 * 16;
+      const uint8_t* src[kR];
+#pragma unroll
+      for (int j = 0; j < kR; ++j)
+        src[j] = p.sfa + static_cast<int64_t>(min(w.row0 + lane + 32 * j, p.a_rows - 1)) * p.lds;
+      for (int h = (u - quad) & (T_SCALE - 1); h < quads; h += T_SCALE) {
+        uint4 v[kR];
+#pragma unroll
+        for (int j = 0; j < kR; ++j)
+          if (lane + 32 * j < n_mma) v[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + 16 * h));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->sf_empty[u], (((quad + h) / T_SCALE) & 1) ^ 1, p.status, 0x809));
+        if (!ok) break;
+        uint8_t* sf = s_sfa + u * 4 * 1024;
+#pragma unroll
+        for (int j = 0; j < kR; ++j) {
+          if (lane + 32 * j < n_mma) {
+            uint8_t* at = sf + (j >> 2) * 512 + lane * 16 + (j & 3) * 4;
+            *reinterpret_cast<uint32_t*>(at) = v[j].x;
+            *reinterpret_cast<uint32_t*>(at + 1024) = v[j].y;
+            *reinterpret_cast<uint32_t*>(at + 2048) = v[j].z;
+            *reinterpret_cast<uint32_t*>(at + 3072) = v[j].w;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(full0);
+      }
+      quad += quads;
+    }
+    if (!ok) bars->abort = 1;
+  } else {
+    // ---------------- epilogue (both CTAs): TMEM lanes = the CTA's 128 W rows, columns = activation rows
+    const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
+    constexpr int kCh = (P_NT_MAX / 32 + 2) / 2;
+    Cursor acc_at;
+    bool ok = true;
+    while (walk.advance(w)) {
+      if (w.rows == 0) continue;
+      const int nchunks = (w.rows + 31) / 32;
+      int slot[kCh];
+      float wt[kCh];
+#pragma unroll
+      for (int u = 0; u < kCh; ++u) column_rows<kGrouped>(p, w, half + 2 * u, lane, slot[u], wt[u]);
+      const int n = w.n_tile * 2 * TM + static_cast<int>(rank) * TM + q * 32 + lane;
+      const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+      const uint32_t acc_empty0 = cluster_addr(&bars->acc_empty[acc_at.slot], 0);
+      if (ok) ok = mbar_wait(&bars->acc_full[acc_at.slot], acc_at.phase, p.status, 0x80a);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + P_NT_MAX * acc_at.slot;
+      const bool store = __all_sync(0xffffffffu, ok && !*(volatile int*)&bars->abort);
+      if (half >= nchunks) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty0);
+      }
+#pragma unroll
+      for (int u = 0; u < kCh; ++u) {
+        const int c = half + 2 * u;
+        if (c >= nchunks) break;
+        uint32_t r[32];
+        tmem_ld32(taddr + 32 * c, r);
+        tmem_ld_wait();
+        if (c + 2 >= nchunks) {  // this warp's last chunk of the item
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_empty0);
+        }
+        if (!store) continue;
+        store_columns<kDtype, kGrouped>(p, r, n, lane, slot[u], wt[u], bias);
+      }
+      acc_at.next(2);
+    }
+  }
+
+  // Neither CTA releases the pair's TMEM or exits while the other may still
+  // arrive on its barriers or read its shared memory.
+  tc_fence_before();
+  __syncwarp();
+  cluster_sync();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -882,38 +1206,54 @@ int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 bool off(const void* p, int a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) != 0; }
 
 template <typename... P, typename... A>
-int launch_pdl(const char* who, void (*fn)(P...), int64_t grid, int threads, size_t smem, cudaStream_t s, A... args) {
+int launch_pdl(const char* who, void (*fn)(P...), int64_t grid, int threads, size_t smem, cudaStream_t s, int cluster,
+               A... args) {
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...);
   if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
   return check_launch(who);
 }
 
-template <int kDtype, bool kGrouped>
-int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, const GemmArgs& p, int64_t items,
-                cudaStream_t s) {
-  static bool attr_set[64] = {false};
+template <typename F>
+int allow_smem(const char* who, F fn, bool (&done)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(&mxf8_gemm_kernel<kDtype, kGrouped>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+  if (dev >= 0 && dev < 64 && !done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
     if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
-    attr_set[dev] = true;
+    done[dev] = true;
   }
-  const size_t smem = t_smem(p.nt);
+  return QDQ_OK;
+}
+
+template <int kDtype, bool kGrouped>
+int launch_gemm(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, const CUtensorMap& tsf, const GemmArgs& p,
+                bool pair, int64_t items, cudaStream_t s) {
+  if (pair) {
+    static bool done[64] = {false};
+    if (int st = allow_smem(who, &mxf8_pair_kernel<kDtype, kGrouped>, done)) return st;
+    const int tok_rows = (p.nt / 2 + p.box - 1) / p.box * p.box;
+    const int64_t pairs = std::min<int64_t>(items, device_sm_count() / 2);
+    return launch_pdl(who, &mxf8_pair_kernel<kDtype, kGrouped>, 2 * pairs, T_THREADS, p_smem(tok_rows), s, 2, tw, ta, tsf, p);
+  }
+  static bool done[64] = {false};
+  if (int st = allow_smem(who, &mxf8_gemm_kernel<kDtype, kGrouped>, done)) return st;
   return launch_pdl(who, &mxf8_gemm_kernel<kDtype, kGrouped>, std::min<int64_t>(items, device_sm_count()), T_THREADS,
-                    smem, s, tw, ta, p);
+                    t_smem(p.nt), s, 1, tw, ta, p);
 }
 
 // How a few-rows launch splits: `split` CTAs of a cluster share an item's K so
@@ -943,33 +1283,10 @@ FewPlan few_plan(int64_t items, int rows, int64_t K, int act) {
 template <int kDtype, bool kGrouped, int kAct>
 int launch_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, const FewArgs& p, int64_t items,
                size_t smem, cudaStream_t s) {
-  static bool attr_set[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64 && !attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(&mxf8_few_rows_kernel<kDtype, kGrouped, kAct>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
-    if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: smem attribute: %s", who, cudaGetErrorString(e));
-    attr_set[dev] = true;
-  }
-  cudaLaunchConfig_t cfg;
-  std::memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(items * p.split));
-  cfg.blockDim = dim3(F_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = p.split;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.split > 1 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mxf8_few_rows_kernel<kDtype, kGrouped, kAct>, tw, ta, p);
-  if (e != cudaSuccess) return fail(QDQ_ERR_CUDA, "%s: launch: %s", who, cudaGetErrorString(e));
-  return check_launch(who);
+  static bool done[64] = {false};
+  if (int st = allow_smem(who, &mxf8_few_rows_kernel<kDtype, kGrouped, kAct>, done)) return st;
+  return launch_pdl(who, &mxf8_few_rows_kernel<kDtype, kGrouped, kAct>, items * p.split, F_THREADS, smem, s, p.split, tw,
+                    ta, p);
 }
 
 template <bool kGrouped, int kAct>
@@ -984,14 +1301,34 @@ int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewAr
                                  : launch_few<QDQ_DTYPE_BF16, kGrouped, kAct>(who, tw, ta, p, items, f.smem, s);
 }
 
-// Rows per item for `rows` wanted, in whole TMA boxes of 64, 32 or 16 rows: a
-// large box costs the producer fewer issues (60 cycles each), a small one a
-// ragged segment fewer idle rows.
-void rows_per_item(GemmArgs& p, int64_t rows, bool grouped) {
-  const int want = static_cast<int>(std::min<int64_t>(rows, NT_MAX));
-  p.box = want > 96 ? 64 : want > 16 ? 32 : 16;
-  p.nt = (want + p.box - 1) / p.box * p.box;
-  if (!grouped) p.box = p.nt;  // one tile's rows in one box
+// Which tiled kernel a dense product takes, and its rows per item.  The cycles
+// of a K-128 stage are the largest of its MMAs' (2 per activation row), its
+// operand bytes at 80 a cycle and its issue (300, pairs 430), plus 80; the
+// launch takes as many stages as the busiest SM has items.  Against the best
+// of five forced choices the rule's was within 5 % on 12 of 14 shapes, e.g.
+// [4096 x 4096 -> 14336] pairs of 240 rows 171 us, of 128 about 210, single
+// CTAs of 192 rows 209; [4096 x 1024 -> 512] single CTAs of 128 rows 8.2 us,
+// pairs 10.2.
+struct TilePlan {
+  bool pair;
+  int nt;
+};
+TilePlan tile_plan(int64_t M, int64_t blocks) {
+  TilePlan best = {false, 0};
+  double least = 0;
+  const int64_t sms = device_sm_count();
+  for (int pair = 0; pair < 2; ++pair) {
+    for (int nt = 16; nt <= (pair ? P_NT_MAX : NT_MAX); nt += 16) {
+      const int64_t items = (M + nt - 1) / nt * (pair ? (blocks + 1) / 2 : blocks), units = pair ? sms / 2 : sms;
+      const double bytes = T_W + nt * TK * (pair ? 0.5 : 1.0);
+      const double cost = static_cast<double>((items + units - 1) / units) * (std::max(std::max(2.0 * nt, bytes / 80.0), pair ? 430.0 : 300.0) + 80.0);
+      if (best.nt == 0 || cost < least) {
+        best = {pair != 0, nt};
+        least = cost;
+      }
+    }
+  }
+  return best;
 }
 
 int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
@@ -1094,15 +1431,21 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
   p.top_k = 1;
   p.a_rows = p.M;
-  rows_per_item(p, M, false);
+  p.pairs = N % 2 == 0 && ldc % 2 == 0 && !off(c, 4);
+  const int64_t blocks = (N + TM - 1) / TM;
+  const TilePlan plan = tile_plan(M, blocks);
+  p.nt = plan.nt;
+  p.box = plan.pair ? plan.nt / 2 : plan.nt;  // one tile's rows in one box
   p.status = status;
-  CUtensorMap tw, ta;
+  CUtensorMap tw, ta, tsf = {};
   if (int st = make_tmap_u8_2d(&tw, w_codes, N, K, ldw, TK, TM, 128)) return st;
   if (int st = make_tmap_u8_2d(&ta, a_codes, M, K, lda, TK, p.box, 128)) return st;
-  const int64_t items = ((M + p.nt - 1) / p.nt) * ((N + TM - 1) / TM);
+  if (plan.pair)
+    if (int st = make_tmap_u32_2d(&tsf, w_sf_tiled, blocks * p.kchunks, 128, 512, 128, 4)) return st;
+  const int64_t items = ((M + p.nt - 1) / p.nt) * (plan.pair ? (blocks + 1) / 2 : blocks);
   if (items >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
-  return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, p, items, s)
-                                     : launch_gemm<QDQ_DTYPE_BF16, false>(who, tw, ta, p, items, s);
+  return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, tsf, p, plan.pair, items, s)
+                                     : launch_gemm<QDQ_DTYPE_BF16, false>(who, tw, ta, tsf, p, plan.pair, items, s);
 }
 
 extern "C" int64_t fp8_linear_workspace_bytes(int64_t M, int64_t K) {
@@ -1213,10 +1556,17 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   uint8_t* scales = codes + up256(num_sorted * K);
   const int64_t ldso = qdq_mxfp8_scale_stride(K);
   GemmArgs p = {};
-  // Rows per item: the average expert's, rounded up to whole blocks, so that few rows leave the shared memory to
-  // more stages of W in flight; never less than a block.
+  // Pairs, unless an odd last W block would leave more than 6 % of their work idle (they gain 4 to 8 %).  Rows per
+  // item: the average expert's, rounded up to whole blocks (few rows leave the shared memory to more stages of W in
+  // flight), in boxes that leave a ragged segment few idle rows.
+  const bool pair = 100 * ((n_tiles + 1) / 2 * 2) <= 106 * n_tiles;
+  const int most = pair ? P_NT_MAX : NT_MAX;
   const int64_t average = (num_sorted + num_experts - 1) / num_experts;
-  rows_per_item(p, (average + moe_block_size - 1) / moe_block_size * moe_block_size, true);
+  const int64_t wanted = (average + moe_block_size - 1) / moe_block_size * moe_block_size;
+  p.nt = static_cast<int>((std::min<int64_t>(wanted, most) + 15) / 16 * 16);
+  const int held = pair ? p.nt / 2 : p.nt;  // rows in one CTA's shared memory
+  p.box = held > 96 ? 64 : held > 16 ? 32 : held > 8 ? 16 : 8;
+  if (!pair) p.nt = (p.nt + p.box - 1) / p.box * p.box;
   const int nbmax = p.nt / moe_block_size;
   {
     const int warps = SEG_THREADS / 32;
@@ -1224,7 +1574,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
     auto* fn = a == nullptr ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, false>
                : dtype == QDQ_DTYPE_FP16 ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_FP16, true>
                                          : &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, true>;
-    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, static_cast<const uint8_t*>(a ? a : a_codes),
+    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, 1, static_cast<const uint8_t*>(a ? a : a_codes),
                             a ? lda * 2 : ldac, static_cast<const uint8_t*>(a_scales), lds, sorted_token_ids,
                             expert_ids, num_tokens_post_padded, moe_block_size, num_blocks, num_experts, nbmax, top_k,
                             n_slots, K, codes, scales, ldso, seg_tab, 0.0f))
@@ -1238,6 +1588,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.c = c;
   p.ldc = ldc;
   p.seg_tab = seg_tab;
+  p.pairs = N % 2 == 0 && ldc % 2 == 0 && !off(c, 4);
   p.sorted_ids = sorted_token_ids;
   p.expert_ids = expert_ids;
   p.topk_w = mul_topk_weights ? topk_weights : nullptr;
@@ -1251,6 +1602,10 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.num_experts = static_cast<int>(num_experts);
   p.status = status;
   if (int st = make_tmap_u8_2d(&ta, codes, num_sorted, K, K, TK, p.box, 128)) return st;
-  return dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, true>(who, tw, ta, p, num_blocks * n_tiles, s)
-                                 : launch_gemm<QDQ_DTYPE_BF16, true>(who, tw, ta, p, num_blocks * n_tiles, s);
+  CUtensorMap tsf = {};
+  if (pair)
+    if (int st = make_tmap_u32_2d(&tsf, w_sf_tiled, num_experts * (p.sf_per_expert / 512), 128, 512, 128, 4)) return st;
+  const int64_t items = num_blocks * (pair ? (n_tiles + 1) / 2 : n_tiles);
+  return dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, true>(who, tw, ta, tsf, p, pair, items, s)
+                                 : launch_gemm<QDQ_DTYPE_BF16, true>(who, tw, ta, tsf, p, pair, items, s);
 }
