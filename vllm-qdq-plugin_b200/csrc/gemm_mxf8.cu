@@ -1106,8 +1106,8 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // ---------------------------------------------------------------------------
 constexpr int SEG_THREADS = 1024;
 
-__device__ void build_segments(const int32_t* __restrict__ expert_ids, int live, int bs, int num_experts, int nbmax,
-                               int32_t* __restrict__ seg_tab) {
+__device__ void build_segments(const int32_t* __restrict__ expert_ids, const int32_t* __restrict__ sorted_ids, int live,
+                               int bs, int num_experts, int n_slots, int nbmax, int32_t* seg_tab) {
   __shared__ int s_start[32], s_count[32];
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5, nw = blockDim.x >> 5;
   int carry_start = -1, carry_count = 0;
@@ -1147,6 +1147,23 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, int live,
     __syncthreads();
   }
   if (t == 0) seg_tab[0] = carry_count;
+  // Padding at a segment's end costs MMAs and loads in steps of 16 rows: cut it, a warp a segment.
+  if (bs > 16) {
+    for (int i = wid; i < carry_count; i += nw) {
+      int4* entry = reinterpret_cast<int4*>(seg_tab + 4) + i;
+      int4 e = *entry;
+      while (e.y > 0) {
+        const int r = e.y - 1 - lane, s = r >= 0 ? __ldcg(sorted_ids + e.x + r) : -1;
+        const unsigned live_rows = __ballot_sync(0xffffffffu, s >= 0 && s < n_slots);
+        if (live_rows != 0) {
+          e.y -= __ffs(live_rows) - 1;
+          break;
+        }
+        e.y = max(0, e.y - 32);
+      }
+      if (lane == 0) *entry = e;
+    }
+  }
 }
 
 // The pass before the grouped product: block 0 builds the segments, the others
@@ -1161,13 +1178,13 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
                         int64_t lds, const int32_t* __restrict__ sorted_ids, const int32_t* __restrict__ expert_ids,
                         const int32_t* __restrict__ num_post_padded, int bs, int num_blocks, int num_experts,
                         int nbmax, int top_k, int n_slots, int K, uint8_t* __restrict__ codes,
-                        uint8_t* __restrict__ scales, int64_t ldso, int32_t* __restrict__ seg_tab, float zero) {
+                        uint8_t* __restrict__ scales, int64_t ldso, int32_t* seg_tab, float zero) {
   pdl_launch_dependents();
   pdl_wait();
   const int npp = __ldcg(num_post_padded);
   const int live = npp <= 0 ? 0 : min(num_blocks, (npp - 1) / bs + 1);
   if (blockIdx.x == 0) {
-    build_segments(expert_ids, live, bs, num_experts, nbmax, seg_tab);
+    build_segments(expert_ids, sorted_ids, live, bs, num_experts, n_slots, nbmax, seg_tab);
     return;
   }
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;

@@ -338,9 +338,13 @@ __device__ __forceinline__ void mx8_codes(const uint32_t (&w)[kW], int e, float 
 // all-ones exponent, as an infinity does.
 template <int kDtype, int kW>
 __device__ __forceinline__ uint32_t absmax_words(const uint32_t (&w)[kW]) {
-  uint32_t m = w[0] & 0x7FFF7FFFu;
+  uint32_t m = w[0];
 #pragma unroll
-  for (int j = 1; j < kW; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+  for (int j = 1; j < kW; ++j) {  // |m| = max(|m|, |w|); the sign is dropped below
+    if (kDtype == QDQ_DTYPE_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[j]));
+    else asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m) : "r"(w[j]));
+  }
+  m &= 0x7FFF7FFFu;
   return max(m & 0xFFFFu, m >> 16);
 }
 

@@ -96,12 +96,17 @@ __device__ __forceinline__ float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// silu(g) * u: with t = exp(-|g|), silu(g) = g (g < 0 ? t : 1) / (1 + t), which
-// overflows nowhere.  t and 1 are carried times 2^24, so that ex2 (which
-// flushes subnormals) reaches down to |g| = 104, where silu is below 2^-140.
-__device__ __forceinline__ float silu_mul(float g, float u) {
-  const float t = ex2_approx(fmaf(-1.44269504088896341f, fabsf(g), 24.0f));
-  return g * ((g < 0.f ? t : 0x1p24f) * rcp_approx(t + 0x1p24f)) * u;
+// silu(g) * u of a pair: with t = exp(-|g|), silu(g) = g (g < 0 ? t : 1) /
+// (1 + t), which overflows nowhere.  t and 1 are carried times 2^24, so that
+// ex2 (which flushes subnormals) reaches down to |g| = 104, where silu is below
+// 2^-140.
+__device__ __forceinline__ float2 silu_mul(float2 g, float2 u) {
+  const float tx = ex2_approx(fmaf(-1.44269504088896341f, fabsf(g.x), 24.0f));
+  const float ty = ex2_approx(fmaf(-1.44269504088896341f, fabsf(g.y), 24.0f));
+  const float2 n = make_float2(g.x < 0.f ? tx : 0x1p24f, g.y < 0.f ? ty : 0x1p24f);
+  const float2 d = add_f32x2(make_float2(tx, ty), make_float2(0x1p24f, 0x1p24f));
+  const float2 s = mul_f32x2(n, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+  return mul_f32x2(mul_f32x2(g, s), u);
 }
 
 // ---------------------------------------------------------------------------
@@ -145,8 +150,10 @@ rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, u
       uint32_t u8[8];
       words(u, u8);
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        y[j] = F::pack(silu_mul(F::lo(y[j]), F::lo(u8[j])), silu_mul(F::hi(y[j]), F::hi(u8[j])));
+      for (int j = 0; j < 8; ++j) {
+        const float2 s = silu_mul(make_float2(F::lo(y[j]), F::hi(y[j])), make_float2(F::lo(u8[j]), F::hi(u8[j])));
+        y[j] = F::pack(s.x, s.y);
+      }
     }
     store_mxfp8<kDtype>(y, cr, sr, col, upr, in_m && col < upr, zero);
     v = vn;

@@ -5,6 +5,7 @@
 // where the host's time is the call's time, so they are C++ rather than ctypes:
 // on the measured host one norm call takes 8 us instead of 25 (GPU time 2.1).
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -35,8 +36,12 @@ int64_t ld(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 void* ptr(const Tensor& t) { return const_cast<void*>(t.const_data_ptr()); }
 void* ptr(const std::optional<Tensor>& t) { return t.has_value() ? ptr(*t) : nullptr; }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
-Tensor bytes(int64_t m, int64_t n, const Tensor& like) { return at::empty({m, n}, like.options().dtype(at::kByte)); }
-Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
+// Straight from torch's caching allocator, without the dispatcher.
+Tensor empty(at::IntArrayRef size, at::ScalarType dtype, const Tensor& like) {
+  return at::detail::empty_cuda(size, dtype, like.device(), std::nullopt);
+}
+Tensor bytes(int64_t m, int64_t n, const Tensor& like) { return empty({m, n}, at::kByte, like); }
+Tensor bytes(int64_t n, const Tensor& like) { return empty({n}, at::kByte, like); }
 
 // What the C ABI cannot see of its pointers: shapes, types and devices.
 void check_16bit(const char* name, const Tensor& x) {
@@ -109,11 +114,11 @@ std::vector<Tensor> rmsnorm_mxfp8(const Tensor& x_, const Tensor& weight, const 
   out.push_back(bytes(m, k, x));
   out.push_back(bytes(m, lds, x));
   if (r.defined()) {
-    out.push_back(at::empty({m, k}, x.options()));
+    out.push_back(empty({m, k}, x.scalar_type(), x));
     h = ptr(out.back());
   }
   if (norm_out) {
-    out.push_back(at::empty({m, k}, x.options()));
+    out.push_back(empty({m, k}, x.scalar_type(), x));
     y = ptr(out.back());
   }
   check("qdq_rmsnorm_mxfp8",
@@ -138,7 +143,7 @@ Tensor mxfp8_linear(const Tensor& a_, const Tensor& w, const Tensor& sf, const s
   const c10::cuda::CUDAGuard guard(a_.device());
   const Tensor a = rows16(a_), b = dense_as(bias, a.scalar_type());
   const int64_t m = a.size(0), k = a.size(1), n = w.size(0), need = fp8_linear_workspace_bytes(m, k);
-  Tensor ws = bytes(need, a), out = at::empty({m, n}, a.options());
+  Tensor ws = bytes(need, a), out = empty({m, n}, a.scalar_type(), a);
   check("fp8_linear_mxf8", fp8_linear_mxf8(ptr(a), ld(a), dtype_code(a), ptr(w), ptr(sf), ptr_or_null(b), ptr(out), m, n,
                                            k, ld(w), n, ptr(ws), need, stream()));
   return out;
@@ -152,7 +157,7 @@ Tensor mxfp8_linear_rows(const Tensor& codes, const Tensor& scales, const Tensor
   const auto dtype = out_fp16 ? at::kHalf : at::kBFloat16;
   const Tensor b = dense_as(bias, dtype);
   const int64_t m = codes.size(0), k = codes.size(1), n = w.size(0);
-  Tensor out = at::empty({m, n}, codes.options().dtype(dtype));
+  Tensor out = empty({m, n}, dtype, codes);
   check("fp8_gemm_mxf8",
         fp8_gemm_mxf8(ptr(codes), ptr(scales), ld(codes), ld(scales), ptr(w), ptr(sf), ptr_or_null(b), ptr(out), m, n, k,
                       ld(w), n, out_fp16 ? QDQ_DTYPE_FP16 : QDQ_DTYPE_BF16, stream()));
@@ -203,7 +208,7 @@ Tensor mxfp8_moe_linear(const Tensor& a, const std::optional<Tensor>& a_scales, 
                         const std::optional<Tensor>& topk_weights, int64_t block, int64_t top_k, bool out_fp16) {
   TORCH_CHECK(a.dim() == 2 && w.dim() == 3 && top_k >= 1, "mxfp8_moe_linear: [M, K] rows, [E, N, K] weights");
   const c10::cuda::CUDAGuard guard(a.device());
-  Tensor out = at::empty({a.size(0) * top_k, w.size(1)}, a.options().dtype(out_fp16 ? at::kHalf : at::kBFloat16));
+  Tensor out = empty({a.size(0) * top_k, w.size(1)}, out_fp16 ? at::kHalf : at::kBFloat16, a);
   mxfp8_moe_linear_out(a, a_scales, w, sf, sorted_ids, expert_ids, num_post_padded, topk_weights, block, top_k, out);
   return out;
 }

@@ -74,7 +74,7 @@ def _torch_ops_commands(obj: Path, out: Path) -> tuple[list[str], list[str]]:
     # The shared libstdc++ by name: a toolchain that links a static one in would give this library its own exception
     # machinery, and an error it raises would end the process instead of reaching Python.
     link_cmd = [cxx, "-shared", "-nostdlib++", "-o", str(out), str(obj), "-l:libstdc++.so.6", f"-L{LIB_DIR}", "-lqdq_b200",
-                *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
+                *(f"-L{p}" for p in cpp_extension.library_paths()), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
                 "-Wl,-rpath,$ORIGIN"]
     return compile_cmd, link_cmd
 
