@@ -29,6 +29,7 @@
 // TMEM, so an item's epilogue overlaps the next item's MMAs.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "mx_quant.cuh"
 #include "sm100.cuh"
@@ -951,20 +952,34 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     for (int kt = 0; kt < nkt;) {
       const int need = kAct == kTiles ? 1 : (kt + 1) * F_CHUNKS * rows;
       for (; ok && covered < need; covered += F_BATCH) ok = mbar_wait(&bars->ready[batches++], 0, p.status, 0x703);
-      const Cursor one = at;
-      at.next(p.ring);
-      const Cursor two = at;
-      const bool pair = ok && kt + 1 < nkt && (kAct == kTiles || covered >= need + F_CHUNKS * rows) &&
-                        __all_sync(0xffffffffu, mbar_test2(&bars->full[one.slot], one.phase, &bars->full[two.slot], two.phase));
-      if (!pair) ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->full[one.slot], one.phase, p.status, 0x704));
+      // four, two or one stage, as many as are full: the loop around them costs as much as two stages' issue
+      const int more = min(nkt - kt, kAct == kTiles ? 4 : (covered - need) / max(1, F_CHUNKS * rows) + 1);
+      Cursor c[4] = {at, at, at, at};
+#pragma unroll
+      for (int i = 1; i < 4; ++i) {
+        c[i] = c[i - 1];
+        c[i].next(p.ring);
+      }
+      int n = 1;
+      if (ok && more >= 4 && p.ring >= 4 &&
+          __all_sync(0xffffffffu, mbar_test4(&bars->full[c[0].slot], c[0].phase, &bars->full[c[1].slot], c[1].phase,
+                                             &bars->full[c[2].slot], c[2].phase, &bars->full[c[3].slot], c[3].phase)))
+        n = 4;
+      else if (ok && more >= 2 && p.ring >= 2 &&
+               __all_sync(0xffffffffu, mbar_test2(&bars->full[c[0].slot], c[0].phase, &bars->full[c[1].slot], c[1].phase)))
+        n = 2;
+      else
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(&bars->full[c[0].slot], c[0].phase, p.status, 0x704));
       if (!ok) break;
       tc_fence_after();
       if (leader) {
-        stage(kt, one.slot);
-        if (pair) stage(kt + 1, two.slot);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < n) stage(kt + i, c[i].slot);
       }
-      if (pair) at.next(p.ring);
-      kt += pair ? 2 : 1;
+      at = n == 4 ? c[3] : n == 2 ? c[1] : c[0];
+      at.next(p.ring);
+      kt += n;
     }
     if (!ok) bars->abort = 1;
     if (leader) tc_commit(&bars->acc_full);  // also on abort: the epilogue waits for the issued MMAs
@@ -1060,32 +1075,44 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   if (p.split > 1) cluster_sync();  // every CTA's partials are in its shared memory
   else __syncthreads();
   if (warp >= 2 && ok) {
-    // thread: one of this CTA's W rows, every `step`-th activation row
-    const int shift = __ffs(TM / p.split) - 1, t = threadIdx.x - 64, step = F_FILL >> shift;
-    const int row = (rank << shift) + (t & ((1 << shift) - 1)), n = n_tile * TM + row;
-    T* C = static_cast<T*>(p.c) + n;
-    const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
-#pragma unroll 2
-    for (int r = t >> shift; r < rows && n < p.N; r += step) {
-      float v;
-      if (p.split == 1) {
-        v = part[r * TM + row];
-      } else {
-        float x[8];
+    const float* mine = part;
+    auto add_up = [&](auto split_c) {  // split_c partials of each sum, 16 loads in flight a thread
+      constexpr int kSplit = decltype(split_c)::value, kU = kSplit == 1 ? 8 : 16 / kSplit;
+      // thread: one of this CTA's W rows, every `step`-th activation row
+      constexpr int kShare = TM / kSplit, step = F_FILL / kShare;
+      const int t = threadIdx.x - 64, row = rank * kShare + t % kShare, n = n_tile * TM + row;
+      if (n >= p.N) return;
+      T* C = static_cast<T*>(p.c) + n;
+      const float bias = (!kGrouped && p.bias != nullptr) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+#pragma unroll 1
+      for (int r0 = t / kShare; r0 < rows; r0 += step * kU) {
+        float x[kU][kSplit];
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          if (c < p.split)
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[c]) : "r"(cluster_addr(part + r * TM + row, c)));
-        v = x[0];
+        for (int u = 0; u < kU; ++u)
 #pragma unroll
-        for (int c = 1; c < 8; ++c)
-          if (c < p.split) v += x[c];
+          for (int c = 0; c < kSplit; ++c) {
+            const float* from = mine + min(r0 + u * step, rows - 1) * TM + row;
+            if (kSplit == 1) x[u][c] = *from;
+            else asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[u][c]) : "r"(cluster_addr(from, c)));
+          }
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int r = r0 + u * step;
+          if (r >= rows) break;
+          float v = x[u][0];
+#pragma unroll
+          for (int c = 1; c < kSplit; ++c) v += x[u][c];
+          const int64_t s = kGrouped ? bars->slot[r] : row0 + r;
+          if (kGrouped) v *= p.topk_w != nullptr ? __ldcg(p.topk_w + s) : 1.0f;
+          else v += bias;
+          C[s * p.ldc] = O::one(v);
+        }
       }
-      const int64_t s = kGrouped ? bars->slot[r] : row0 + r;
-      if (kGrouped) v *= p.topk_w != nullptr ? __ldcg(p.topk_w + s) : 1.0f;
-      else v += bias;
-      C[s * p.ldc] = O::one(v);
-    }
+    };
+    if (p.split == 1) add_up(std::integral_constant<int, 1>());
+    else if (p.split == 2) add_up(std::integral_constant<int, 2>());
+    else if (p.split == 4) add_up(std::integral_constant<int, 4>());
+    else add_up(std::integral_constant<int, 8>());
   }
   if (p.split > 1) {
     __syncwarp();

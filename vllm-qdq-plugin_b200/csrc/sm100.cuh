@@ -68,6 +68,25 @@ __device__ __forceinline__ bool mbar_test2(uint64_t* bar0, uint32_t parity0, uin
       : "memory");
   return ok != 0;
 }
+// The same for four barriers.
+__device__ __forceinline__ bool mbar_test4(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2,
+                                           uint64_t* b3, uint32_t p3) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r, s;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 s, [%7], %8;\n\t"
+      "and.pred p, p, q;\n\t"
+      "and.pred r, r, s;\n\t"
+      "and.pred p, p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b0)), "r"(p0), "r"(smem_u32(b1)), "r"(p1), "r"(smem_u32(b2)), "r"(p2), "r"(smem_u32(b3)), "r"(p3)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ uint64_t global_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
