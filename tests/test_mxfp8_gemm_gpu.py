@@ -321,3 +321,98 @@ def test_operators_trace_under_compile(cuda_device):
     want = layer(x, x)
     got = torch.compile(layer, backend="eager", fullgraph=True)(x, x)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_broadcast_rows_and_parameters(cuda_device):
+    """Expanded activations are copied, not misread; norm weights that are parameters are taken as they are."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows, rmsnorm_mxfp8
+    dev, m, k = cuda_device, 24, 96
+    one = activation(1, k, torch.bfloat16, 1, dev)
+    wide, dense = one.expand(m, k), one.repeat(m, 1)
+    g = torch.nn.Parameter(torch.randn(k, device=dev).to(torch.bfloat16))
+    assert torch.equal(mxfp8_rows(wide).codes, mxfp8_rows(dense).codes)
+    assert torch.equal(rmsnorm_mxfp8(wide, g, wide)[1], rmsnorm_mxfp8(dense, g.detach(), dense)[1])
+    w = prepare_mxfp8_weight(*random_weight(130, k, seed=1, dev=dev))
+    assert torch.equal(mxfp8_linear(wide, w), mxfp8_linear(dense, w))
+    wm = prepare_mxfp8_moe_weight(*random_weight(2, 130, k, seed=1, dev=dev))
+    _, sid, eid, ntp, tw = routing(m, 2, 2, 16, 1, dev)
+    both = [mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 2, True) for x in (wide, dense)]
+    assert torch.equal(*both)
+    _ok()
+
+
+def test_chains_of_small_calls(cuda_device):
+    """Many short kernels in flight behind one another, each reading what the one before wrote: eager and captured."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import rmsnorm_mxfp8, silu_mul_mxfp8
+    dev, m, k = cuda_device, 4, 256
+    g = torch.ones(k, dtype=torch.bfloat16, device=dev)
+    ups = [prepare_mxfp8_weight(*random_weight(2 * k, k, seed=i, dev=dev)) for i in range(4)]
+    downs = [prepare_mxfp8_weight(*random_weight(k, k, seed=9 + i, dev=dev)) for i in range(4)]
+
+    def layers(x, wait):
+        h = x
+        for i in range(24):
+            rows, h, _ = rmsnorm_mxfp8(x, g, h)
+            wait()
+            up = mxfp8_linear(rows, ups[i % 4])
+            wait()
+            act = silu_mul_mxfp8(up)
+            wait()
+            x = mxfp8_linear(act, downs[i % 4])
+            wait()
+            x = mxfp8_linear(x, downs[(i + 1) % 4])
+            wait()
+        return x, h
+
+    x = activation(m, k, torch.bfloat16, 1, dev)
+    want = layers(x, torch.cuda.synchronize)
+    for _ in range(20):
+        got = layers(x, lambda: None)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layers(x, lambda: None)
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want)) and want[0].isfinite().all()
+    _ok()
+
+
+def test_first_call_of_a_process_inside_a_capture(tmp_path):
+    """Nothing has to run before a capture: not the library's load, nor a kernel's first launch."""
+    import subprocess
+    import sys
+    from conftest import REPO
+    script = tmp_path / "first.py"
+    script.write_text(f"""
+import sys
+sys.path[:0] = [{str(REPO / "vllm-qdq-plugin_b200")!r}, {str(REPO)!r}, {str(REPO / "tests")!r}]
+import torch
+from mxfp8_cases import activation, random_weight, routing
+from vllm_qdq_plugin.gemm import Mxfp8MoeWeight, Mxfp8Weight, mxfp8_linear, mxfp8_moe_linear
+from vllm_qdq_plugin.qdq import rmsnorm_mxfp8
+dev = torch.device("cuda", 0)
+x = activation(40, 256, torch.bfloat16, 1, dev)
+g = torch.ones(256, dtype=torch.bfloat16, device=dev)
+codes, scales = random_weight(2, 512, 256, seed=1, dev=dev)
+sf = torch.full((2 * 512 * 8,), 118, dtype=torch.uint8, device=dev)
+w, wm = Mxfp8Weight(codes[0], sf, 512, 256), Mxfp8MoeWeight(codes, sf, 2, 512, 256)
+_, sid, eid, ntp, tw = routing(40, 2, 1, 16, 1, dev)
+big = activation(700, 256, torch.bfloat16, 2, dev)
+torch.cuda.synchronize()
+def run():
+    rows = rmsnorm_mxfp8(x, g)[0]
+    return mxfp8_linear(rows, w), mxfp8_linear(big, w), mxfp8_moe_linear(rows, wm, sid, eid, ntp, tw, 16, 1, True)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run())) and all(o.isfinite().all() for o in out)
+print("ok")
+""")
+    done = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "ok" in done.stdout, done.stderr[-2000:]

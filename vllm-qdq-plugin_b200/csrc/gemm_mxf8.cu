@@ -854,7 +854,6 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   const int num_kt = (p.K + TK - 1) / TK;
   const int kt0 = rank * p.kt_per, nkt = max(0, min(p.kt_per, num_kt - kt0));
 
-  pdl_launch_dependents();
   int expert = 0;
   if (kGrouped) {
     pdl_wait();  // the routing may come from the kernel before
@@ -903,6 +902,9 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Only now may the next kernel start: were it let in before this CTA's
+  // tcgen05.alloc, it could hold the tensor memory that this one waits for.
+  pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);  // uniform
   const int rows = kGrouped ? bars->live : min(p.rows, p.M - row0);
 

@@ -25,10 +25,11 @@ int dtype_code(const Tensor& t) {
   return t.scalar_type() == at::kHalf ? QDQ_DTYPE_FP16 : QDQ_DTYPE_BF16;
 }
 
-// The tensor, or a copy whose rows start on 16-byte boundaries with unit element stride.
+// The tensor, or a copy whose rows are apart (not broadcast) and start on 16-byte boundaries with unit element stride.
 Tensor rows16(const Tensor& t) {
   const bool dense = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 &&
-                     (t.dim() < 2 || t.size(0) <= 1 || t.stride(0) * t.element_size() % 16 == 0);
+                     (t.dim() < 2 || t.size(0) <= 1 ||
+                      (t.stride(0) >= t.size(1) && t.stride(0) * t.element_size() % 16 == 0));
   return dense ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 

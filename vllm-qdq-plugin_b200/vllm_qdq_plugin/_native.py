@@ -198,8 +198,9 @@ def same_device(device: torch.device, *tensors: torch.Tensor | None) -> None:
 
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy of it whose rows start on 16-byte boundaries with unit element stride."""
-    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[0] <= 1 or x.stride(0) * x.element_size() % 16 == 0):
+    """x, or a copy of it whose rows are apart (not broadcast) and start on 16-byte boundaries with unit element stride."""
+    if x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and (
+            x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) * x.element_size() % 16 == 0)):
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
