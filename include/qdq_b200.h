@@ -375,10 +375,12 @@ int fp4_moe_mxf4(const void* a, int64_t lda, int dtype, const void* w_codes, con
  * them.  They serve the float8_e4m3fn layers, whose activations the reference
  * only quant-dequantises (vllm_qdq_plugin/patch.py:61-67, :150-152).
  *
- * MXFP8 rows: codes [M, K] E4M3 bytes (row stride ldc) and scales [M, lds]
- * E8M0 bytes, row-major: K / 32 scales of a row, then zeros up to a multiple
- * of 16.  lds >= qdq_mxfp8_scale_stride(K); base addresses and row strides of
- * codes and scales are multiples of 16 bytes; K % 32 == 0.
+ * MXFP8 rows: codes [M, K] E4M3 bytes (row stride ldc) and scales, E8M0 bytes,
+ * K / 32 a row (row stride lds).  Base addresses and row strides of codes and
+ * scales are multiples of 16 bytes and lds >= qdq_mxfp8_scale_stride(K): the
+ * products read a row's scales 16 at a time, so the bytes behind K / 32 up to
+ * that stride are read (the last row's too); their values have no effect.
+ * K % 32 == 0.
  * ------------------------------------------------------------------------- */
 
 /* K / 32 rounded up to a multiple of 16: the least lds of MXFP8 rows. */

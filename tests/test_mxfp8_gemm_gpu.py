@@ -63,9 +63,9 @@ def test_linear_takes_strided_rows_and_its_weights_bias(cuda_device):
     assert torch.equal(mxfp8_linear(torch.nn.functional.pad(a, (3, 0))[:, 3:], w), want)
     held = torch.full((m, k + 64), 0x7F, dtype=torch.uint8, device=cuda_device)  # NaN codes behind every row
     held[:, :k] = rows.codes
-    stored = torch.full((m, rows.stored.shape[1] + 16), 0xFF, dtype=torch.uint8, device=cuda_device)
-    stored[:, : rows.stored.shape[1]] = rows.stored
-    view = Mxfp8Rows(held[:, :k], stored[:, : rows.stored.shape[1]], torch.bfloat16)
+    stored = torch.full((m, 48), 0xFF, dtype=torch.uint8, device=cuda_device)  # and NaN scales
+    stored[:, : k // 32] = rows.scales
+    view = Mxfp8Rows(held[:, :k], stored[:, : k // 32], torch.bfloat16)
     assert torch.equal(mxfp8_linear(view, w), want)
     wpad = torch.full((n, k + 16), 0x7F, dtype=torch.uint8, device=cuda_device)
     wpad[:, :k] = codes
@@ -278,8 +278,9 @@ def test_refusals_name_the_argument(cuda_device):
         lambda: Mxfp8Rows.from_codes(rows.codes, rows.scales[:, :1]), lambda: Mxfp8Rows.from_codes(rows.codes.view(torch.int8), rows.scales),
         lambda: Mxfp8Rows.from_codes(rows.codes, rows.scales, torch.float32),
         lambda: mxfp8_linear(x.float(), w), lambda: mxfp8_linear(x[:, :32], w), lambda: mxfp8_linear(x, w, g),
-        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.scales, rows.dtype), w),
-        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.stored[:4], rows.dtype), w),
+        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.scales.contiguous(), rows.dtype), w),
+        lambda: mxfp8_linear(Mxfp8Rows(rows.codes, rows.scales[:4], rows.dtype), w),
+        lambda: mxfp8_linear(Mxfp8Rows(rows.codes[:1], rows.scales[:1].contiguous().clone(), rows.dtype), w),
         lambda: mxfp8_linear(x, dataclasses.replace(w, codes=w.codes.cpu())),
         lambda: prepare_mxfp8_weight(w.codes, rows.scales), lambda: prepare_mxfp8_moe_weight(w.codes, rows.scales),
         lambda: mxfp8_moe_linear(x, wm, sid.long(), eid, ntp, tw, 16, 1, False),
@@ -316,7 +317,7 @@ def test_operators_trace_under_compile(cuda_device):
     def layer(x, r):
         rows, h, _ = rmsnorm_mxfp8(x, g, r)
         act = silu_mul_mxfp8(mxfp8_linear(rows, w))
-        return act.codes, act.stored, h
+        return act.codes, act.scales, h
 
     want = layer(x, x)
     got = torch.compile(layer, backend="eager", fullgraph=True)(x, x)
@@ -416,3 +417,24 @@ print("ok")
 """)
     done = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "ok" in done.stdout, done.stderr[-2000:]
+
+
+@pytest.mark.parametrize("m,k", [(3, 2880), (70, 352), (300, 96), (2000, 544)])
+def test_padding_of_scale_rows_has_no_effect(cuda_device, m, k):
+    """The bytes between rows of scales are read and must not count, whatever they are, in every form of the product."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import Mxfp8Rows, mxfp8_rows
+    dev, n, e = cuda_device, 640, 3
+    a = activation(m, k, torch.bfloat16, 1, dev)
+    rows = mxfp8_rows(a)
+    w = prepare_mxfp8_weight(*random_weight(n, k, seed=1, dev=dev))
+    wm = prepare_mxfp8_moe_weight(*random_weight(e, n, k, seed=2, dev=dev))
+    _, sid, eid, ntp, tw = routing(m, e, 2, 32, 1, dev)
+    seen = []
+    for fill in (0x00, 0xFF, 0x7F):
+        stored = torch.full((m, (k // 32 + 15) // 16 * 16), fill, dtype=torch.uint8, device=dev)
+        stored[:, : k // 32] = rows.scales
+        r = Mxfp8Rows(rows.codes, stored[:, : k // 32], torch.bfloat16)
+        seen.append((mxfp8_linear(r, w), mxfp8_moe_linear(r, wm, sid, eid, ntp, tw, 32, 2, True)))
+    assert all(torch.equal(x, y) for s in seen[1:] for x, y in zip(s, seen[0])) and seen[0][0].isfinite().all()
+    _ok()

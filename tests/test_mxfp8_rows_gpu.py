@@ -35,8 +35,6 @@ def _quantize(y):
 def _same_rows(rows, y):
     codes, scales = _quantize(y)
     assert torch.equal(rows.codes, codes) and torch.equal(rows.scales, scales)
-    pad = rows.stored[:, y.shape[1] // 32:]
-    assert not pad.any(), "scale bytes behind K / 32 must be zero"
 
 
 def _wide(m, k, dtype, seed, dev):
@@ -81,7 +79,7 @@ def test_rows_hold_infinities_and_nan_within_their_group(cuda_device, bad):
     w = torch.ones(256, dtype=torch.bfloat16, device=cuda_device)
     a, b = rmsnorm_mxfp8(x, w)[0], rmsnorm_mxfp8(y, w)[0]
     others = torch.arange(5, device=cuda_device) != 2
-    assert torch.equal(a.codes[others], b.codes[others]) and torch.equal(a.stored[others], b.stored[others])
+    assert torch.equal(a.codes[others], b.codes[others]) and torch.equal(a.scales[others], b.scales[others])
 
 
 def test_rows_from_codes_and_strided_inputs(cuda_device):
@@ -89,7 +87,7 @@ def test_rows_from_codes_and_strided_inputs(cuda_device):
     x = _wide(37, 288, torch.bfloat16, 5, cuda_device)
     want = mxfp8_rows(x)
     rows = Mxfp8Rows.from_codes(*mxfp8_quantize(x))
-    assert torch.equal(rows.codes, want.codes) and torch.equal(rows.stored, want.stored)
+    assert torch.equal(rows.codes, want.codes) and torch.equal(rows.scales, want.scales)
     w = torch.randn(288, device=cuda_device).to(torch.bfloat16)
     for view in (torch.cat([x, x], 1)[:, :288],                       # padded rows, 16-byte aligned
                  torch.nn.functional.pad(x, (1, 2))[:, 1:289],        # rows off the 16-byte grid
@@ -97,7 +95,7 @@ def test_rows_from_codes_and_strided_inputs(cuda_device):
                  torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(37, 288)):  # base off the grid
         assert torch.equal(view, x)
         got = mxfp8_rows(view)
-        assert torch.equal(got.codes, want.codes) and torch.equal(got.stored, want.stored)
+        assert torch.equal(got.codes, want.codes) and torch.equal(got.scales, want.scales)
         a, b = rmsnorm_mxfp8(view, w, view)[:2], rmsnorm_mxfp8(x, w, x)[:2]
         assert torch.equal(a[0].codes, b[0].codes) and torch.equal(a[1], b[1])
     wide = torch.cat([x, x.flip(0), x], 1)[:, : 2 * 288]
@@ -125,7 +123,7 @@ def test_rmsnorm_against_64_bits(cuda_device, m, k, dtype, with_residual):
     assert ((y.double() - want).abs() <= bound).all()
     _same_rows(rows, y)
     again = rmsnorm_mxfp8(x, w, r, 1e-5)
-    assert again[2] is None and torch.equal(again[0].codes, rows.codes) and torch.equal(again[0].stored, rows.stored)
+    assert again[2] is None and torch.equal(again[0].codes, rows.codes) and torch.equal(again[0].scales, rows.scales)
 
 
 def test_rmsnorm_of_zero_rows_and_zero_eps(cuda_device):
@@ -206,12 +204,12 @@ def test_rows_on_another_stream_and_in_a_graph(cuda_device):
     with torch.cuda.graph(graph):
         a, b = rmsnorm_mxfp8(h, w, h)[0], silu_mul_mxfp8(x)
     for fill in (0, 255):
-        for t in (a.codes, a.stored, b.codes, b.stored):
+        for t in (a.codes, a.scales, b.codes, b.scales):
             t.fill_(fill)
         graph.replay()
         torch.cuda.synchronize()
-        assert torch.equal(a.codes, want.codes) and torch.equal(a.stored, want.stored)
-        assert torch.equal(b.codes, gate.codes) and torch.equal(b.stored, gate.stored)
+        assert torch.equal(a.codes, want.codes) and torch.equal(a.scales, want.scales)
+        assert torch.equal(b.codes, gate.codes) and torch.equal(b.scales, gate.scales)
     h.mul_(2)  # the graph reads its inputs anew
     graph.replay()
     torch.cuda.synchronize()

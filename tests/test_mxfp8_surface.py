@@ -149,11 +149,12 @@ def test_fake_kernels_give_the_shapes():
     with FakeTensorMode():
         x = torch.empty(5, 544, dtype=torch.float16, device="cuda")
         codes, scales = torch.ops.qdq_b200.mxfp8_rows(x)
-        assert codes.shape == (5, 544) and scales.shape == (5, 32) and codes.dtype == scales.dtype == torch.uint8
+        assert codes.shape == (5, 544) and scales.shape == (5, 17) and codes.dtype == scales.dtype == torch.uint8
+        assert scales.stride() == (32, 1)
         codes, scales = torch.ops.qdq_b200.silu_mul_mxfp8(x[:, :64])
-        assert codes.shape == (5, 32) and scales.shape == (5, 16)
+        assert codes.shape == (5, 32) and scales.shape == (5, 1)
         out = torch.ops.qdq_b200.rmsnorm_mxfp8(x, x[0], x, 1e-6, True)
-        assert [tuple(t.shape) for t in out] == [(5, 544), (5, 32), (5, 544), (5, 544)] and out[2].dtype == x.dtype
+        assert [tuple(t.shape) for t in out] == [(5, 544), (5, 17), (5, 544), (5, 544)] and out[2].dtype == x.dtype
         w, sf = torch.empty(7, 544, dtype=torch.uint8, device="cuda"), torch.empty(9, dtype=torch.uint8, device="cuda")
         assert torch.ops.qdq_b200.mxfp8_linear(x, w, sf, None).shape == (5, 7)
         y = torch.ops.qdq_b200.mxfp8_linear_rows(codes, scales, w, sf, None, False)

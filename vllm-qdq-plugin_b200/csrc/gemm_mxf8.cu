@@ -22,6 +22,8 @@
 //               layout that tcgen05.cp expects.  One proxy fence a quad: a
 //               fence per stage held the whole ring to 0.55 us a stage
 //   warps 6-13  epilogue: TMEM lanes = W rows, columns = activation rows
+// Scale bytes behind K / 32 (the rows' padding) are masked: their codes are
+// zeros, but zero times a stale NaN scale would not be.
 // What the kernel before it on the stream may have written (scales, routing,
 // segments) is read past L1 (__ldcg): under programmatic dependent launch this
 // kernel's CTAs start before that one has finished.
@@ -131,6 +133,23 @@ struct Cursor {
     }
   }
 };
+
+// The scale bytes of K-128 stage kt that lie inside K.
+__device__ __forceinline__ uint32_t scale_mask(int K, int kt) {
+  const int valid = max(K / 32 - 4 * kt, 0);
+  return valid >= 4 ? 0xFFFFFFFFu : (1u << (8 * valid)) - 1u;
+}
+
+template <int kR>
+__device__ __forceinline__ void mask_quad(uint4 (&v)[kR], int K, int kt) {
+#pragma unroll
+  for (int j = 0; j < kR; ++j) {
+    v[j].x &= scale_mask(K, kt);
+    v[j].y &= scale_mask(K, kt + 1);
+    v[j].z &= scale_mask(K, kt + 2);
+    v[j].w &= scale_mask(K, kt + 3);
+  }
+}
 
 struct Item {
   int row0;     // first activation row (dense) or first sorted position (grouped)
@@ -405,6 +424,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll
         for (int j = 0; j < kR; ++j)
           if (lane + 32 * j < n_mma) v[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + 16 * h));
+        if (h + 1 == quads) mask_quad(v, p.K, 4 * h);
         ok = mbar_wait(&bars->sf_empty[u], (((quad + h) / T_SCALE) & 1) ^ 1, p.status, 0x606);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
@@ -684,6 +704,7 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
 #pragma unroll
         for (int j = 0; j < kR; ++j)
           if (lane + 32 * j < n_mma) v[j] = __ldcg(reinterpret_cast<const uint4*>(src[j] + 16 * h));
+        if (h + 1 == quads) mask_quad(v, p.K, 4 * h);
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->sf_empty[u], (((quad + h) / T_SCALE) & 1) ^ 1, p.status, 0x809));
         if (!ok) break;
         uint8_t* sf = s_sfa + u * 4 * 1024;
@@ -887,6 +908,9 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   if (warp == 1) {
     tmem_alloc(&bars->tmem_base, F_TMEM);
     tmem_relinquish();
+    // Only now may the next kernel start: let in before this CTA's
+    // tcgen05.alloc, it could hold the tensor memory that this one waits for.
+    pdl_launch_dependents();
   }
   if (kGrouped && warp == 2) {  // the block's live slots, in order
     int n = 0;
@@ -902,9 +926,6 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // Only now may the next kernel start: were it let in before this CTA's
-  // tcgen05.alloc, it could hold the tensor memory that this one waits for.
-  pdl_launch_dependents();
   const uint32_t tmem = __shfl_sync(0xffffffffu, bars->tmem_base, 0);  // uniform
   const int rows = kGrouped ? bars->live : min(p.rows, p.M - row0);
 
@@ -990,6 +1011,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
     // neighbouring lanes down the rows, the SMs' reads of the same few lines queued for 3 us)
     pdl_wait();
     const int words = nkt * rows;
+    const uint32_t tail = scale_mask(p.K, num_kt - 1);
     for (int i0 = threadIdx.x - 64; i0 < words; i0 += 2 * F_FILL) {
       uint32_t v[2];
       int at[2];
@@ -998,6 +1020,7 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
         const int i = i0 + u * F_FILL, r = i / nkt, kt = i - r * nkt;
         at[u] = kt * 512 + (r & 31) * 16 + (r >> 5) * 4;
         if (i < words) v[u] = __ldcg(reinterpret_cast<const uint32_t*>(p.sfa + (row0 + r) * p.lds + (kt0 + kt) * 4));
+        if (kt0 + kt + 1 == num_kt) v[u] &= tail;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -1238,7 +1261,6 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
           if ((c & 3) == 0) scales[pos * ldso + (c >> 2)] = static_cast<uint8_t>(e);
         }
       }
-      for (int g = gpr + lane; g < ldso; g += 32) scales[pos * ldso + g] = 0;
     } else {
       for (int c = lane; c < 2 * gpr; c += 32)
         reinterpret_cast<uint4*>(dst)[c] = __ldcg(reinterpret_cast<const uint4*>(src) + c);

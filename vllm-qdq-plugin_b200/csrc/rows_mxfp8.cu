@@ -11,10 +11,9 @@
 // that the codes are those of mxfp8_qdq behind it.  All sums and products
 // before it are fp32.
 //
-// Layout: codes [M, K] row-major bytes; scales [M, lds] row-major E8M0 bytes,
-// K / 32 of them followed by zeros up to a multiple of 16, so that the product
-// loads 16 scales (512 elements of K) of a row at once and its last stage
-// finds 2^-127 rather than a stale NaN behind K.
+// Layout: codes [M, K] row-major bytes; scales row-major E8M0 bytes, K / 32 a
+// row, rows lds (a multiple of 16) apart, so that the product loads 16 scales
+// (512 elements of K) of a row at once; what lies between is not written.
 //
 // All three are one HBM pass: a lane owns units of 16 elements (two 16-byte
 // loads), the two lanes of a group exchange their maxima by a shuffle.
@@ -71,12 +70,11 @@ __device__ __forceinline__ Unit unit_of(const uint32_t (&w)[8]) {
   return {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
 
-// MXFP8 of unit `col` (of upr in the row): codes, and from the group's first
-// lane the scale; behind the last group also the zeros up to a multiple of 16
-// scales.  Every lane of the warp takes part in the shuffle.
+// MXFP8 of unit `col` of a row: codes, and from the group's first lane the
+// scale.  Every lane of the warp takes part in the shuffle.
 template <int kDtype>
 __device__ __forceinline__ void store_mxfp8(const uint32_t (&y)[8], uint8_t* codes_row, uint8_t* scales_row,
-                                            uint32_t col, uint32_t upr, bool live, float zero) {
+                                            uint32_t col, bool live, float zero) {
   uint32_t amax = absmax_words<kDtype>(y);
   amax = max(amax, __shfl_xor_sync(kAll, amax, 1));
   const int e = mx8_exp<kDtype>(amax);
@@ -84,11 +82,7 @@ __device__ __forceinline__ void store_mxfp8(const uint32_t (&y)[8], uint8_t* cod
   uint32_t c[4];
   mx8_codes<kDtype>(y, e, zero, c);
   *reinterpret_cast<uint4*>(codes_row + col * 16u) = make_uint4(c[0], c[1], c[2], c[3]);
-  if ((col & 1u) == 0) {
-    scales_row[col >> 1] = static_cast<uint8_t>(e);
-    if (col + 2 == upr)
-      for (uint32_t p = upr >> 1; p < (((upr >> 1) + 15u) & ~15u); ++p) scales_row[p] = 0;
-  }
+  if ((col & 1u) == 0) scales_row[col >> 1] = static_cast<uint8_t>(e);
 }
 
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -155,7 +149,7 @@ rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, u
         y[j] = F::pack(s.x, s.y);
       }
     }
-    store_mxfp8<kDtype>(y, cr, sr, col, upr, in_m && col < upr, zero);
+    store_mxfp8<kDtype>(y, cr, sr, col, in_m && col < upr, zero);
     v = vn;
     u = un;
   }
@@ -253,7 +247,7 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
         a8[j] = F::pack(n.x, n.y);
       }
       if (y_out != nullptr && col < upr) store_unit<kWide>(y_out + row * ldy + col * 16u, unit_of(a8));
-      store_mxfp8<kDtype>(a8, codes + row * ldc, scales + row * lds, col, upr, col < upr, zero);
+      store_mxfp8<kDtype>(a8, codes + row * ldc, scales + row * lds, col, col < upr, zero);
     }
     if (!kWarpRow) __syncthreads();
   }

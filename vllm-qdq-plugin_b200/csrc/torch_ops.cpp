@@ -56,13 +56,31 @@ void check_k(const char* name, int64_t k) {
 void check_device(const Tensor& x, const Tensor& t) {
   TORCH_CHECK(t.device() == x.device(), "expected every tensor on ", x.device(), ", got one on ", t.device());
 }
+// MXFP8 rows: scales [M, K / 32] whose rows lie in storage padded to the stride the products read.
 void check_rows(const char* name, const Tensor& codes, const Tensor& scales) {
   TORCH_CHECK(codes.dim() == 2 && codes.scalar_type() == at::kByte && scales.dim() == 2 &&
                   scales.scalar_type() == at::kByte && scales.size(0) == codes.size(0) &&
-                  scales.size(1) == qdq_mxfp8_scale_stride(codes.size(1)),
+                  scales.size(1) * 32 == codes.size(1),
               name, ": malformed MXFP8 rows");
-  TORCH_CHECK(codes.stride(1) == 1 && scales.stride(1) == 1, name, ": MXFP8 rows must be dense along K");
+  const int64_t m = codes.size(0), need = qdq_mxfp8_scale_stride(codes.size(1));
+  TORCH_CHECK(codes.stride(1) == 1 && (scales.size(1) == 1 || scales.stride(1) == 1), name,
+              ": MXFP8 rows must be dense along K");
+  const int64_t step = m > 1 ? scales.stride(0) : need;
+  TORCH_CHECK(m == 0 || (step >= need && static_cast<int64_t>(scales.storage().nbytes()) >=
+                                             scales.storage_offset() + (m - 1) * step + need),
+              name, ": the scales' rows are not padded (make the rows with Mxfp8Rows.from_codes)");
   check_device(codes, scales);
+}
+int64_t scale_ld(const Tensor& scales, int64_t k) {
+  return scales.size(0) > 1 ? scales.stride(0) : qdq_mxfp8_scale_stride(k);
+}
+// [m, k / 32] scales in storage of whole padded rows.
+Tensor new_scales(int64_t m, int64_t k, const Tensor& like) {
+  const int64_t lds = qdq_mxfp8_scale_stride(k);
+  Tensor t = bytes(m, lds, like);
+  const int64_t sizes[2] = {m, k / 32}, strides[2] = {lds, 1};
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef(sizes, 2), at::IntArrayRef(strides, 2));
+  return t;
 }
 Tensor dense_as(const std::optional<Tensor>& t, at::ScalarType dtype) {
   return t.has_value() ? t->to(dtype).contiguous() : Tensor();
@@ -75,7 +93,7 @@ std::tuple<Tensor, Tensor> rows_op(const char* name, F fn, const Tensor& x_, int
   const c10::cuda::CUDAGuard guard(x_.device());
   const Tensor x = rows16(x_);
   const int64_t m = x.size(0), lds = qdq_mxfp8_scale_stride(k);
-  Tensor codes = bytes(m, k, x), scales = bytes(m, lds, x);
+  Tensor codes = bytes(m, k, x), scales = new_scales(m, k, x);
   check(name, fn(ptr(x), ptr(codes), ptr(scales), m, k, ld(x), k, lds, dtype_code(x), stream()));
   return {codes, scales};
 }
@@ -113,7 +131,7 @@ std::vector<Tensor> rmsnorm_mxfp8(const Tensor& x_, const Tensor& weight, const 
     r = rows16(*residual);
   }
   out.push_back(bytes(m, k, x));
-  out.push_back(bytes(m, lds, x));
+  out.push_back(new_scales(m, k, x));
   if (r.defined()) {
     out.push_back(empty({m, k}, x.scalar_type(), x));
     h = ptr(out.back());
@@ -160,7 +178,7 @@ Tensor mxfp8_linear_rows(const Tensor& codes, const Tensor& scales, const Tensor
   const int64_t m = codes.size(0), k = codes.size(1), n = w.size(0);
   Tensor out = empty({m, n}, dtype, codes);
   check("fp8_gemm_mxf8",
-        fp8_gemm_mxf8(ptr(codes), ptr(scales), ld(codes), ld(scales), ptr(w), ptr(sf), ptr_or_null(b), ptr(out), m, n, k,
+        fp8_gemm_mxf8(ptr(codes), ptr(scales), ld(codes), scale_ld(scales, k), ptr(w), ptr(sf), ptr_or_null(b), ptr(out), m, n, k,
                       ld(w), n, out_fp16 ? QDQ_DTYPE_FP16 : QDQ_DTYPE_BF16, stream()));
   return out;
 }
@@ -197,7 +215,7 @@ void mxfp8_moe_linear_out(const Tensor& a_, const std::optional<Tensor>& a_scale
   Tensor ws = bytes(need, a);
   check("fp8_moe_mxf8",
         fp8_moe_mxf8(raw ? ptr(a) : nullptr, raw ? ld(a) : 0, raw ? nullptr : ptr(a), ptr(a_scales), raw ? 0 : ld(a),
-                     raw ? 0 : ld(*a_scales), dtype_code(out), ptr(w), ptr(sf), w.size(0),
+                     raw ? 0 : scale_ld(*a_scales, k), dtype_code(out), ptr(w), ptr(sf), w.size(0),
                      static_cast<const int32_t*>(ptr(sorted_ids)), static_cast<const int32_t*>(ptr(expert_ids)),
                      static_cast<const int32_t*>(ptr(num_post_padded)), static_cast<const float*>(ptr_or_null(tw)),
                      sorted, static_cast<int>(block), static_cast<int>(top_k), tw.defined() ? 1 : 0, ptr(out),

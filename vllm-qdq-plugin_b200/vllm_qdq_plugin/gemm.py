@@ -28,7 +28,7 @@ import torch
 from . import _native
 from ._log import init_logger
 from .qdq.mxfp4 import mxfp4_quantize
-from .qdq.mxfp8_rows import Mxfp8Rows, scale_stride
+from .qdq.mxfp8_rows import Mxfp8Rows
 
 logger = init_logger(__name__)
 
@@ -541,9 +541,9 @@ def _(a, a_scales, w_codes, w_sf_tiled, sorted_token_ids, expert_ids, num_tokens
 # tensor to dispatch on, these give the errors of the other operators.
 def _check_mxfp8_rows(name: str, a: torch.Tensor | Mxfp8Rows, k: int) -> None:
     if isinstance(a, Mxfp8Rows):
-        _native.require_cuda(a.codes, a.stored)
-        assert a.codes.dim() == 2 and a.codes.dtype == torch.uint8 and a.stored.dtype == torch.uint8 and (
-            tuple(a.stored.shape) == (a.codes.shape[0], scale_stride(a.codes.shape[1]))), f"{name}: malformed MXFP8 rows"
+        _native.require_cuda(a.codes, a.scales)
+        assert a.codes.dim() == 2 and a.codes.dtype == torch.uint8 and a.scales.dtype == torch.uint8 and (
+            tuple(a.scales.shape) == (a.codes.shape[0], a.codes.shape[1] // 32)), f"{name}: malformed MXFP8 rows"
     else:
         assert a.dim() == 2 and a.dtype in (torch.bfloat16, torch.float16), (
             f"{name}: the activation must be 2-D bf16/fp16 or MXFP8 rows")
@@ -563,7 +563,7 @@ def mxfp8_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8Weight, bias: torch.T
     try:
         if isinstance(a, Mxfp8Rows):
             _native.load_ops(a.codes)
-            return _mxfp8_linear_rows_op(a.codes, a.stored, weight.codes, weight.sf_tiled, bias, a.dtype == torch.float16)
+            return _mxfp8_linear_rows_op(a.codes, a.scales, weight.codes, weight.sf_tiled, bias, a.dtype == torch.float16)
         _native.load_ops(a)
         return _mxfp8_linear_op(a, weight.codes, weight.sf_tiled, bias)
     except RuntimeError:
@@ -583,7 +583,7 @@ def mxfp8_moe_linear(a: torch.Tensor | Mxfp8Rows, weight: Mxfp8MoeWeight, sorted
     a: [M, K] bf16/fp16, or MXFP8 rows; out: [M * top_k, N] of a's dtype (allocated when None; rows of
     slots that are not routed keep their contents).  moe_block_size in [1, 64]."""
     rows = isinstance(a, Mxfp8Rows)
-    codes, scales = (a.codes, a.stored) if rows else (a, None)
+    codes, scales = (a.codes, a.scales) if rows else (a, None)
     assert not mul_topk_weights or topk_weights is not None, "mul_topk_weights needs topk_weights"
     tw = topk_weights if mul_topk_weights else None
     assert out is None or out.dtype == a.dtype, (out.dtype, a.dtype)

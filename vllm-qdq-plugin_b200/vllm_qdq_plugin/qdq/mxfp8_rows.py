@@ -32,13 +32,14 @@ def scale_stride(k: int) -> int:
 class Mxfp8Rows:
     """Rows of MXFP8: element (m, k) stands for E4M3(codes[m, k]) * 2^(scales[m, k // 32] - 127).
 
-    `stored` holds the scales as the products read them: rows padded with
-    zeros to `scale_stride(K)` bytes.  `dtype` is the 16-bit type of the tensor
-    the rows were made from, and of a product's output.
+    The rows of `scales` lie `scale_stride(K)` bytes apart, or further, in a
+    storage that holds the last one's padding too (the products read 16 scales
+    at a time; `from_codes` lays scales out so).  `dtype` is the 16-bit type of
+    the tensor the rows were made from, and of a product's output.
     """
 
     codes: torch.Tensor    # uint8 [M, K] E4M3
-    stored: torch.Tensor   # uint8 [M, scale_stride(K)] E8M0
+    scales: torch.Tensor   # uint8 [M, K / 32] E8M0, padded row stride
     dtype: torch.dtype
 
     @property
@@ -48,12 +49,6 @@ class Mxfp8Rows:
     @property
     def device(self) -> torch.device:
         return self.codes.device
-
-    @property
-    def scales(self) -> torch.Tensor:
-        """E8M0 scales [M, K / 32] (a view)."""
-        n = self.codes.shape[1] // 32
-        return self.stored if self.stored.shape[1] == n else self.stored.narrow(1, 0, n)
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> "Mxfp8Rows":
@@ -65,9 +60,8 @@ class Mxfp8Rows:
         assert codes.dim() == 2 and codes.shape[1] > 0 and codes.shape[1] % 32 == 0, tuple(codes.shape)
         m, k = codes.shape
         assert tuple(scales.shape) == (m, k // 32), (tuple(codes.shape), tuple(scales.shape))
-        stored = torch.zeros((m, scale_stride(k)), dtype=torch.uint8, device=codes.device)
-        stored[:, : k // 32] = scales
-        return cls(_native.rows16(codes), stored, dtype)
+        stored = torch.empty((m, scale_stride(k)), dtype=torch.uint8, device=codes.device)[:, : k // 32]
+        return cls(_native.rows16(codes), stored.copy_(scales), dtype)
 
     def dequantize(self) -> torch.Tensor:
         """The values in `dtype`: what `mxfp8_qdq` returns for the same tensor."""
@@ -88,7 +82,8 @@ _rmsnorm_op = torch.ops.qdq_b200.rmsnorm_mxfp8.default
 
 
 def _new_rows(x: torch.Tensor, m: int, k: int) -> tuple[torch.Tensor, torch.Tensor]:
-    return x.new_empty((m, k), dtype=torch.uint8), x.new_empty((m, scale_stride(k)), dtype=torch.uint8)
+    return (x.new_empty((m, k), dtype=torch.uint8),
+            x.new_empty_strided((m, k // 32), (scale_stride(k), 1), dtype=torch.uint8))
 
 
 @torch.library.register_fake("qdq_b200::mxfp8_rows")
