@@ -10,7 +10,7 @@
 // idle M, and a ragged segment of an expert's rows costs its own width.
 //
 // One CTA per SM walks work items (a segment of at most NT activation rows,
-// 128 rows of W); 12 warps:
+// 128 rows of W); 14 warps:
 //   warp 0      TMA producer: W codes and scales of a K-128 stage, and the
 //               codes of the segment's rows, which are consecutive (grouped:
 //               a pass before copies the routed rows into sorted order)
@@ -50,7 +50,7 @@ constexpr int T_EPI = 8;             // epilogue warps
 constexpr int T_SCALE = 4;           // scale warps = quads of stages in the scale ring
 constexpr int T_THREADS = 32 * (2 + T_SCALE + T_EPI);
 constexpr uint32_t T_TMEM = 512, T_SFW = 2 * NT_MAX, T_SFA = T_SFW + 4;
-constexpr uint32_t T_SF_COLS = 12;   // four sets of scale columns in turn: a stage's copies overlap the MMAs before it
+constexpr uint32_t T_SF_COLS = 12;   // four sets of scale columns in turn: a stage's copies need not wait for the MMAs before it
 
 __host__ __device__ constexpr int t_stage_bytes(int nt) { return T_W + nt * TK; }       // codes
 __host__ __device__ constexpr int t_sf_bytes(int nt) { return nt > 128 ? 1024 : 512; }  // a stage's activation scales
@@ -162,8 +162,7 @@ struct Item {
 // one W panel run side by side, so the CTAs in flight share it in L2.
 // Grouped: segment-major, so that each expert's W streams from HBM once while
 // its rows stay in L2; the next item's segment entry is fetched while the
-// present item runs (read when it was needed, it held the ring up for 1 us an
-// item).
+// present item runs.
 template <bool kGrouped>
 struct Walk {
   const GemmArgs& p;
@@ -1165,9 +1164,9 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
   int carry_start = -1, carry_count = 0;
   for (int base = 0; base < live; base += blockDim.x) {
     const int b = base + t;
-    const int e = b < live ? __ldg(expert_ids + b) : -1;
+    const int e = b < live ? __ldcg(expert_ids + b) : -1;
     const bool valid = e >= 0 && e < num_experts;
-    const bool first = valid && (b == 0 || __ldg(expert_ids + b - 1) != e);
+    const bool first = valid && (b == 0 || __ldcg(expert_ids + b - 1) != e);
     int start = first ? b : -1;  // the first block of b's run: a running maximum
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1191,7 +1190,7 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
     }
     if (seg) {
       int nb = 1;
-      while (nb < nbmax && b + nb < live && __ldg(expert_ids + b + nb) == e) ++nb;
+      while (nb < nbmax && b + nb < live && __ldcg(expert_ids + b + nb) == e) ++nb;
       reinterpret_cast<int4*>(seg_tab + 4)[at] = make_int4(b * bs, nb * bs, e, 0);
     }
     carry_start = last;
@@ -1373,10 +1372,9 @@ int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewAr
 // of a K-128 stage are the largest of its MMAs' (2 per activation row), its
 // operand bytes at 80 a cycle and its issue (300, pairs 430), plus 80; the
 // launch takes as many stages as the busiest SM has items.  Against the best
-// of five forced choices the rule's was within 5 % on 12 of 14 shapes, e.g.
-// [4096 x 4096 -> 14336] pairs of 240 rows 171 us, of 128 about 210, single
-// CTAs of 192 rows 209; [4096 x 1024 -> 512] single CTAs of 128 rows 8.2 us,
-// pairs 10.2.
+// of five forced choices the rule's was within 6 % on 14 shapes, e.g.
+// [4096 x 4096 -> 14336] pairs of 240 rows 171 us, single CTAs of 192 rows
+// 209; [4096 x 1024 -> 512] single CTAs of 128 rows 8.2 us, pairs 10.2.
 struct TilePlan {
   bool pair;
   int nt;
@@ -1389,7 +1387,8 @@ TilePlan tile_plan(int64_t M, int64_t blocks) {
     for (int nt = 16; nt <= (pair ? P_NT_MAX : NT_MAX); nt += 16) {
       const int64_t items = (M + nt - 1) / nt * (pair ? (blocks + 1) / 2 : blocks), units = pair ? sms / 2 : sms;
       const double bytes = T_W + nt * TK * (pair ? 0.5 : 1.0);
-      const double cost = static_cast<double>((items + units - 1) / units) * (std::max(std::max(2.0 * nt, bytes / 80.0), pair ? 430.0 : 300.0) + 80.0);
+      const double stage = std::max(std::max(2.0 * nt, bytes / 80.0), pair ? 430.0 : 300.0) + 80.0;
+      const double cost = static_cast<double>((items + units - 1) / units) * stage;
       if (best.nt == 0 || cost < least) {
         best = {pair != 0, nt};
         least = cost;
@@ -1511,7 +1510,7 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   if (plan.pair)
     if (int st = make_tmap_u32_2d(&tsf, w_sf_tiled, blocks * p.kchunks, 128, 512, 128, 4)) return st;
   const int64_t items = ((M + p.nt - 1) / p.nt) * (plan.pair ? (blocks + 1) / 2 : blocks);
-  if (items >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if (items >= (1ll << 30)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
   return out_dtype == QDQ_DTYPE_FP16 ? launch_gemm<QDQ_DTYPE_FP16, false>(who, tw, ta, tsf, p, plan.pair, items, s)
                                      : launch_gemm<QDQ_DTYPE_BF16, false>(who, tw, ta, tsf, p, plan.pair, items, s);
 }
@@ -1582,7 +1581,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   const int64_t num_blocks = num_sorted / moe_block_size;
   if (num_blocks == 0) return QDQ_OK;
   const int64_t n_tiles = (N + TM - 1) / TM;
-  if (num_blocks * n_tiles >= (1ll << 31)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
+  if (num_blocks * n_tiles >= (1ll << 30)) return fail(QDQ_ERR_UNSUPPORTED, "%s: too many tiles", who);
   int* status = device_status_ptr();
   if (status == nullptr) return QDQ_ERR_CUDA;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
