@@ -25,7 +25,7 @@ def _rows_values(rows):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 1, 32), (1, 4096, 4096), (2, 300, 96), (16, 512, 1024),
-                                   (17, 129, 544), (33, 640, 512), (64, 1024, 2080), (65, 200, 288), (100, 1001, 2880),
+                                   (17, 129, 544), (33, 640, 512), (64, 1024, 2080), (5, 300, 4128), (65, 200, 288), (100, 1001, 2880),
                                    (128, 256, 256), (129, 257, 352), (192, 384, 512), (193, 384, 512),
                                    (333, 768, 2048), (1000, 136, 160), (257, 2050, 4128),
                                    (1500, 2560, 544), (2100, 1281, 288), (700, 5002, 320), (4111, 640, 128)])

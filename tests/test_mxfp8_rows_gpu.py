@@ -90,6 +90,7 @@ def test_rows_from_codes_and_strided_inputs(cuda_device):
     assert torch.equal(rows.codes, want.codes) and torch.equal(rows.scales, want.scales)
     w = torch.randn(288, device=cuda_device).to(torch.bfloat16)
     for view in (torch.cat([x, x], 1)[:, :288],                       # padded rows, 16-byte aligned
+                 torch.nn.functional.pad(x, (8, 8))[:, 8:296],        # 16-byte aligned, off the 32-byte grid
                  torch.nn.functional.pad(x, (1, 2))[:, 1:289],        # rows off the 16-byte grid
                  x.t().contiguous().t(),                              # strided along K
                  torch.cat([x.new_zeros(1), x.reshape(-1)])[1:].view(37, 288)):  # base off the grid
