@@ -438,3 +438,52 @@ def test_padding_of_scale_rows_has_no_effect(cuda_device, m, k):
         seen.append((mxfp8_linear(r, w), mxfp8_moe_linear(r, wm, sid, eid, ntp, tw, 32, 2, True)))
     assert all(torch.equal(x, y) for s in seen[1:] for x, y in zip(s, seen[0])) and seen[0][0].isfinite().all()
     _ok()
+
+
+@pytest.mark.parametrize("m,n,shift,gap", [(600, 328, 0, 8), (600, 328, 8, 16), (600, 328, 2, 8), (600, 328, 0, 2),
+                                           (600, 328, 1, 8), (600, 328, 0, 3), (600, 326, 0, 2), (600, 325, 0, 3),
+                                           (4100, 2568, 0, 8), (4100, 2568, 2, 8), (4100, 2562, 0, 6), (4100, 2563, 1, 1)])
+def test_output_rows_at_any_address(cuda_device, m, n, shift, gap):
+    """Products into rows that start `shift` elements into memory and `n + gap` apart: what lies between stays."""
+    from vllm_qdq_plugin import _native
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    k, dev = 160, cuda_device
+    rows = mxfp8_rows(activation(m, k, torch.bfloat16, n, dev))
+    codes, scales = random_weight(n, k, seed=m, dev=dev)
+    w = prepare_mxfp8_weight(codes, scales)
+    bias = torch.randn(n, device=dev).to(torch.bfloat16)
+    want = mxfp8_linear(rows, w, bias)
+    check_product(want, _rows_values(rows), values(codes, scales), bias, f"{m}x{n}")
+    held = torch.full((shift + m * (n + gap) + 8,), -3.0, dtype=torch.bfloat16, device=dev)
+    out = held[shift : shift + m * (n + gap)].view(m, n + gap)
+    lib = _native.lib()
+    sf = torch.empty(lib.qdq_sf_tiled_bytes(n, k), dtype=torch.uint8, device=dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.qdq_sf_tile(scales.data_ptr(), sf.data_ptr(), n, k, k // 32, 32, stream) == 0
+    torch.cuda.synchronize()
+    assert lib.fp8_gemm_mxf8(rows.codes.data_ptr(), rows.scales.data_ptr(), rows.codes.stride(0), rows.scales.stride(0),
+                             codes.data_ptr(), sf.data_ptr(), bias.data_ptr(), out.data_ptr(), m, n, k, k, n + gap, 0,
+                             stream) == 0
+    assert torch.equal(out[:, :n], want) and (out[:, n:] == -3).all()
+    assert (held[:shift] == -3).all() and (held[shift + m * (n + gap) :] == -3).all()
+    _ok()
+
+
+@pytest.mark.parametrize("m,e,top_k,bs,n,k", [(400, 128, 4, 16, 2568, 96),   # pairs of few rows, many items an SM
+                                              (512, 8, 2, 64, 2600, 64),     # the experts' rows in one item
+                                              (911, 4, 2, 16, 390, 224),     # several items an expert
+                                              (300, 4, 2, 64, 1000, 96),
+                                              (1422, 64, 4, 8, 127, 192),
+                                              (120, 16, 2, 64, 1312, 64)])
+def test_moe_tile_choices(cuda_device, m, e, top_k, bs, n, k):
+    from vllm_qdq_plugin.gemm import mxfp8_moe_linear, prepare_mxfp8_moe_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    rows = mxfp8_rows(activation(m, k, torch.bfloat16, m, cuda_device))
+    codes, scales = random_weight(e, n, k, seed=n, dev=cuda_device)
+    w = prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, top_k, bs, m, cuda_device)
+    for mul in (False, True):
+        out = mxfp8_moe_linear(rows, w, sid, eid, ntp, tw, bs, top_k, mul)
+        check_moe(out, _rows_values(rows), codes, scales, ids, f"m={m} e={e} n={n}", tw if mul else None)
+    _ok()

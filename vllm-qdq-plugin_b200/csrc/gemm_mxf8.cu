@@ -116,7 +116,7 @@ struct GemmArgs {
   int top_k, bs, num_blocks, num_experts;
   int a_rows;                  // rows of the activation codes (grouped: sorted positions)
   int nt, box;                 // activation rows per item, and per TMA box
-  int pairs;                   // C takes 4-byte stores of two columns
+  int wide;                    // neighbouring n that C takes in one store: 8, 2 or 1
   int* status;
 };
 
@@ -212,38 +212,66 @@ __device__ __forceinline__ void column_rows(const GemmArgs& p, const Item& w, in
 }
 
 // Stores 32 accumulator columns (activation rows) of this lane's W row n.
-// Neighbouring lanes hold neighbouring n: they exchange halves, so that a lane
-// stores two n of one row at once, the even lanes of the even rows, the odd
-// lanes of the odd ones.  All exchanges come before the stores (in turn with
-// them, each store waited for its row's shuffle: 18 k cycles an item of 240
-// rows where the MMAs take 15 k).
+// Eight neighbouring lanes hold eight neighbouring n: they transpose eight rows
+// among themselves in three exchanges (two n a word, two words, four), so that
+// a lane stores 16 bytes of each of four rows.  All exchanges come before the
+// stores.  (Stored two bytes at a time, each behind its row's shuffle, an item
+// of 240 rows took 18 k cycles where its MMAs take 15 k at K = 4096; four bytes
+// at a time 11 k.)  A C whose rows start on 4-byte boundaries only takes the
+// words of the first exchange.
 template <int kDtype, bool kGrouped>
 __device__ __forceinline__ void store_columns(const GemmArgs& p, const uint32_t (&r)[32], int n, int lane, int slot,
                                               float wt, float bias) {
   using O = Out16<kDtype>;
   using T = typename O::T;
   T* C = static_cast<T*>(p.c);
-  if (p.pairs) {
-    const int odd = lane & 1;
-    uint32_t v[16];
-    int row[16];
+  if (p.wide > 1) {
+    const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+    const bool scaled = kGrouped && p.topk_w != nullptr;
+    uint32_t v[16];  // word i: row 2 i + b0, n pair
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float a = __uint_as_float(r[2 * i]) + bias, b = __uint_as_float(r[2 * i + 1]) + bias;
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? a : b, 1);
-      float lo = odd ? other : a, hi = odd ? b : other;
-      if (kGrouped) {
-        const float f = __shfl_sync(0xffffffffu, wt, 2 * i + odd);
+      const float x = __uint_as_float(r[2 * i]) + bias, y = __uint_as_float(r[2 * i + 1]) + bias;
+      const float other = __shfl_xor_sync(0xffffffffu, b0 ? x : y, 1);
+      float lo = b0 ? other : x, hi = b0 ? y : other;
+      if (scaled) {
+        const float f = __shfl_sync(0xffffffffu, wt, 2 * i + (lane & 1));
         lo *= f;
         hi *= f;
       }
-      row[i] = __shfl_sync(0xffffffffu, slot, 2 * i + odd);
       v[i] = O::two(lo, hi);
     }
-    if (n < p.N) {  // N is even: both n of a pair are inside, or neither
+    if (p.wide == 2) {  // N is even: both n of a pair are inside, or neither
+      int at[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (row[i] >= 0) *reinterpret_cast<uint32_t*>(C + static_cast<int64_t>(row[i]) * p.ldc + (n & ~1)) = v[i];
+      for (int i = 0; i < 16; ++i) at[i] = __shfl_sync(0xffffffffu, slot, 2 * i + (lane & 1));
+      if (n < p.N) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (at[i] >= 0) *reinterpret_cast<uint32_t*>(C + static_cast<int64_t>(at[i]) * p.ldc + (n & ~1)) = v[i];
+      }
+      return;
+    }
+    uint32_t q[8][2];  // words of row 4 j + 2 b1 + b0, n quad
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, b1 ? v[2 * j] : v[2 * j + 1], 2);
+      q[j][0] = b1 ? other : v[2 * j];
+      q[j][1] = b1 ? v[2 * j + 1] : other;
+    }
+    uint4 o[4];
+    int row[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // row 8 j + lane % 8, n octet
+      const uint32_t o0 = __shfl_xor_sync(0xffffffffu, b2 ? q[2 * j][0] : q[2 * j + 1][0], 4);
+      const uint32_t o1 = __shfl_xor_sync(0xffffffffu, b2 ? q[2 * j][1] : q[2 * j + 1][1], 4);
+      o[j] = b2 ? make_uint4(o0, o1, q[2 * j + 1][0], q[2 * j + 1][1]) : make_uint4(q[2 * j][0], q[2 * j][1], o0, o1);
+      row[j] = __shfl_sync(0xffffffffu, slot, 8 * j + (lane & 7));
+    }
+    if (n < p.N) {  // N is a multiple of 8: an octet is inside or outside as a whole
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row[j] >= 0) *reinterpret_cast<uint4*>(C + static_cast<int64_t>(row[j]) * p.ldc + (n & ~7)) = o[j];
     }
   } else {
 #pragma unroll
@@ -1380,27 +1408,52 @@ int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewAr
 // of five forced choices the rule's was within 6 % on 14 shapes, e.g.
 // [4096 x 4096 -> 14336] pairs of 240 rows 171 us, single CTAs of 192 rows
 // 209; [4096 x 1024 -> 512] single CTAs of 128 rows 8.2 us, pairs 10.2.
+//
+// Grouped: `segments(nt)` estimates the segments at nt rows per item from what
+// the host knows, `rows` the rows of an average one.  Where every expert has one
+// segment (`experts` of them) its weights come from memory, which gives an SM no
+// stage in less than 700 cycles.  Both kernels then take the same time but for
+// starts, tails and idle halves of pairs, and pairs that cost up to 6 % more
+// stages are taken where their own stage is shorter (192 rows an item: 512
+// tokens, 8 experts of 14336 x 4096, 99.8 us, single CTAs 103.5; 4096 tokens, 128
+// experts of 2880 x 2880, 235 and 249) or an SM has 16 items or more (64 tokens,
+// 128 experts of 5760 x 2880: 284 and 293; with 7 items, 16 tokens, 8 experts of
+// 14336 x 4096: 87.8 and 84.3).
 struct TilePlan {
   bool pair;
   int nt;
 };
-TilePlan tile_plan(int64_t M, int64_t blocks) {
+template <typename Segments>
+TilePlan tile_plan(int64_t rows, int64_t blocks, int64_t experts, Segments segments) {
   TilePlan best = {false, 0};
-  double least = 0;
+  double least = 0, stage = 0;
   const int64_t sms = device_sm_count();
   for (int pair = 0; pair < 2; ++pair) {
     for (int nt = 16; nt <= (pair ? P_NT_MAX : NT_MAX); nt += 16) {
-      const int64_t items = (M + nt - 1) / nt * (pair ? (blocks + 1) / 2 : blocks), units = pair ? sms / 2 : sms;
-      const double bytes = T_W + nt * TK * (pair ? 0.5 : 1.0);
-      const double stage = std::max(std::max(2.0 * nt, bytes / 80.0), pair ? 430.0 : 300.0) + 80.0;
-      const double cost = static_cast<double>((items + units - 1) / units) * stage;
-      if (best.nt == 0 || cost < least) {
+      const int64_t segs = segments(nt);
+      if (segs <= 0) continue;
+      const int64_t items = segs * (pair ? (blocks + 1) / 2 : blocks), units = pair ? sms / 2 : sms;
+      const int64_t waves = (items + units - 1) / units;
+      const double used = static_cast<double>(std::min<int64_t>(nt, rows));
+      const double bytes = T_W + used * TK * (pair ? 0.5 : 1.0);
+      const double own = std::max(std::max(2.0 * used, bytes / 80.0), pair ? 430.0 : 300.0) + 80.0;
+      const bool streams = segs == experts;
+      const double cost = static_cast<double>(waves) * std::max(own, streams ? 700.0 : 0.0);
+      const bool liked = pair && !best.pair && streams && (own < stage || waves >= 16);
+      if (best.nt == 0 || cost < (liked ? 1.06 : 1.0) * least) {
         best = {pair != 0, nt};
         least = cost;
+        stage = own;
       }
     }
   }
   return best;
+}
+
+// The neighbouring n that C, rows of `ldc` elements of 16 bits, takes in one store.
+int store_width(const void* c, int64_t ldc, int64_t N) {
+  if (N % 8 == 0 && ldc % 8 == 0 && !off(c, 16)) return 8;
+  return N % 2 == 0 && ldc % 2 == 0 && !off(c, 4) ? 2 : 1;
 }
 
 int check_product(const char* who, int dtype, int64_t M, int64_t N, int64_t K) {
@@ -1503,9 +1556,9 @@ extern "C" int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t 
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
   p.top_k = 1;
   p.a_rows = p.M;
-  p.pairs = N % 2 == 0 && ldc % 2 == 0 && !off(c, 4);
+  p.wide = store_width(c, ldc, N);
   const int64_t blocks = (N + TM - 1) / TM;
-  const TilePlan plan = tile_plan(M, blocks);
+  const TilePlan plan = tile_plan(M, blocks, 0, [&](int nt) { return (M + nt - 1) / nt; });
   p.nt = plan.nt;
   p.box = plan.pair ? plan.nt / 2 : plan.nt;  // one tile's rows in one box
   p.status = status;
@@ -1628,17 +1681,19 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   uint8_t* scales = codes + up256(num_sorted * K);
   const int64_t ldso = qdq_mxfp8_scale_stride(K);
   GemmArgs p = {};
-  // Pairs, unless an odd last W block would leave more than 6 % of their work idle (they gain 4 to 8 %).  Rows per
-  // item: the average expert's, rounded up to whole blocks (few rows leave the shared memory to more stages of W in
-  // flight), in boxes that leave a ragged segment few idle rows.
-  const bool pair = 100 * ((n_tiles + 1) / 2 * 2) <= 106 * n_tiles;
-  const int most = pair ? P_NT_MAX : NT_MAX;
-  const int64_t average = (num_sorted + num_experts - 1) / num_experts;
-  const int64_t wanted = (average + moe_block_size - 1) / moe_block_size * moe_block_size;
-  p.nt = static_cast<int>((std::min<int64_t>(wanted, most) + 15) / 16 * 16);
+  // An average expert's rows in whole blocks, over as many experts as can be hit.  Few rows per item leave the shared
+  // memory to more stages of W in flight; boxes leave a ragged segment few idle rows.
+  const int64_t experts = std::min(num_experts, num_blocks);
+  const int64_t average = ((num_sorted + experts - 1) / experts + moe_block_size - 1) / moe_block_size * moe_block_size;
+  const TilePlan plan = tile_plan(average, n_tiles, experts, [&](int nt) {
+    const int64_t rows = nt / moe_block_size * moe_block_size;
+    return rows == 0 ? int64_t(0) : experts * ((average + rows - 1) / rows);
+  });
+  const bool pair = plan.pair;
+  p.nt = plan.nt;
   const int held = pair ? p.nt / 2 : p.nt;  // rows in one CTA's shared memory
   p.box = held > 96 ? 64 : held > 16 ? 32 : held > 8 ? 16 : 8;
-  if (!pair) p.nt = (p.nt + p.box - 1) / p.box * p.box;
+  if (!pair) p.nt = std::min(NT_MAX, (p.nt + p.box - 1) / p.box * p.box);
   const int nbmax = p.nt / moe_block_size;
   {
     const int warps = SEG_THREADS / 32;
@@ -1660,7 +1715,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.c = c;
   p.ldc = ldc;
   p.seg_tab = seg_tab;
-  p.pairs = N % 2 == 0 && ldc % 2 == 0 && !off(c, 4);
+  p.wide = store_width(c, ldc, N);
   p.sorted_ids = sorted_token_ids;
   p.expert_ids = expert_ids;
   p.topk_w = mul_topk_weights ? topk_weights : nullptr;
