@@ -417,9 +417,8 @@ int qdq_rmsnorm_mxfp8(const void* x, const void* residual, const void* weight, v
  * row stride lds).  W: E4M3 codes [N, K] (row stride ldw bytes, 16-byte
  * aligned) with E8M0 scales per 32 in the tiled layout of qdq_sf_tile (block
  * 32, qdq_sf_tiled_bytes(N, K)).  K % 32 == 0.
- * Stream order: launched with programmatic dependent launch; W and its scales
- * may be read while the previous kernel on the stream finishes and must not be
- * written by it.  Everything else keeps full stream order.
+ * Launched with programmatic dependent launch, in full stream order: nothing is
+ * read before the work before it on the stream is complete.
  */
 int fp8_gemm_mxf8(const void* a_codes, const void* a_scales, int64_t lda, int64_t lds, const void* w_codes,
                   const void* w_sf_tiled, const void* bias, void* c, int64_t M, int64_t N, int64_t K,

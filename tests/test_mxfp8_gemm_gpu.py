@@ -487,3 +487,44 @@ def test_moe_tile_choices(cuda_device, m, e, top_k, bs, n, k):
         out = mxfp8_moe_linear(rows, w, sid, eid, ntp, tw, bs, top_k, mul)
         check_moe(out, _rows_values(rows), codes, scales, ids, f"m={m} e={e} n={n}", tw if mul else None)
     _ok()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 1024), (5, 640, 4128), (60, 2048, 512), (100, 512, 1024), (2100, 1280, 288)])
+def test_weight_changed_by_the_kernel_before(cuda_device, m, n, k):
+    """A weight's codes and scales changed in place right before each product, eager and captured."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    dev = cuda_device
+    a = activation(m, k, torch.bfloat16, m, dev)
+    rows = mxfp8_rows(a)
+    codes, scales = random_weight(n, k, seed=3, dev=dev)
+    codes.bitwise_and_(0x87)  # room for a change of the exponent that leaves no NaN
+    w = prepare_mxfp8_weight(codes.clone(), scales)
+    sf = w.sf_tiled.clone()
+    steps = [(x, i) for i in range(1, 6) for x in (a, rows)]
+    want = [mxfp8_linear(x, prepare_mxfp8_weight(codes + 8 * i, scales + i)) for x, i in steps]
+    ints, tiled = codes.to(torch.int16), sf.to(torch.int16)
+
+    def run():
+        got = []
+        for x, i in steps:
+            torch.add(ints, 8 * i, out=w.codes)  # converting kernels, not copies
+            torch.add(tiled, i, out=w.sf_tiled)
+            got.append(mxfp8_linear(x, w))
+            w.sf_tiled.fill_(0)
+            w.codes.fill_(0x38)
+            got.append(mxfp8_linear(x, w))
+        return got
+
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = run()
+        assert all(torch.equal(g, e) for g, e in zip(got[::2], want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, e) for g, e in zip(got[::2], want))
+    _ok()

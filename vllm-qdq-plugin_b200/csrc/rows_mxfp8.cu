@@ -116,8 +116,10 @@ __global__ void __launch_bounds__(kRowThreads)
 rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t M,
                   uint32_t upr, uint32_t tpr, int64_t ldx, int64_t ldc, int64_t lds, float zero) {
   using F = Fmt<kDtype>;
-  pdl_launch_dependents();
+  // In this order: a dependent that starts early still finds all that was written before this kernel (the few-rows
+  // product reads its weight then).
   pdl_wait();
+  pdl_launch_dependents();
   const uint32_t rpc = kRowThreads / tpr, t = threadIdx.x & (tpr - 1);
   const int64_t row = static_cast<int64_t>(blockIdx.x) * rpc + threadIdx.x / tpr;
   const bool in_m = row < M;

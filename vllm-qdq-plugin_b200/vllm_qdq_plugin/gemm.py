@@ -453,12 +453,6 @@ class Mxfp8MoeWeight:
     k: int
 
 
-def _settle(device: torch.device) -> None:
-    """A kernel behind the one that laid a weight out.  The MXFP8 product of few rows starts to read its weight while
-    the kernel just before it on the stream finishes, so that kernel must not be the one that writes the weight."""
-    torch.zeros(1, device=device)
-
-
 def _check_mxfp8_weight(codes: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
     _native.require_cuda(codes, scales)
     _native.same_device(codes.device, scales)
@@ -475,7 +469,6 @@ def prepare_mxfp8_weight(codes: torch.Tensor, scales: torch.Tensor, bias: torch.
     n, k = codes.shape
     with _native.on_device(codes.device):
         sf = _tile_scales(scales, n, k)
-        _settle(codes.device)
     return Mxfp8Weight(codes=codes, sf_tiled=sf, n=n, k=k, bias=bias)
 
 
@@ -496,7 +489,6 @@ def prepare_mxfp8_moe_weight(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp8
         else:
             for i in range(e):
                 _native.call("qdq_sf_tile", scales[i].data_ptr(), sf[i * per:].data_ptr(), n, k, k // 32, 32, stream)
-        _settle(codes.device)
     return Mxfp8MoeWeight(codes=codes, sf_tiled=sf, e=e, n=n, k=k)
 
 
