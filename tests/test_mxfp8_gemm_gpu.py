@@ -528,3 +528,25 @@ def test_weight_changed_by_the_kernel_before(cuda_device, m, n, k):
     torch.cuda.synchronize()
     assert all(torch.equal(g, e) for g, e in zip(got[::2], want))
     _ok()
+
+
+def test_weights_that_were_not_prepared_are_refused(cuda_device):
+    import dataclasses
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    m, n, k, e, dev = 4, 200, 512, 2, cuda_device
+    a = activation(m, k, torch.bfloat16, 1, dev)
+    rows = mxfp8_rows(a)
+    codes, scales = random_weight(e, n, k, seed=1, dev=dev)
+    one, many = prepare_mxfp8_weight(codes[0], scales[0]), prepare_mxfp8_moe_weight(codes, scales)
+    _, sid, eid, ntp, tw = routing(m, e, 1, 16, 1, dev)
+    wide = torch.zeros((n, k), dtype=torch.bfloat16, device=dev)
+    across = codes[0].t().contiguous().t()
+    for x in (a, rows):
+        for change in ({"sf_tiled": one.sf_tiled[:-1]}, {"sf_tiled": scales[0]}, {"codes": wide}, {"codes": across}):
+            with pytest.raises(RuntimeError, match="weight's"):
+                mxfp8_linear(x, dataclasses.replace(one, **change))
+        for change in ({"sf_tiled": one.sf_tiled}, {"sf_tiled": scales[0]}, {"codes": wide.expand(e, n, k).contiguous()}):
+            with pytest.raises(RuntimeError, match="weight's"):
+                mxfp8_moe_linear(x, dataclasses.replace(many, **change), sid, eid, ntp, tw, 16, 1, True)
+    _ok()

@@ -146,8 +146,16 @@ std::vector<Tensor> rmsnorm_mxfp8(const Tensor& x_, const Tensor& weight, const 
   return out;
 }
 
+// A weight's scales in the tiled layout.
+void check_scales(const char* name, const Tensor& sf, int64_t need) {
+  TORCH_CHECK(sf.element_size() == 1 && sf.is_contiguous() && sf.numel() >= need, name, ": the weight's tiled scales need ",
+              need, " bytes, got ", sf.numel());
+}
+
 void check_linear(const char* name, const Tensor& a, const Tensor& w, const Tensor& sf, const std::optional<Tensor>& bias) {
   TORCH_CHECK(w.dim() == 2 && w.size(1) == a.size(1), name, ": K=", a.size(1), " of the activation is not the weight's");
+  TORCH_CHECK(w.element_size() == 1 && w.stride(1) == 1, name, ": the weight's codes must be bytes, dense along K");
+  check_scales(name, sf, qdq_sf_tiled_bytes(w.size(0), w.size(1)));
   check_device(a, w);
   check_device(a, sf);
   if (bias.has_value()) {
@@ -192,6 +200,8 @@ void mxfp8_moe_linear_out(const Tensor& a_, const std::optional<Tensor>& a_scale
   else check_rows(name, a_, *a_scales);
   TORCH_CHECK(w.dim() == 3 && w.is_contiguous() && w.size(2) == a_.size(1), name, ": K=", a_.size(1),
               " of the activation is not the weight's");
+  TORCH_CHECK(w.element_size() == 1, name, ": the weight's codes must be bytes");
+  check_scales(name, sf, w.size(0) * qdq_sf_tiled_bytes(w.size(1), w.size(2)));
   TORCH_CHECK(top_k >= 1 && block >= 1 && block <= 64, name, ": top_k must be positive, moe_block_size in [1, 64]");
   const int64_t slots = a_.size(0) * top_k, n = w.size(1);
   for (const Tensor* t : {&sorted_ids, &expert_ids, &num_post_padded}) {
