@@ -739,10 +739,9 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         for (int j = 0; j < kR; ++j) {
           if (lane + 32 * j < n_mma) {
             uint8_t* at = sf + (j >> 2) * 512 + lane * 16 + (j & 3) * 4;
-            *reinterpret_cast<uint32_t*>(at) = v[j].x;
-            *reinterpret_cast<uint32_t*>(at + 1024) = v[j].y;
-            *reinterpret_cast<uint32_t*>(at + 2048) = v[j].z;
-            *reinterpret_cast<uint32_t*>(at + 3072) = v[j].w;
+            const uint32_t four[4] = {v[j].x, v[j].y, v[j].z, v[j].w};  // one word for each stage of the quad
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(at + i * 1024) = four[i];
           }
         }
         fence_proxy_async_smem();
