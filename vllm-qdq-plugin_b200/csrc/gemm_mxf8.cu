@@ -68,12 +68,13 @@ struct __align__(8) TBars {
   int abort;
 };
 constexpr int kSmemMax = 227 * 1024;
+constexpr int T_OUT = 16 * TM * 2;  // an epilogue half's output rows on their way out
 __host__ __device__ constexpr int t_stages(int nt) {
-  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars)) - t_quads_bytes(nt)) / t_stage_bytes(nt);
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(TBars)) - t_quads_bytes(nt) - 2 * T_OUT) / t_stage_bytes(nt);
   return n < T_STAGES_MAX ? n : T_STAGES_MAX;
 }
 __host__ __device__ constexpr int t_smem(int nt) {
-  return 1024 + t_stages(nt) * t_stage_bytes(nt) + t_quads_bytes(nt) + static_cast<int>(sizeof(TBars));
+  return 1024 + t_stages(nt) * t_stage_bytes(nt) + t_quads_bytes(nt) + 2 * T_OUT + static_cast<int>(sizeof(TBars));
 }
 
 template <int kDtype>
@@ -211,75 +212,92 @@ __device__ __forceinline__ void column_rows(const GemmArgs& p, const Item& w, in
   if (kGrouped && p.topk_w != nullptr && slot >= 0) wt = __ldcg(p.topk_w + slot);
 }
 
-// Stores 32 accumulator columns (activation rows) of this lane's W row n.
-// Eight neighbouring lanes hold eight neighbouring n: they transpose eight rows
-// among themselves in three exchanges (two n a word, two words, four), so that
-// a lane stores 16 bytes of each of four rows.  All exchanges come before the
-// stores.  (Stored two bytes at a time, each behind its row's shuffle, an item
-// of 240 rows took 18 k cycles where its MMAs take 15 k at K = 4096; four bytes
-// at a time 11 k.)  A C whose rows start on 4-byte boundaries only takes the
-// words of the first exchange.
-template <int kDtype, bool kGrouped>
-__device__ __forceinline__ void store_columns(const GemmArgs& p, const uint32_t (&r)[32], int n, int lane, int slot,
-                                              float wt, float bias) {
-  using O = Out16<kDtype>;
-  using T = typename O::T;
+// The output rows of 16 columns from shared memory, whole rows of 128 n at a
+// time by the half's four warps: kWidth neighbouring n a store.
+template <int kWidth, typename T>
+__device__ __forceinline__ void store_rows(const GemmArgs& p, const uint8_t* out, int n0, int t, int slot, int first) {
+  constexpr int kUnits = TM / kWidth, kRows = 128 / kUnits;  // stores a row, rows a pass
   T* C = static_cast<T*>(p.c);
-  if (p.wide > 1) {
-    const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
-    const bool scaled = kGrouped && p.topk_w != nullptr;
-    uint32_t v[16];  // word i: row 2 i + b0, n pair
+  const int j = t % kUnits * kWidth;  // this thread's n within the tile
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float x = __uint_as_float(r[2 * i]) + bias, y = __uint_as_float(r[2 * i + 1]) + bias;
-      const float other = __shfl_xor_sync(0xffffffffu, b0 ? x : y, 1);
-      float lo = b0 ? other : x, hi = b0 ? y : other;
-      if (scaled) {
-        const float f = __shfl_sync(0xffffffffu, wt, 2 * i + (lane & 1));
-        lo *= f;
-        hi *= f;
+  for (int i = 0; i < 16; i += kRows) {
+    const int r = i + t / kUnits;
+    const int row = __shfl_sync(0xffffffffu, slot, first + r);
+    const uint8_t* at = out + r * (2 * TM) + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2;
+    if (row < 0 || n0 + j >= p.N) continue;  // N is a multiple of kWidth
+    T* to = C + static_cast<int64_t>(row) * p.ldc + n0 + j;
+    if (kWidth == 8) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(at);
+    else if (kWidth == 2) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(at);
+    else *to = *reinterpret_cast<const T*>(at);
+  }
+}
+
+// Stores 32 accumulator columns (activation rows) of the tile's 128 W rows n0..:
+// the four warps of an epilogue half hold 32 W rows each as 8x8 fragments, which
+// stmatrix transposes into rows of the output in shared memory (16 rows at a
+// time; chunk j of row r lies at j ^ (r % 8), free of bank conflicts), and store
+// whole lines from there.  An item of 240 rows takes 5.6 k cycles, about half of
+// them for the stores.  (Transposed by shuffles in registers, with 64 bytes of a
+// row a store, it took 8 k, as long as its MMAs take at K = 2048; two bytes at a
+// time, each behind its row's shuffle, 18 k.)
+template <int kDtype, bool kGrouped>
+__device__ __forceinline__ void store_columns(const GemmArgs& p, uint32_t (&acc)[32], uint8_t* out, int half, int q,
+                                              int lane, int n0, int cols, int slot, float wt, const float (&bias)[4],
+                                              bool store) {
+  using O = Out16<kDtype>;
+  const uint32_t to = smem_u32(out) + (lane & 7) * (2 * TM) + (((4 * q + (lane >> 3)) ^ (lane & 7)) << 4);
+  // acc[16 h + 4 c + 2 g + e]: W row 16 h + 8 g + lane / 4 of the warp's, column 8 c + 2 (lane % 4) + e
+  if (!kGrouped && p.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) acc[i] = __float_as_uint(__uint_as_float(acc[i]) + bias[(i >> 4) * 2 + ((i >> 1) & 1)]);
+  }
+  if (kGrouped && p.topk_w != nullptr) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float f = __shfl_sync(0xffffffffu, wt, 8 * c + 2 * (lane & 3) + e);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          uint32_t& x = acc[(g >> 1) * 16 + 4 * c + 2 * (g & 1) + e];
+          x = __float_as_uint(__uint_as_float(x) * f);
+        }
       }
-      v[i] = O::two(lo, hi);
     }
-    if (p.wide == 2) {  // N is even: both n of a pair are inside, or neither
-      int at[16];
+  }
 #pragma unroll
-      for (int i = 0; i < 16; ++i) at[i] = __shfl_sync(0xffffffffu, slot, 2 * i + (lane & 1));
-      if (n < p.N) {
+  for (int s = 0; s < 2; ++s) {
+    if (16 * s >= cols) break;
+    uint32_t v[2][4];  // columns 16 s + 8 i .. + 7, W rows 8 g .. + 7 of the warp's
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (at[i] >= 0) *reinterpret_cast<uint32_t*>(C + static_cast<int64_t>(at[i]) * p.ldc + (n & ~1)) = v[i];
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t* a = acc + (g >> 1) * 16 + 4 * (2 * s + i) + 2 * (g & 1);
+        v[i][g] = O::two(__uint_as_float(a[0]), __uint_as_float(a[1]));
       }
-      return;
     }
-    uint32_t q[8][2];  // words of row 4 j + 2 b1 + b0, n quad
+    named_barrier(1 + half, 128);  // the rows before have been read
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, b1 ? v[2 * j] : v[2 * j + 1], 2);
-      q[j][0] = b1 ? other : v[2 * j];
-      q[j][1] = b1 ? v[2 * j + 1] : other;
+    for (int i = 0; i < 2; ++i) stmatrix_x4_trans(to + i * 8 * (2 * TM), v[i]);
+    named_barrier(1 + half, 128);
+    if (store) {
+      const int t = 32 * q + lane;
+      if (p.wide == 8) store_rows<8, typename O::T>(p, out, n0, t, slot, 16 * s);
+      else if (p.wide == 2) store_rows<2, typename O::T>(p, out, n0, t, slot, 16 * s);
+      else store_rows<1, typename O::T>(p, out, n0, t, slot, 16 * s);
     }
-    uint4 o[4];
-    int row[4];
+  }
+}
+
+// The bias of a lane's four W rows n + 8 g + lane / 4 of the warp's 32.
+template <int kDtype>
+__device__ __forceinline__ void fragment_bias(const GemmArgs& p, int n, int lane, float (&bias)[4]) {
+  using O = Out16<kDtype>;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {  // row 8 j + lane % 8, n octet
-      const uint32_t o0 = __shfl_xor_sync(0xffffffffu, b2 ? q[2 * j][0] : q[2 * j + 1][0], 4);
-      const uint32_t o1 = __shfl_xor_sync(0xffffffffu, b2 ? q[2 * j][1] : q[2 * j + 1][1], 4);
-      o[j] = b2 ? make_uint4(o0, o1, q[2 * j + 1][0], q[2 * j + 1][1]) : make_uint4(q[2 * j][0], q[2 * j][1], o0, o1);
-      row[j] = __shfl_sync(0xffffffffu, slot, 8 * j + (lane & 7));
-    }
-    if (n < p.N) {  // N is a multiple of 8: an octet is inside or outside as a whole
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (row[j] >= 0) *reinterpret_cast<uint4*>(C + static_cast<int64_t>(row[j]) * p.ldc + (n & ~7)) = o[j];
-    }
-  } else {
-#pragma unroll
-    for (int l = 0; l < 32; ++l) {
-      const int s = __shfl_sync(0xffffffffu, slot, l);
-      const float f = __shfl_sync(0xffffffffu, wt, l);
-      if (s >= 0 && n < p.N) C[static_cast<int64_t>(s) * p.ldc + n] = O::one(__uint_as_float(r[l]) * f + bias);
-    }
+  for (int g = 0; g < 4; ++g) {
+    const int at = n + 8 * g + (lane >> 2);
+    bias[g] = p.bias != nullptr && at < p.N ? O::load(static_cast<const typename O::T*>(p.bias) + at) : 0.f;
   }
 }
 
@@ -291,11 +309,12 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // code stages | quads of W scales | quads of activation scales | barriers
+  // code stages | quads of W scales | quads of activation scales | output rows | barriers
   const int S = t_stages(p.nt), stage_bytes = T_W + p.nt * TK, sf_bytes = t_sf_bytes(p.nt);
   uint8_t* s_sfw = smem + S * stage_bytes;
   uint8_t* s_sfa = s_sfw + 4 * T_SCALE * 512;
-  TBars* bars = reinterpret_cast<TBars*>(s_sfa + 4 * T_SCALE * sf_bytes);
+  uint8_t* s_out = s_sfa + 4 * T_SCALE * sf_bytes;
+  TBars* bars = reinterpret_cast<TBars*>(s_out + 2 * T_OUT);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int n_tiles = (p.N + TM - 1) / TM;
   const int num_kt = (p.K + TK - 1) / TK;
@@ -477,19 +496,19 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   } else {
     // ---------------- epilogue: warp reads TMEM lanes 32 (warp % 4).., column chunks half, half + 2, ...
     const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
-    constexpr int kCh = (NT_MAX / 32 + 1) / 2;
+    uint8_t* out = s_out + half * T_OUT;
     bool ok = true;
     int j = 0;
     while (walk.advance(w)) {
       if (w.rows == 0) continue;
       const int nchunks = (w.rows + 31) / 32;
       // output rows of this warp's columns, fetched while the MMAs run
-      int slot[kCh];
-      float wt[kCh];
-#pragma unroll
-      for (int u = 0; u < kCh; ++u) column_rows<kGrouped>(p, w, half + 2 * u, lane, slot[u], wt[u]);
-      const int n = w.n_tile * TM + q * 32 + lane;
-      const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+      int slot;
+      float wt;
+      column_rows<kGrouped>(p, w, half, lane, slot, wt);
+      const int n0 = w.n_tile * TM;
+      float bias[4];
+      fragment_bias<kDtype>(p, n0 + q * 32, lane, bias);
       const int buf = j & 1;
       if (ok) ok = mbar_wait(&bars->acc_full[buf], (j >> 1) & 1, p.status, 0x607);
       ok = __all_sync(0xffffffffu, ok);
@@ -500,19 +519,20 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         tc_fence_before();
         mbar_arrive(&bars->acc_empty[buf]);
       }
-#pragma unroll
-      for (int u = 0; u < kCh; ++u) {
-        const int c = half + 2 * u;
-        if (c >= nchunks) break;
+#pragma unroll 1
+      for (int c = half; c < nchunks; c += 2) {
         uint32_t r[32];
-        tmem_ld32(taddr + 32 * c, r);
+        tmem_ld_frag(taddr + 32 * c, r);
+        tmem_ld_frag(taddr + (16u << 16) + 32 * c, r + 16);
         tmem_ld_wait();
         if (c + 2 >= nchunks) {  // this warp's last chunk of the item
           tc_fence_before();
           mbar_arrive(&bars->acc_empty[buf]);
         }
-        if (!store) continue;
-        store_columns<kDtype, kGrouped>(p, r, n, lane, slot[u], wt[u], bias);
+        const int rows = slot;
+        const float factor = wt;
+        column_rows<kGrouped>(p, w, c + 2, lane, slot, wt);  // the next chunk's
+        store_columns<kDtype, kGrouped>(p, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
       }
       ++j;
     }
@@ -560,11 +580,11 @@ struct __align__(8) PBars {
 __host__ __device__ constexpr int p_stage_bytes(int tok) { return T_W + tok * TK; }  // tok: token rows held by a CTA
 constexpr int P_QUADS = 4 * T_SCALE * (1024 + 512);
 __host__ __device__ constexpr int p_stages(int tok) {
-  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(PBars)) - P_QUADS) / p_stage_bytes(tok);
+  const int n = (kSmemMax - 1024 - static_cast<int>(sizeof(PBars)) - P_QUADS - 2 * T_OUT) / p_stage_bytes(tok);
   return n < P_STAGES_MAX ? n : P_STAGES_MAX;
 }
 __host__ __device__ constexpr int p_smem(int tok) {
-  return 1024 + p_stages(tok) * p_stage_bytes(tok) + P_QUADS + static_cast<int>(sizeof(PBars));
+  return 1024 + p_stages(tok) * p_stage_bytes(tok) + P_QUADS + 2 * T_OUT + static_cast<int>(sizeof(PBars));
 }
 
 template <int kDtype, bool kGrouped>
@@ -575,12 +595,13 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  // code stages | quads of W scales | quads of activation scales | barriers
+  // code stages | quads of W scales | quads of activation scales | output rows | barriers
   const int tok_rows = (p.nt / 2 + p.box - 1) / p.box * p.box;
   const int S = p_stages(tok_rows), stage_bytes = p_stage_bytes(tok_rows);
   uint8_t* s_sfw = smem + S * stage_bytes;
   uint8_t* s_sfa = s_sfw + 4 * T_SCALE * 512;
-  PBars* bars = reinterpret_cast<PBars*>(s_sfa + 4 * T_SCALE * 1024);
+  uint8_t* s_out = s_sfa + 4 * T_SCALE * 1024;
+  PBars* bars = reinterpret_cast<PBars*>(s_out + 2 * T_OUT);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int n_tiles = (p.N + 2 * TM - 1) / (2 * TM);
@@ -754,18 +775,18 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
   } else {
     // ---------------- epilogue (both CTAs): TMEM lanes = the CTA's 128 W rows, columns = activation rows
     const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
-    constexpr int kCh = (P_NT_MAX / 32 + 2) / 2;
+    uint8_t* out = s_out + half * T_OUT;
     Cursor acc_at;
     bool ok = true;
     while (walk.advance(w)) {
       if (w.rows == 0) continue;
       const int nchunks = (w.rows + 31) / 32;
-      int slot[kCh];
-      float wt[kCh];
-#pragma unroll
-      for (int u = 0; u < kCh; ++u) column_rows<kGrouped>(p, w, half + 2 * u, lane, slot[u], wt[u]);
-      const int n = w.n_tile * 2 * TM + static_cast<int>(rank) * TM + q * 32 + lane;
-      const float bias = (!kGrouped && p.bias != nullptr && n < p.N) ? O::load(static_cast<const T*>(p.bias) + n) : 0.f;
+      int slot;
+      float wt;
+      column_rows<kGrouped>(p, w, half, lane, slot, wt);
+      const int n0 = (2 * w.n_tile + static_cast<int>(rank)) * TM;
+      float bias[4];
+      fragment_bias<kDtype>(p, n0 + q * 32, lane, bias);
       const uint32_t acc_empty0 = cluster_addr(&bars->acc_empty[acc_at.slot], 0);
       if (ok) ok = mbar_wait(&bars->acc_full[acc_at.slot], acc_at.phase, p.status, 0x80a);
       ok = __all_sync(0xffffffffu, ok);
@@ -777,20 +798,21 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(acc_empty0);
       }
-#pragma unroll
-      for (int u = 0; u < kCh; ++u) {
-        const int c = half + 2 * u;
-        if (c >= nchunks) break;
+#pragma unroll 1
+      for (int c = half; c < nchunks; c += 2) {
         uint32_t r[32];
-        tmem_ld32(taddr + 32 * c, r);
+        tmem_ld_frag(taddr + 32 * c, r);
+        tmem_ld_frag(taddr + (16u << 16) + 32 * c, r + 16);
         tmem_ld_wait();
         if (c + 2 >= nchunks) {  // this warp's last chunk of the item
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(acc_empty0);
         }
-        if (!store) continue;
-        store_columns<kDtype, kGrouped>(p, r, n, lane, slot[u], wt[u], bias);
+        const int rows = slot;
+        const float factor = wt;
+        column_rows<kGrouped>(p, w, c + 2, lane, slot, wt);  // the next chunk's
+        store_columns<kDtype, kGrouped>(p, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
       }
       acc_at.next(2);
     }
