@@ -550,3 +550,23 @@ def test_weights_that_were_not_prepared_are_refused(cuda_device):
             with pytest.raises(RuntimeError, match="weight's"):
                 mxfp8_moe_linear(x, dataclasses.replace(many, **change), sid, eid, ntp, tw, 16, 1, True)
     _ok()
+
+
+@pytest.mark.parametrize("m,e,top_k,bs,n,k", [(700, 9, 8, 16, 64, 2080), (4200, 3, 2, 64, 200, 2048), (1500, 6, 4, 64, 136, 3104),
+                                              (130, 5, 2, 8, 640, 4128), (40, 40, 3, 64, 512, 8224), (2100, 300, 1, 1, 128, 96)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_moe_of_16_bit_rows_is_that_of_their_mxfp8_rows(cuda_device, m, e, top_k, bs, n, k, dtype):
+    """Rows that many slots share, rows split over several warps, one row a warp: the codes are always those of mxfp8_rows."""
+    from vllm_qdq_plugin.gemm import mxfp8_moe_linear, prepare_mxfp8_moe_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    a = activation(m, k, dtype, m + k, cuda_device)
+    wide = torch.nn.functional.pad(a, (8, 0))[:, 8:]  # rows further apart
+    codes, scales = random_weight(e, n, k, seed=n, dev=cuda_device)
+    w = prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, top_k, bs, m, cuda_device)
+    rows = mxfp8_rows(a)
+    want = mxfp8_moe_linear(rows, w, sid, eid, ntp, tw, bs, top_k, True)
+    check_moe(want, _rows_values(rows), codes, scales, ids, f"m={m} e={e} k={k}", tw)
+    for x in (a, wide):
+        assert torch.equal(mxfp8_moe_linear(x, w, sid, eid, ntp, tw, bs, top_k, True), want)
+    _ok()

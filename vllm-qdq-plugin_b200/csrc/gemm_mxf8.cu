@@ -1214,13 +1214,19 @@ constexpr int SEG_THREADS = 1024;
 __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int32_t* __restrict__ sorted_ids, int live,
                                int bs, int num_experts, int n_slots, int nbmax, int32_t* seg_tab) {
   __shared__ int s_start[32], s_count[32];
+  __shared__ int s_expert[1 + SEG_THREADS + P_NT_MAX];  // the chunk's, the block's before it and nbmax behind it
   const int t = threadIdx.x, lane = t & 31, wid = t >> 5, nw = blockDim.x >> 5;
   int carry_start = -1, carry_count = 0;
   for (int base = 0; base < live; base += blockDim.x) {
     const int b = base + t;
-    const int e = b < live ? __ldcg(expert_ids + b) : -1;
+    for (int i = t; i < 1 + SEG_THREADS + P_NT_MAX; i += blockDim.x) {
+      const int at = base - 1 + i;
+      s_expert[i] = at >= 0 && at < live ? __ldcg(expert_ids + at) : -1;
+    }
+    __syncthreads();
+    const int e = s_expert[1 + t];
     const bool valid = e >= 0 && e < num_experts;
-    const bool first = valid && (b == 0 || __ldcg(expert_ids + b - 1) != e);
+    const bool first = valid && (b == 0 || s_expert[t] != e);
     int start = first ? b : -1;  // the first block of b's run: a running maximum
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1244,7 +1250,7 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
     }
     if (seg) {
       int nb = 1;
-      while (nb < nbmax && b + nb < live && __ldcg(expert_ids + b + nb) == e) ++nb;
+      while (nb < nbmax && s_expert[1 + t + nb] == e) ++nb;  // nbmax <= P_NT_MAX
       reinterpret_cast<int4*>(seg_tab + 4)[at] = make_int4(b * bs, nb * bs, e, 0);
     }
     carry_start = last;
@@ -1252,38 +1258,54 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
     __syncthreads();
   }
   if (t == 0) seg_tab[0] = carry_count;
-  // Padding at a segment's end costs MMAs and loads in steps of 16 rows: cut it, a warp a segment.
+  // Padding at a segment's end costs MMAs and loads in steps of 16 rows: cut it, a warp four segments at a time, so
+  // that their loads overlap.
   if (bs > 16) {
-    for (int i = wid; i < carry_count; i += nw) {
-      int4* entry = reinterpret_cast<int4*>(seg_tab + 4) + i;
-      int4 e = *entry;
-      while (e.y > 0) {
-        const int r = e.y - 1 - lane, s = r >= 0 ? __ldcg(sorted_ids + e.x + r) : -1;
-        const unsigned live_rows = __ballot_sync(0xffffffffu, s >= 0 && s < n_slots);
-        if (live_rows != 0) {
-          e.y -= __ffs(live_rows) - 1;
-          break;
-        }
-        e.y = max(0, e.y - 32);
+    constexpr int kU = 4;
+    for (int i0 = wid * kU; i0 < carry_count; i0 += nw * kU) {
+      int4 e[kU];
+      int s[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        e[u] = i0 + u < carry_count ? reinterpret_cast<int4*>(seg_tab + 4)[i0 + u] : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int r = e[u].y - 1 - lane;
+        s[u] = r >= 0 ? __ldcg(sorted_ids + e[u].x + r) : -1;
       }
-      if (lane == 0) *entry = e;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        int rows = e[u].y;
+        while (rows > 0) {
+          const unsigned live_rows = __ballot_sync(0xffffffffu, s[u] >= 0 && s[u] < n_slots);
+          if (live_rows != 0) {
+            rows -= __ffs(live_rows) - 1;
+            break;
+          }
+          rows = max(0, rows - 32);
+          const int r = rows - 1 - lane;
+          s[u] = r >= 0 ? __ldcg(sorted_ids + e[u].x + r) : -1;
+        }
+        if (lane == 0 && i0 + u < carry_count) seg_tab[4 + 4 * (i0 + u) + 1] = rows;
+      }
     }
   }
 }
 
 // The pass before the grouped product: block 0 builds the segments, the others
-// lay the routed rows out in sorted order, a warp a row, quantising 16-bit rows
-// (kRaw) or copying MXFP8 rows.  Positions that no live slot fills keep what
-// the workspace held: their columns of the accumulators are dropped.  (Gathering
-// the rows in the product instead, by 4-row TMA gathers, took 65 cycles a
-// gather, 3100 a stage of 192 rows against 600 with boxes of sorted rows.)
+// lay the routed rows out in sorted order, 2^wpr_log warps a row with four
+// 16-byte loads in flight each, quantising 16-bit rows (kRaw) or copying MXFP8
+// rows.  Positions that no live slot fills keep what the workspace held: their
+// columns of the accumulators are dropped.  (Gathering the rows in the product
+// instead, by 4-row TMA gathers, took 65 cycles a gather, 3100 a stage of 192
+// rows against 600 with boxes of sorted rows.)
 template <int kDtype, bool kRaw>
 __global__ void __launch_bounds__(SEG_THREADS)
 mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const uint8_t* __restrict__ a_scales,
                         int64_t lds, const int32_t* __restrict__ sorted_ids, const int32_t* __restrict__ expert_ids,
                         const int32_t* __restrict__ num_post_padded, int bs, int num_blocks, int num_experts,
                         int nbmax, int top_k, int n_slots, int K, uint8_t* __restrict__ codes,
-                        uint8_t* __restrict__ scales, int64_t ldso, int32_t* seg_tab, float zero) {
+                        uint8_t* __restrict__ scales, int64_t ldso, int32_t* seg_tab, int wpr_log, float zero) {
   pdl_launch_dependents();
   pdl_wait();
   const int npp = __ldcg(num_post_padded);
@@ -1292,33 +1314,45 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
     build_segments(expert_ids, sorted_ids, live, bs, num_experts, n_slots, nbmax, seg_tab);
     return;
   }
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rpc = SEG_THREADS / 32 >> wpr_log;
+  const int part = warp & ((1 << wpr_log) - 1);
   const int64_t positions = static_cast<int64_t>(live) * bs;
   const int gpr = K / 32;
-  for (int64_t pos = static_cast<int64_t>(blockIdx.x - 1) * warps + (threadIdx.x >> 5); pos < positions;
-       pos += static_cast<int64_t>(gridDim.x - 1) * warps) {
+  for (int64_t pos = static_cast<int64_t>(blockIdx.x - 1) * rpc + (warp >> wpr_log); pos < positions;
+       pos += static_cast<int64_t>(gridDim.x - 1) * rpc) {
     const int s = __ldcg(sorted_ids + pos);
     if (s < 0 || s >= n_slots) continue;
-    const uint8_t* src = a + static_cast<int64_t>(s / top_k) * lda_bytes;
+    const uint4* src = reinterpret_cast<const uint4*>(a + static_cast<int64_t>(s / top_k) * lda_bytes);
     uint8_t* dst = codes + pos * K;
-    if (kRaw) {
-      for (int c0 = 0; c0 < 4 * gpr; c0 += 32) {  // 16-byte chunks of 8 elements, four lanes a group
-        const int c = c0 + lane;
-        const uint4 v = c < 4 * gpr ? __ldcg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-        uint32_t amax = absmax8(v);
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const int e = mx8_exp<kDtype>(amax);
-        if (c < 4 * gpr) {
-          *reinterpret_cast<uint2*>(dst + 8 * c) = chunk_codes<kDtype>(v, e, zero);
-          if ((c & 3) == 0) scales[pos * ldso + (c >> 2)] = static_cast<uint8_t>(e);
+    const int chunks = (kRaw ? 4 : 2) * gpr;  // 16-byte chunks: 8 elements, four lanes a group; or 16 codes
+    if (!kRaw) {
+      const uint4* from = reinterpret_cast<const uint4*>(a_scales + static_cast<int64_t>(s / top_k) * lds);
+      for (int c = part * 32 + lane; c < ldso / 16; c += 32 << wpr_log)
+        reinterpret_cast<uint4*>(scales + pos * ldso)[c] = __ldcg(from + c);
+    }
+    for (int c0 = part * 128; c0 < chunks; c0 += 128 << wpr_log) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + 32 * u + lane;
+        v[u] = c < chunks ? __ldcg(src + c) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int c = c0 + 32 * u + lane;
+        if (kRaw) {
+          uint32_t amax = absmax8(v[u]);
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+          amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+          const int e = mx8_exp<kDtype>(amax);
+          if (c < chunks) {
+            *reinterpret_cast<uint2*>(dst + 8 * c) = chunk_codes<kDtype>(v[u], e, zero);
+            if ((c & 3) == 0) scales[pos * ldso + (c >> 2)] = static_cast<uint8_t>(e);
+          }
+        } else if (c < chunks) {
+          reinterpret_cast<uint4*>(dst)[c] = v[u];
         }
       }
-    } else {
-      for (int c = lane; c < 2 * gpr; c += 32)
-        reinterpret_cast<uint4*>(dst)[c] = __ldcg(reinterpret_cast<const uint4*>(src) + c);
-      const uint4* from = reinterpret_cast<const uint4*>(a_scales + static_cast<int64_t>(s / top_k) * lds);
-      for (int c = lane; c < ldso / 16; c += 32) reinterpret_cast<uint4*>(scales + pos * ldso)[c] = __ldcg(from + c);
     }
   }
 }
@@ -1640,8 +1674,9 @@ extern "C" int fp8_linear_mxf8(const void* a, int64_t lda, int dtype, const void
 
 extern "C" int64_t fp8_moe_workspace_bytes(int64_t size_m, int64_t num_sorted, int moe_block_size, int64_t K) {
   if (size_m <= 0 || num_sorted <= 0 || moe_block_size <= 0 || K <= 0) return 0;
-  return up256(16 * (1 + num_sorted / moe_block_size)) + up256(num_sorted * K) +
-         up256(num_sorted * qdq_mxfp8_scale_stride(K));
+  const int64_t row = qdq_mxfp8_scale_stride(K);
+  return up256(16 * (1 + num_sorted / moe_block_size)) + up256(num_sorted * K) + up256(num_sorted * row) +
+         up256(size_m * K) + up256(size_m * row);
 }
 
 extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, const void* a_scales, int64_t ldac,
@@ -1715,6 +1750,20 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   uint8_t* codes = static_cast<uint8_t*>(workspace) + up256(16 * (1 + num_blocks));
   uint8_t* scales = codes + up256(num_sorted * K);
   const int64_t ldso = qdq_mxfp8_scale_stride(K);
+  // 16-bit rows that several slots read are quantised once, by a pass of their own, where it spares the pass below 2^23
+  // elements (4096 tokens, 4 of 32 experts, K = 2880: 60 -> 49 us a call; 1024 tokens, 8 of 32, K = 2048: 31 -> 27.5;
+  // 2048 tokens, 4 of 32, K = 1024, 6 M spared: no difference; 1024 tokens, 2 of 32, K = 2048, 2 M: 15.9 -> 17.3).
+  bool raw = a != nullptr;
+  if (raw && size_m * (top_k - 1) >= (1ll << 23) / K) {
+    uint8_t* once = scales + up256(num_sorted * ldso);
+    uint8_t* once_scales = once + up256(size_m * K);
+    if (int st = qdq_mxfp8_rows(a, once, once_scales, size_m, K, lda, K, ldso, dtype, stream)) return st;
+    raw = false;
+    a_codes = once;
+    a_scales = once_scales;
+    ldac = K;
+    lds = ldso;
+  }
   GemmArgs p = {};
   // An average expert's rows in whole blocks, over as many experts as can be hit.  Few rows per item leave the shared
   // memory to more stages of W in flight; boxes leave a ragged segment few idle rows.
@@ -1731,15 +1780,19 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   if (!pair) p.nt = std::min(NT_MAX, (p.nt + p.box - 1) / p.box * p.box);
   const int nbmax = p.nt / moe_block_size;
   {
-    const int warps = SEG_THREADS / 32;
-    const int64_t grid = 1 + std::min<int64_t>((num_sorted + warps - 1) / warps, 2 * device_sm_count());
-    auto* fn = a == nullptr ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, false>
+    // Several warps a row (128 chunks each) while all of them are resident at once.
+    int wpr_log = 0;
+    while (wpr_log < 5 && (128ll << wpr_log) < K / (raw ? 8 : 16) && (num_sorted << wpr_log) <= 32 * device_sm_count())
+      ++wpr_log;
+    const int64_t rpc = SEG_THREADS / 32 >> wpr_log;
+    const int64_t grid = 1 + std::min<int64_t>((num_sorted + rpc - 1) / rpc, 2 * device_sm_count());
+    auto* fn = !raw ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, false>
                : dtype == QDQ_DTYPE_FP16 ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_FP16, true>
                                          : &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, true>;
-    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, 1, static_cast<const uint8_t*>(a ? a : a_codes),
-                            a ? lda * 2 : ldac, static_cast<const uint8_t*>(a_scales), lds, sorted_token_ids,
+    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, 1, static_cast<const uint8_t*>(raw ? a : a_codes),
+                            raw ? lda * 2 : ldac, static_cast<const uint8_t*>(a_scales), lds, sorted_token_ids,
                             expert_ids, num_tokens_post_padded, moe_block_size, num_blocks, num_experts, nbmax, top_k,
-                            n_slots, K, codes, scales, ldso, seg_tab, 0.0f))
+                            n_slots, K, codes, scales, ldso, seg_tab, wpr_log, 0.0f))
       return st;
   }
   p.sfw = static_cast<const uint8_t*>(w_sf_tiled);
