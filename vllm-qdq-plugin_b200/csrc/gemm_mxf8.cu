@@ -212,23 +212,42 @@ __device__ __forceinline__ void column_rows(const GemmArgs& p, const Item& w, in
   if (kGrouped && p.topk_w != nullptr && slot >= 0) wt = __ldcg(p.topk_w + slot);
 }
 
+// Where the output goes: copies in registers (behind a barrier's memory clobber
+// every field of the kernel's arguments would be loaded again).
+struct Target {
+  void* c;
+  int64_t ldc;
+  int n, wide;
+  bool biased, scaled;
+  __device__ explicit Target(const GemmArgs& p)
+      : c(p.c), ldc(p.ldc), n(p.N), wide(p.wide), biased(p.bias != nullptr), scaled(p.topk_w != nullptr) {}
+};
+
 // The output rows of 16 columns from shared memory, whole rows of 128 n at a
-// time by the half's four warps: kWidth neighbouring n a store.
+// time by the half's four warps: kWidth neighbouring n a store, up to four
+// stores' words read before the first of them.
 template <int kWidth, typename T>
-__device__ __forceinline__ void store_rows(const GemmArgs& p, const uint8_t* out, int n0, int t, int slot, int first) {
+__device__ __forceinline__ void store_rows(const Target& to, const uint8_t* out, int n0, int t, int slot, int first) {
+  using Word = std::conditional_t<kWidth == 8, uint4, std::conditional_t<kWidth == 2, uint32_t, uint16_t>>;
   constexpr int kUnits = TM / kWidth, kRows = 128 / kUnits;  // stores a row, rows a pass
-  T* C = static_cast<T*>(p.c);
-  const int j = t % kUnits * kWidth;  // this thread's n within the tile
+  constexpr int kPasses = 16 / kRows, kBatch = kPasses < 4 ? kPasses : 4;
+  const int j = t % kUnits * kWidth, n = n0 + j;  // N is a multiple of kWidth
 #pragma unroll
-  for (int i = 0; i < 16; i += kRows) {
-    const int r = i + t / kUnits;
-    const int row = __shfl_sync(0xffffffffu, slot, first + r);
-    const uint8_t* at = out + r * (2 * TM) + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2;
-    if (row < 0 || n0 + j >= p.N) continue;  // N is a multiple of kWidth
-    T* to = C + static_cast<int64_t>(row) * p.ldc + n0 + j;
-    if (kWidth == 8) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(at);
-    else if (kWidth == 2) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(at);
-    else *to = *reinterpret_cast<const T*>(at);
+  for (int i0 = 0; i0 < kPasses; i0 += kBatch) {
+    Word x[kBatch];
+    int row[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = (i0 + i) * kRows + t / kUnits;
+      row[i] = __shfl_sync(0xffffffffu, slot, first + r);
+      x[i] = *reinterpret_cast<const Word*>(out + r * (2 * TM) + (((j >> 3) ^ (r & 7)) << 4) + (j & 7) * 2);
+    }
+    if (n < to.n) {
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (row[i] >= 0)
+          *reinterpret_cast<Word*>(static_cast<T*>(to.c) + static_cast<int64_t>(row[i]) * to.ldc + n) = x[i];
+    }
   }
 }
 
@@ -236,22 +255,22 @@ __device__ __forceinline__ void store_rows(const GemmArgs& p, const uint8_t* out
 // the four warps of an epilogue half hold 32 W rows each as 8x8 fragments, which
 // stmatrix transposes into rows of the output in shared memory (16 rows at a
 // time; chunk j of row r lies at j ^ (r % 8), free of bank conflicts), and store
-// whole lines from there.  An item of 240 rows takes 5.6 k cycles, about half of
-// them for the stores.  (Transposed by shuffles in registers, with 64 bytes of a
-// row a store, it took 8 k, as long as its MMAs take at K = 2048; two bytes at a
-// time, each behind its row's shuffle, 18 k.)
+// whole lines from there: [4080 x 128] -> 9472 in 25.0 us, where filling the output
+// takes 20.3.  (Transposed by shuffles in registers, 64 bytes of a row a store,
+// 41; with the accumulator handed back by an arrival with release, which waits
+// for the stores before it, 35.)
 template <int kDtype, bool kGrouped>
-__device__ __forceinline__ void store_columns(const GemmArgs& p, uint32_t (&acc)[32], uint8_t* out, int half, int q,
+__device__ __forceinline__ void store_columns(const Target& target, uint32_t (&acc)[32], uint8_t* out, int half, int q,
                                               int lane, int n0, int cols, int slot, float wt, const float (&bias)[4],
                                               bool store) {
   using O = Out16<kDtype>;
   const uint32_t to = smem_u32(out) + (lane & 7) * (2 * TM) + (((4 * q + (lane >> 3)) ^ (lane & 7)) << 4);
   // acc[16 h + 4 c + 2 g + e]: W row 16 h + 8 g + lane / 4 of the warp's, column 8 c + 2 (lane % 4) + e
-  if (!kGrouped && p.bias != nullptr) {
+  if (!kGrouped && target.biased) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) acc[i] = __float_as_uint(__uint_as_float(acc[i]) + bias[(i >> 4) * 2 + ((i >> 1) & 1)]);
   }
-  if (kGrouped && p.topk_w != nullptr) {
+  if (kGrouped && target.scaled) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
 #pragma unroll
@@ -283,9 +302,9 @@ __device__ __forceinline__ void store_columns(const GemmArgs& p, uint32_t (&acc)
     named_barrier(1 + half, 128);
     if (store) {
       const int t = 32 * q + lane;
-      if (p.wide == 8) store_rows<8, typename O::T>(p, out, n0, t, slot, 16 * s);
-      else if (p.wide == 2) store_rows<2, typename O::T>(p, out, n0, t, slot, 16 * s);
-      else store_rows<1, typename O::T>(p, out, n0, t, slot, 16 * s);
+      if (target.wide == 8) store_rows<8, typename O::T>(target, out, n0, t, slot, 16 * s);
+      else if (target.wide == 2) store_rows<2, typename O::T>(target, out, n0, t, slot, 16 * s);
+      else store_rows<1, typename O::T>(target, out, n0, t, slot, 16 * s);
     }
   }
 }
@@ -497,6 +516,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     // ---------------- epilogue: warp reads TMEM lanes 32 (warp % 4).., column chunks half, half + 2, ...
     const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
     uint8_t* out = s_out + half * T_OUT;
+    const Target target(p);
     bool ok = true;
     int j = 0;
     while (walk.advance(w)) {
@@ -532,7 +552,7 @@ mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         const int rows = slot;
         const float factor = wt;
         column_rows<kGrouped>(p, w, c + 2, lane, slot, wt);  // the next chunk's
-        store_columns<kDtype, kGrouped>(p, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
+        store_columns<kDtype, kGrouped>(target, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
       }
       ++j;
     }
@@ -776,6 +796,7 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     // ---------------- epilogue (both CTAs): TMEM lanes = the CTA's 128 W rows, columns = activation rows
     const int q = warp & 3, half = (warp - 2 - T_SCALE) >> 2;
     uint8_t* out = s_out + half * T_OUT;
+    const Target target(p);
     Cursor acc_at;
     bool ok = true;
     while (walk.advance(w)) {
@@ -796,7 +817,7 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
       if (half >= nchunks) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(acc_empty0);
+        if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0);
       }
 #pragma unroll 1
       for (int c = half; c < nchunks; c += 2) {
@@ -807,12 +828,12 @@ mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         if (c + 2 >= nchunks) {  // this warp's last chunk of the item
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_empty0);
+          if (lane == 0) mbar_arrive_cluster_relaxed(acc_empty0);
         }
         const int rows = slot;
         const float factor = wt;
         column_rows<kGrouped>(p, w, c + 2, lane, slot, wt);  // the next chunk's
-        store_columns<kDtype, kGrouped>(p, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
+        store_columns<kDtype, kGrouped>(target, r, out, half, q, lane, n0, w.rows - 32 * c, rows, factor, bias, store);
       }
       acc_at.next(2);
     }
