@@ -1775,7 +1775,7 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   // elements (4096 tokens, 4 of 32 experts, K = 2880: 60 -> 49 us a call; 1024 tokens, 8 of 32, K = 2048: 31 -> 27.5;
   // 2048 tokens, 4 of 32, K = 1024, 6 M spared: no difference; 1024 tokens, 2 of 32, K = 2048, 2 M: 15.9 -> 17.3).
   bool raw = a != nullptr;
-  if (raw && size_m * (top_k - 1) >= (1ll << 23) / K) {
+  if (raw && top_k > 1 && size_m * (top_k - 1) >= (1ll << 23) / K) {
     uint8_t* once = scales + up256(num_sorted * ldso);
     uint8_t* once_scales = once + up256(size_m * K);
     if (int st = qdq_mxfp8_rows(a, once, once_scales, size_m, K, lda, K, ldso, dtype, stream)) return st;
