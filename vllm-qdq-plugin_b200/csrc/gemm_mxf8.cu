@@ -1230,7 +1230,11 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // the same expert, cut into at most nbmax blocks.  One CTA; blocks are walked
 // in chunks of the CTA's size with carries, entries come out in order.
 // ---------------------------------------------------------------------------
+// Threads of the pass's CTAs.  Copying MXFP8 rows, three CTAs of 512 stand on an SM where one of 1024 did (64 tokens,
+// 4 of 128 experts: 281.6 -> 279.4 us a call; 911 tokens, 2 of 4: 9.7 -> 9.1); quantising, 1024 are faster (4096 tokens
+// of K = 4096: 40.7 us, with 512 43.3).
 constexpr int SEG_THREADS = 1024;
+__host__ __device__ constexpr int prepare_threads(bool raw) { return raw ? SEG_THREADS : SEG_THREADS / 2; }
 
 __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int32_t* __restrict__ sorted_ids, int live,
                                int bs, int num_experts, int n_slots, int nbmax, int32_t* seg_tab) {
@@ -1240,7 +1244,7 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
   int carry_start = -1, carry_count = 0;
   for (int base = 0; base < live; base += blockDim.x) {
     const int b = base + t;
-    for (int i = t; i < 1 + SEG_THREADS + P_NT_MAX; i += blockDim.x) {
+    for (int i = t; i < 1 + static_cast<int>(blockDim.x) + P_NT_MAX; i += blockDim.x) {
       const int at = base - 1 + i;
       s_expert[i] = at >= 0 && at < live ? __ldcg(expert_ids + at) : -1;
     }
@@ -1321,7 +1325,7 @@ __device__ void build_segments(const int32_t* __restrict__ expert_ids, const int
 // instead, by 4-row TMA gathers, took 65 cycles a gather, 3100 a stage of 192
 // rows against 600 with boxes of sorted rows.)
 template <int kDtype, bool kRaw>
-__global__ void __launch_bounds__(SEG_THREADS)
+__global__ void __launch_bounds__(prepare_threads(kRaw))
 mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const uint8_t* __restrict__ a_scales,
                         int64_t lds, const int32_t* __restrict__ sorted_ids, const int32_t* __restrict__ expert_ids,
                         const int32_t* __restrict__ num_post_padded, int bs, int num_blocks, int num_experts,
@@ -1335,7 +1339,7 @@ mxf8_moe_prepare_kernel(const uint8_t* __restrict__ a, int64_t lda_bytes, const 
     build_segments(expert_ids, sorted_ids, live, bs, num_experts, n_slots, nbmax, seg_tab);
     return;
   }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rpc = SEG_THREADS / 32 >> wpr_log;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rpc = prepare_threads(kRaw) / 32 >> wpr_log;
   const int part = warp & ((1 << wpr_log) - 1);
   const int64_t positions = static_cast<int64_t>(live) * bs;
   const int gpr = K / 32;
@@ -1802,15 +1806,17 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   const int nbmax = p.nt / moe_block_size;
   {
     // Several warps a row (128 chunks each) while all of them are resident at once.
+    const int threads = prepare_threads(raw), warps = threads / 32, per_sm = raw ? 1 : 3;
     int wpr_log = 0;
-    while (wpr_log < 5 && (128ll << wpr_log) < K / (raw ? 8 : 16) && (num_sorted << wpr_log) <= 32 * device_sm_count())
+    while ((2 << wpr_log) <= warps && (128ll << wpr_log) < K / (raw ? 8 : 16) &&
+           (num_sorted << wpr_log) <= static_cast<int64_t>(per_sm) * warps * device_sm_count())
       ++wpr_log;
-    const int64_t rpc = SEG_THREADS / 32 >> wpr_log;
-    const int64_t grid = 1 + std::min<int64_t>((num_sorted + rpc - 1) / rpc, 2 * device_sm_count());
+    const int64_t rpc = warps >> wpr_log;
+    const int64_t grid = 1 + std::min<int64_t>((num_sorted + rpc - 1) / rpc, std::max(2, per_sm) * device_sm_count());
     auto* fn = !raw ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, false>
                : dtype == QDQ_DTYPE_FP16 ? &mxf8_moe_prepare_kernel<QDQ_DTYPE_FP16, true>
                                          : &mxf8_moe_prepare_kernel<QDQ_DTYPE_BF16, true>;
-    if (int st = launch_pdl(who, fn, grid, SEG_THREADS, 0, s, 1, static_cast<const uint8_t*>(raw ? a : a_codes),
+    if (int st = launch_pdl(who, fn, grid, threads, 0, s, 1, static_cast<const uint8_t*>(raw ? a : a_codes),
                             raw ? lda * 2 : ldac, static_cast<const uint8_t*>(a_scales), lds, sorted_token_ids,
                             expert_ids, num_tokens_post_padded, moe_block_size, num_blocks, num_experts, nbmax, top_k,
                             n_slots, K, codes, scales, ldso, seg_tab, wpr_log, 0.0f))
