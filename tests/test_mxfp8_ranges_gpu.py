@@ -56,3 +56,37 @@ def test_gate_of_far_gates_and_large_factors(cuda_device, gate):
             assert ((got - want).abs() <= (2.0 ** -8 + 2.0 ** -3) * want.abs()).all(), (up, got[0, 0], want[0, 0])
             checked += 1
     assert checked
+
+
+@pytest.mark.parametrize("k", [64, 544, 2880, 8192, 32800])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-6])
+def test_rmsnorm_over_the_range_of_bf16(cuda_device, k, eps):
+    """Rows whose squares fp32 does not hold, next to ordinary ones: the norm is that of 64 bits."""
+    from vllm_qdq_plugin.qdq import mxfp8_quantize, rmsnorm_mxfp8
+    dev = cuda_device
+    exponents = [126, 100, 70, 63, 58, 40, 0, -40, -50, -62, -70, -100, -125, -131]
+    gen = torch.Generator(device=dev).manual_seed(k)
+    x = torch.rand(len(exponents), k, generator=gen, device=dev).double() + 0.5
+    x = x * torch.exp2(torch.tensor(exponents, device=dev).double())[:, None]
+    x[:, 1::2] *= -1
+    x[:, 5] *= 2.0 ** -40  # one small value among the others
+    x = x.to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(k, generator=gen, device=dev)).to(torch.bfloat16)
+    rows, _, y = rmsnorm_mxfp8(x, w, eps=eps, norm_out=True)
+    d = x.double()
+    want = d / (d.square().mean(1, keepdim=True) + eps).sqrt() * w.double()
+    # half a bf16 step and the fp32 path (sums, rsqrtf, products: 2^-17), absolutely half a step of the smallest numbers
+    bound = (2.0 ** -8 + 2.0 ** -17) * want.abs() + 2.0 ** -134
+    assert x.isfinite().all() and ((y.double() - want).abs() <= bound).all()
+    codes, scales = mxfp8_quantize(y)
+    assert torch.equal(rows.codes, codes) and torch.equal(rows.scales, scales)
+
+
+def test_rmsnorm_of_infinite_rows(cuda_device):
+    """An infinity makes its own row what the formula gives: 0 where h is finite, NaN where it is not."""
+    from vllm_qdq_plugin.qdq import rmsnorm_mxfp8
+    x = torch.ones(3, 96, dtype=torch.bfloat16, device=cuda_device)
+    x[1, 7] = float("inf")
+    y = rmsnorm_mxfp8(x, x[0], norm_out=True)[2]
+    assert y[1, 7].isnan() and not y[1, torch.arange(96, device=cuda_device) != 7].any()
+    assert torch.equal(y[0], y[2]) and (y[0] == 1).all()

@@ -161,6 +161,64 @@ rows_mxfp8_kernel(const uint16_t* __restrict__ x, uint8_t* __restrict__ codes, u
   }
 }
 
+// A value summed over the row's threads, the same in all of them.  The caller
+// has a barrier before `part` is written again.
+template <bool kWarpRow>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  if (!kWarpRow) {
+    if (lane == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lane < (blockDim.x >> 5) ? part[lane] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  }
+  return v;
+}
+
+// A bf16 row whose squares leave the range of fp32 (bf16 reaches from 2^-133 to
+// 2^128), from its stored h: summed as (h f)^2 with a power of two f, and
+// normalised as (h f) rsqrt(mean (h f)^2 + eps f^2) w.  It reads the row again:
+// scaled in the registers of the kernel below, it cost all rows the order of
+// their loads ([16384, 8192] 138.5 -> 150 us; this way 138.5, [32768, 1024]
+// 37.6 -> 38.8).
+template <bool kWarpRow>
+__device__ __forceinline__ void rmsnorm_far_row(const uint16_t* h, const uint16_t* w, uint16_t* y, uint8_t* codes,
+                                             uint8_t* scales, uint32_t upr, float* part, float f, float eps, float zero) {
+  using F = Fmt<QDQ_DTYPE_BF16>;
+  const uint32_t t = kWarpRow ? threadIdx.x & 31u : threadIdx.x, step = kWarpRow ? 32u : blockDim.x;
+  const uint4 *h4 = reinterpret_cast<const uint4*>(h), *w4 = reinterpret_cast<const uint4*>(w);
+  float sq = 0.f;
+#pragma unroll 1
+  for (uint32_t col = t; col < upr; col += step) {
+    uint32_t a8[8];
+    words({__ldcg(h4 + 2 * col), __ldcg(h4 + 2 * col + 1)}, a8);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = F::lo(a8[j]) * f, b = F::hi(a8[j]) * f;
+      sq = fmaf(a, a, fmaf(b, b, sq));
+    }
+  }
+  if (!kWarpRow) __syncthreads();  // the sums of the caller have been read
+  const float rs = rsqrtf(row_sum<kWarpRow>(sq, part) / (static_cast<float>(upr) * 16.0f) + eps * f * f);
+#pragma unroll 1
+  for (uint32_t col0 = 0; col0 < upr; col0 += step) {
+    const uint32_t col = col0 + t;
+    uint32_t a8[8] = {}, w8[8] = {};
+    if (col < upr) {
+      words({__ldcg(h4 + 2 * col), __ldcg(h4 + 2 * col + 1)}, a8);
+      words({__ldcg(w4 + 2 * col), __ldcg(w4 + 2 * col + 1)}, w8);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      a8[j] = F::pack(F::lo(a8[j]) * f * rs * F::lo(w8[j]), F::hi(a8[j]) * f * rs * F::hi(w8[j]));
+    if (y != nullptr && col < upr) store_unit<false>(y + col * 16u, unit_of(a8));
+    store_mxfp8<QDQ_DTYPE_BF16>(a8, codes, scales, col, col < upr, zero);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // rmsnorm: one row per warp (kWarpRow, up to 32 * kC units) or per CTA; the
 // row stays in registers (kC units per thread) between the sum of squares
@@ -182,7 +240,6 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
   const int64_t rstep = kWarpRow ? static_cast<int64_t>(gridDim.x) * (kRowThreads / 32) : gridDim.x;
   for (int64_t row = row0; row < M; row += rstep) {
     Unit h[kC];
-    float ss = 0.f;
     const uint16_t* xr = x + row * ldx;
 #pragma unroll
     for (int i = 0; i < kC; ++i) {
@@ -223,16 +280,14 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
         sq = fma_f32x2(a, a, sq);
       }
     }
-    ss = sq.x + sq.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
-    if (!kWarpRow) {
-      // the barrier at the loop's end keeps this row's sums until every thread has read them
-      if (lane == 0) part[warp] = ss;
-      __syncthreads();
-      ss = lane < (blockDim.x >> 5) ? part[lane] : 0.f;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+    // The barrier at the loop's end keeps this row's sums until every thread has read them.
+    const float ss = row_sum<kWarpRow>(sq.x + sq.y, part);
+    // Out of fp32's range, or so near its lower end that squares are lost and eps does not outweigh them.
+    if (kDtype == QDQ_DTYPE_BF16 && (!(ss <= 0x1p120f) || (ss < 0x1p-90f && eps < 0x1p-60f))) {
+      rmsnorm_far_row<kWarpRow>(res != nullptr ? h_out + row * ldh : xr, w, y_out != nullptr ? y_out + row * ldy : nullptr,
+                                codes + row * ldc, scales + row * lds, upr, part, ss < 1.0f ? 0x1p90f : 0x1p-80f, eps, zero);
+      if (!kWarpRow) __syncthreads();
+      continue;
     }
     const float rs = rsqrtf(ss / (static_cast<float>(upr) * 16.0f) + eps);
 #pragma unroll
