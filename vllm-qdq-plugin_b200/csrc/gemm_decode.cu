@@ -262,7 +262,7 @@ mxf4_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
     float gs = 0.f;
     if (kNV) {
       if (a_gs != nullptr) {
-        gs = __ldg(a_gs);
+        gs = ld_ordered(a_gs);
       } else {
         const uint32_t crank = cluster_rank();
         const int qt = threadIdx.x - 64, cpr = K / 8;  // 16-byte chunks per row
@@ -270,7 +270,7 @@ mxf4_decode_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_cons
         for (int i = qt + D_QUANT_THREADS * static_cast<int>(crank); i < M * cpr;
              i += D_QUANT_THREADS * kDecCluster) {
           const int row = i / cpr, c = i - row * cpr;
-          m8 = max(m8, absmax8(ld_stream(reinterpret_cast<const uint4*>(a_raw + row * lda + c * 8))));
+          m8 = max(m8, absmax8(ld_stream_ordered(reinterpret_cast<const uint4*>(a_raw + row * lda + c * 8))));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m8 = max(m8, __shfl_xor_sync(0xffffffffu, m8, o));

@@ -249,7 +249,7 @@ mxf4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_consta
     // ---------------- epilogue: TMEM lanes 32 (warp % 4).. = tile rows, columns 128 h ..
     const int q = warp & 3, h = (warp - 2) >> 2;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + ACC_COL + h * 128;
-    const float alpha = kNV ? w_gs / *a_gs : 1.0f;
+    const float alpha = kNV ? w_gs / ld_ordered(a_gs) : 1.0f;
     bool ok = true;
     int i = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++i) {
@@ -487,7 +487,7 @@ mxf4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_c
     pdl_wait();  // C, the bias and the activation's global scale belong to the stream's order
     const int q = warp & 3, h = (warp - 2) >> 2;
     const uint32_t taddr = tmem + (static_cast<uint32_t>(q * 32) << 16) + ACC_COL + h * 128;
-    const float alpha = kNV ? w_gs / *a_gs : 1.0f;
+    const float alpha = kNV ? w_gs / ld_ordered(a_gs) : 1.0f;
     const uint32_t acc_empty0 = cluster_addr(&bars->acc_empty, 0);
     bool ok = true;
     int i = 0;

@@ -88,7 +88,7 @@ mxfp4_vec_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ y,
         so[u] = (static_cast<uint64_t>(row >> 7) * static_cast<uint64_t>(lds) + (gi >> 2)) * 512u +
                 (row & 31u) * 16u + ((row >> 5) & 3u) * 4u + (gi & 3u);
       }
-      v[u] = ok[u] ? ld_stream(reinterpret_cast<const uint4*>(x + xo[u])) : make_uint4(0, 0, 0, 0);
+      v[u] = ok[u] ? ld_stream_in<kTiledSF>(reinterpret_cast<const uint4*>(x + xo[u])) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
@@ -201,7 +201,7 @@ nvfp4_vec_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ y,
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
   }
-  const float gs = __ldg(gsp);
+  const float gs = ld_in<kTiledSF>(gsp);
   const float rgs = zero_safe_recip(gs);
   const uint32_t lane = threadIdx.x & 31u;
   const uint64_t stride = static_cast<uint64_t>(gridDim.x) * blockDim.x * kUnroll;
@@ -233,7 +233,7 @@ nvfp4_vec_kernel(const uint16_t* __restrict__ x, uint16_t* __restrict__ y,
         so[u] = (static_cast<uint64_t>(row >> 7) * static_cast<uint64_t>(lds) + (gi >> 2)) * 512u +
                 (row & 31u) * 16u + ((row >> 5) & 3u) * 4u + (gi & 3u);
       }
-      v[u] = ok[u] ? ld_stream(reinterpret_cast<const uint4*>(x + xo[u])) : make_uint4(0, 0, 0, 0);
+      v[u] = ok[u] ? ld_stream_in<kTiledSF>(reinterpret_cast<const uint4*>(x + xo[u])) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -395,7 +395,7 @@ amax_gs_small_kernel(const uint16_t* __restrict__ x, int M, int K, int64_t ldx, 
 #pragma unroll 4
   for (int c = static_cast<int>(rank) * kThreads + threadIdx.x; c < total; c += kAmaxCtas * kThreads) {
     const int row = c / cpr, col = c - row * cpr;
-    m = max(m, absmax8(ld_stream(reinterpret_cast<const uint4*>(x + row * ldx + col * 8))));
+    m = max(m, absmax8(ld_stream_ordered(reinterpret_cast<const uint4*>(x + row * ldx + col * 8))));
   }
   m = __reduce_max_sync(kFull, m);
   if ((threadIdx.x & 31u) == 0) warp_max[threadIdx.x >> 5] = m;

@@ -41,12 +41,12 @@ template <bool kWide>
 __device__ __forceinline__ Unit load_unit(const uint16_t* p) {
   Unit u;
   if (kWide) {
-    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+    asm volatile("ld.global.L1::no_allocate.L2::256B.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(u.a.x), "=r"(u.a.y), "=r"(u.a.z), "=r"(u.a.w), "=r"(u.b.x), "=r"(u.b.y), "=r"(u.b.z), "=r"(u.b.w)
                  : "l"(p));
   } else {
     const uint4* q = reinterpret_cast<const uint4*>(p);
-    u = {ld_stream(q), ld_stream(q + 1)};
+    u = {ld_stream_ordered(q), ld_stream_ordered(q + 1)};
   }
   return u;
 }
@@ -296,7 +296,7 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
       Unit wv = zero_unit();
       if (col < upr) {
         const uint4* p = reinterpret_cast<const uint4*>(w + col * 16u);
-        wv = {__ldg(p), __ldg(p + 1)};
+        wv = {ld_ordered(p), ld_ordered(p + 1)};
       }
       uint32_t a8[8], w8[8];
       words(h[i], a8);
