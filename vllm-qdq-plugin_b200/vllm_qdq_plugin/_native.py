@@ -118,16 +118,24 @@ def lib() -> ctypes.CDLL:
 _OPS_LOADED = False
 
 
-def load_ops(x: torch.Tensor) -> None:
-    """Load (building first if missing or stale) the torch.library kernels of csrc/torch_ops.cpp for the CUDA tensor x."""
+# A compiler that traces a call runs this while it traces (the lock and ctypes cannot be traced) and keeps no guard on
+# _OPS_LOADED, which would compile the first call's graph again for the second.
+@torch.compiler.assume_constant_result
+def _load_ops() -> None:
     global _OPS_LOADED
     if not _OPS_LOADED:
-        require_cuda(x)
         lib()
         with _LOCK:
             if not _OPS_LOADED:
                 torch.ops.load_library(str(_build.TORCH_OPS_PATH))
                 _OPS_LOADED = True
+
+
+def load_ops(x: torch.Tensor) -> None:
+    """Load (building first if missing or stale) the torch.library kernels of csrc/torch_ops.cpp for the CUDA tensor x."""
+    if not x.is_cuda:
+        require_cuda(x)
+    _load_ops()
 
 
 def library_path() -> str:

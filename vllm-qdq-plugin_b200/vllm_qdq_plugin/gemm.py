@@ -456,6 +456,7 @@ class Mxfp8MoeWeight:
 def _check_mxfp8_weight(codes: torch.Tensor, scales: torch.Tensor, dims: int) -> None:
     _native.require_cuda(codes, scales)
     _native.same_device(codes.device, scales)
+    _native.load_ops(codes)  # a graph compiled in another process may be the first to call the products
     assert codes.element_size() == 1 and scales.element_size() == 1, (codes.dtype, scales.dtype)
     assert codes.dim() == dims and codes.shape[-1] > 0 and codes.shape[-1] % 32 == 0, tuple(codes.shape)
     assert tuple(scales.shape) == (*codes.shape[:-1], codes.shape[-1] // 32), (codes.shape, scales.shape)
