@@ -12,6 +12,9 @@
 
 #include "qdq_b200.h"
 
+// The torch that this file was compiled against, as text in the library: it is rebuilt for another.
+extern "C" const char qdq_torch_ops_built_for[] = QDQ_BUILT_FOR;
+
 namespace {
 
 using at::Tensor;

@@ -127,7 +127,7 @@ def _load_ops() -> None:
         lib()
         with _LOCK:
             if not _OPS_LOADED:
-                torch.ops.load_library(str(_build.TORCH_OPS_PATH))
+                torch.ops.load_library(str(_build.build_ops()))
                 _OPS_LOADED = True
 
 
