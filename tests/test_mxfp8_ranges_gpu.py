@@ -5,6 +5,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+from mxfp8_cases import activation, check_moe, check_product, random_weight, routing, values
+
 pytestmark = pytest.mark.gpu
 
 
@@ -90,3 +92,109 @@ def test_rmsnorm_of_infinite_rows(cuda_device):
     y = rmsnorm_mxfp8(x, x[0], norm_out=True)[2]
     assert y[1, 7].isnan() and not y[1, torch.arange(96, device=cuda_device) != 7].any()
     assert torch.equal(y[0], y[2]) and (y[0] == 1).all()
+
+
+def _far_groups(m, k, dev):
+    """bf16 groups with maxima of 2^20 to 2^127 (scale exponents to both sides of 143), values up to 2^200 below them and
+    zeros of both signs among them."""
+    gen = torch.Generator(device=dev).manual_seed(m + k)
+    exponent = torch.randint(20, 127, (m, k // 32), generator=gen, device=dev).double().repeat_interleave(32, 1)
+    below = torch.randint(0, 200, (m, k), generator=gen, device=dev).double()
+    below[torch.rand(m, k, generator=gen, device=dev) < 0.6] = 0
+    x = (torch.randn(m, k, generator=gen, device=dev).double() * torch.exp2(exponent - below)).to(torch.bfloat16)
+    x[torch.rand(m, k, generator=gen, device=dev) < 0.1] = -0.0
+    x[torch.rand(m, k, generator=gen, device=dev) < 0.1] = 0.0
+    assert x.isfinite().all()
+    return x
+
+
+def test_rows_of_large_values(cuda_device):
+    from vllm_qdq_plugin.qdq import mxfp8_qdq, mxfp8_quantize, mxfp8_rows
+    x = _far_groups(300, 544, cuda_device)
+    rows = mxfp8_rows(x)
+    codes, scales = mxfp8_quantize(x)
+    assert int(scales.min()) < 143 < int(scales.max())
+    assert torch.equal(rows.codes, codes) and torch.equal(rows.scales, scales)
+    assert torch.equal(rows.dequantize(), mxfp8_qdq(x))
+
+
+@pytest.mark.parametrize("m", [2, 50, 300])
+def test_products_of_large_16_bit_rows(cuda_device, m):
+    """Quantised inside the product of few rows, by the pass before it, and by the experts' layout pass."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    dev, k, n, e = cuda_device, 288, 200, 3
+    x = _far_groups(m, k, dev) * 2.0 ** -60  # the sums stay in bf16's range; groups keep exponents beyond 143 - 60
+    big = _far_groups(m, k, dev)
+    codes, scales = random_weight(e, n, k, seed=1, dev=dev)
+    w, wm = prepare_mxfp8_weight(codes[0], scales[0]), prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, 2, 16, 1, dev)
+    rows = mxfp8_rows(x)
+    a = values(rows.codes, rows.scales)
+    check_product(mxfp8_linear(x, w), a, values(codes[0], scales[0]), what=f"m={m}")
+    check_moe(mxfp8_moe_linear(x, wm, sid, eid, ntp, tw, 16, 2, True), a, codes, scales, ids, f"experts m={m}", tw)
+    # the codes inside are those of mxfp8_rows, whatever the exponent: the same product of both
+    rows = mxfp8_rows(big)
+    assert int(rows.scales.max()) > 143
+    same = lambda a, b: torch.equal(a.nan_to_num(1, 2, 3), b.nan_to_num(1, 2, 3))  # noqa: E731
+    assert same(mxfp8_linear(big, w), mxfp8_linear(rows, w))
+    assert same(mxfp8_moe_linear(big, wm, sid, eid, ntp, tw, 16, 2, True), mxfp8_moe_linear(rows, wm, sid, eid, ntp, tw, 16, 2, True))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+@pytest.mark.parametrize("m", [3, 70, 300])
+def test_products_of_rows_that_are_not_finite(cuda_device, m, bad):
+    """The rule of mxfp8_qdq: a NaN makes its row's outputs NaN; an infinity gives its group the scale 2^-127, in which
+    the infinity saturates to 448 2^-127 and the finite values beside it to as little.  Other rows are as they were."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, mxfp8_moe_linear, prepare_mxfp8_moe_weight, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_qdq, mxfp8_rows
+    dev, n, k, e = cuda_device, 160, 416, 2
+    x = activation(m, k, torch.bfloat16, 9, dev)
+    x[m // 2, 37] = bad
+    codes, scales = random_weight(e, n, k, seed=4, dev=dev)
+    w, wm = prepare_mxfp8_weight(codes[0], scales[0]), prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, 1, 16, 1, dev)
+    q = mxfp8_qdq(x).double()
+    clean = torch.arange(m, device=dev) != m // 2
+    for a in (x, mxfp8_rows(x)):
+        out, grouped = mxfp8_linear(a, w), mxfp8_moe_linear(a, wm, sid, eid, ntp, tw, 16, 1, False)
+        if bad != bad:
+            assert out[m // 2].isnan().all() and grouped[m // 2].isnan().all()
+        else:
+            assert q.isfinite().all() and q[m // 2, 32:64].abs().max() <= 448 * 2.0 ** -127
+            check_product(out[~clean], q[~clean], values(codes[0], scales[0]), what=f"m={m}")
+        check_product(out[clean], q[clean], values(codes[0], scales[0]), what=f"m={m}")
+        rest = clean.nonzero()[:, 0]
+        check_moe(grouped[rest], q[rest], codes, scales, ids[rest.cpu().numpy()], f"experts m={m}")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 50257, 64), (64, 20000, 96), (1, 64, 131072), (3, 130, 262144), (70, 128, 65536),
+                                   (100000, 8, 32)])
+def test_linear_of_extreme_shapes(cuda_device, m, n, k):
+    """More W tiles than SMs for one token, K beyond what a CTA keeps, many rows of a narrow weight."""
+    from vllm_qdq_plugin.gemm import mxfp8_linear, prepare_mxfp8_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    x = activation(m, k, torch.bfloat16, m + n, cuda_device)
+    codes, scales = random_weight(n, k, seed=n, dev=cuda_device)
+    w = prepare_mxfp8_weight(codes, scales)
+    rows = mxfp8_rows(x)
+    a, exact_w = values(rows.codes, rows.scales), values(codes, scales)
+    for given in (x, rows):
+        check_product(mxfp8_linear(given, w), a, exact_w, what=f"{m}x{n}x{k}")
+
+
+@pytest.mark.parametrize("m,e,n,k", [(3, 1, 64, 131072), (40, 2, 40000, 32), (500, 1, 64, 32), (9, 500, 32, 64)])
+def test_experts_of_extreme_shapes(cuda_device, m, e, n, k):
+    """One expert, many, wide and long ones; num_tokens_post_padded beyond the sorted slots counts as all of them."""
+    from vllm_qdq_plugin.gemm import mxfp8_moe_linear, prepare_mxfp8_moe_weight
+    from vllm_qdq_plugin.qdq import mxfp8_rows
+    x = activation(m, k, torch.bfloat16, m + n, cuda_device)
+    codes, scales = random_weight(e, n, k, seed=n, dev=cuda_device)
+    w = prepare_mxfp8_moe_weight(codes, scales)
+    ids, sid, eid, ntp, tw = routing(m, e, 1, 16, 3, cuda_device)
+    live = int(ntp)
+    rows = mxfp8_rows(x)
+    a = values(rows.codes, rows.scales)
+    for given in (x, rows):
+        out = mxfp8_moe_linear(given, w, sid[:live].contiguous(), eid, ntp * 1000, tw, 16, 1, True)
+        check_moe(out, a, codes, scales, ids, f"m={m} e={e}", tw)

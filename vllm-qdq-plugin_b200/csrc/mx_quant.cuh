@@ -282,9 +282,11 @@ __device__ __forceinline__ float2 mx8_scaled(float a, float b, float inv, float 
 }
 
 // E4M3 codes of a bf16 pair, w = x * inv with inv >= 2^-16 a power of two (as
-// a bf16 pair): the product is exact in bf16 and fma(x, inv, +0) makes a -0
-// quotient +0; magnitudes in [7, 8) * 2^-9 (bf16 0x3C60 .. 0x3C7F) lose their
-// low mantissa bits as in mx8_pair_f16.
+// a bf16 pair): the product is exact in bf16 where it is a normal number, and
+// below that, far under 2^-10, it rounds to a value of its own sign whose code
+// is the zero of that sign, as that of the exact quotient; fma(x, inv, +0)
+// makes a -0 quotient +0.  Magnitudes in [7, 8) * 2^-9 (bf16 0x3C60 .. 0x3C7F)
+// lose their low mantissa bits as in mx8_pair_f16.
 __device__ __forceinline__ uint32_t mx8_pair_bf16(uint32_t x, uint32_t inv2, uint32_t zero2) {
   uint32_t t, eq, out;
   asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(t) : "r"(x), "r"(inv2), "r"(zero2));

@@ -113,7 +113,11 @@ def _check(name: str, x: torch.Tensor, k: int) -> None:
 # the errors of the other operators (AssertionError for shapes and types); they
 # run only where a call was refused, or has no CUDA tensor to dispatch on.
 def mxfp8_rows(x: torch.Tensor) -> Mxfp8Rows:
-    """MXFP8 rows of x [M, K] bf16/fp16 (CUDA, K % 32 == 0): the codes and scales of `mxfp8_quantize`."""
+    """MXFP8 rows of x [M, K] bf16/fp16 (CUDA, K % 32 == 0): the codes and scales of `mxfp8_quantize`.
+
+    A NaN stays one.  An infinity gives its group of 32 the scale 2^-127, in which it saturates and every value beside it
+    too: what the group then adds to a product is next to nothing (the rule of `mxfp8_qdq`).
+    """
     try:
         _native.load_ops(x)
         return Mxfp8Rows(*_rows_op(x), x.dtype)
@@ -144,6 +148,8 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
 
         h = x + residual              (rounded to x's dtype; h = x without a residual)
         y = h * rsqrt(mean(h^2) + eps) * weight     (fp32, rounded to x's dtype)
+
+    The squares' sum leaves fp32's range for no finite row, bf16's largest and smallest among them.
 
     Args:
         x: [M, K] bf16/fp16 (CUDA), K a multiple of 32 up to 65536.
