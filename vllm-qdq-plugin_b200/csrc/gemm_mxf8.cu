@@ -111,10 +111,9 @@ struct GemmArgs {
   int64_t ldc;
   const int32_t* seg_tab;      // grouped: [count, -, -, -], then (first position, rows, expert, -) per segment
   const int32_t* sorted_ids;
-  const int32_t* expert_ids;
   const float* topk_w;         // nullptr: no scaling
   int M, N, K, kchunks;        // M: dense rows, grouped slots (size_m * top_k)
-  int top_k, bs, num_blocks, num_experts;
+  int num_blocks, num_experts;
   int a_rows;                  // rows of the activation codes (grouped: sorted positions)
   int nt, box;                 // activation rows per item, and per TMA box
   int wide;                    // neighbouring n that C takes in one store: 8, 2 or 1
@@ -324,8 +323,6 @@ template <int kDtype, bool kGrouped>
 __global__ void __launch_bounds__(T_THREADS, 1)
 mxf8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
                  const __grid_constant__ GemmArgs p) {
-  using O = Out16<kDtype>;
-  using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // code stages | quads of W scales | quads of activation scales | output rows | barriers
@@ -611,8 +608,6 @@ template <int kDtype, bool kGrouped>
 __global__ void __launch_bounds__(T_THREADS, 1)
 mxf8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
                  const __grid_constant__ CUtensorMap tmap_sfw, const __grid_constant__ GemmArgs p) {
-  using O = Out16<kDtype>;
-  using T = typename O::T;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   // code stages | quads of W scales | quads of activation scales | output rows | barriers
@@ -1637,7 +1632,6 @@ int product_of_rows(const char* who, bool early, const void* a_codes, const void
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
-  p.top_k = 1;
   p.a_rows = p.M;
   p.wide = store_width(c, ldc, N);
   const int64_t blocks = (N + TM - 1) / TM;
@@ -1832,14 +1826,11 @@ extern "C" int fp8_moe_mxf8(const void* a, int64_t lda, const void* a_codes, con
   p.seg_tab = seg_tab;
   p.wide = store_width(c, ldc, N);
   p.sorted_ids = sorted_token_ids;
-  p.expert_ids = expert_ids;
   p.topk_w = mul_topk_weights ? topk_weights : nullptr;
   p.M = static_cast<int>(n_slots);
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.kchunks = static_cast<int>((K / 32 + 7) / 8 * 2);
-  p.top_k = top_k;
-  p.bs = moe_block_size;
   p.num_blocks = static_cast<int>(num_blocks);
   p.num_experts = static_cast<int>(num_experts);
   p.status = status;

@@ -423,7 +423,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
 }
-// The same for 16 columns.
 // 16 lanes x 32 columns as 8x8 fragments: of lane t, r[4 i + {0, 1}] is TMEM lane
 // t / 4, columns 8 i + 2 (t % 4) + {0, 1}, and r[4 i + {2, 3}] lane t / 4 + 8.
 __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t* r) {
@@ -441,6 +440,7 @@ __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, const uint32_t 
                "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
 }
+// tmem_ld32 for 16 columns.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
