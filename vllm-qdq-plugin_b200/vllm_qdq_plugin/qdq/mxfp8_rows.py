@@ -102,9 +102,10 @@ def _(x, weight, residual, eps, norm_out):
     return [*_new_rows(x, *x.shape), *(x.new_empty(x.shape) for _ in range(more))]
 
 
-def _check(name: str, x: torch.Tensor, k: int) -> None:
+def _check(name: str, x: torch.Tensor, parts: int = 1) -> None:
     assert x.dim() == 2, f"{name} only supports 2D tensors, but got {x.dim()}D"
     assert x.dtype in _DTYPES, f"{name} only supports fp16/bf16 tensors, but got {x.dtype}"
+    k = x.shape[1] // parts
     assert k > 0 and k % 32 == 0, f"{name}: K={k} must be a positive multiple of 32"
     _native.require_cuda(x)
 
@@ -122,7 +123,7 @@ def mxfp8_rows(x: torch.Tensor) -> Mxfp8Rows:
         _native.load_ops(x)
         return Mxfp8Rows(*_rows_op(x), x.dtype)
     except RuntimeError:
-        _check("mxfp8_rows", x, x.shape[-1])
+        _check("mxfp8_rows", x)
         raise
 
 
@@ -138,7 +139,7 @@ def silu_mul_mxfp8(x: torch.Tensor) -> Mxfp8Rows:
         _native.load_ops(x)
         return Mxfp8Rows(*_silu_mul_op(x), x.dtype)
     except RuntimeError:
-        _check("silu_mul_mxfp8", x, x.shape[-1] // 2)
+        _check("silu_mul_mxfp8", x, 2)
         raise
 
 
@@ -165,7 +166,7 @@ def rmsnorm_mxfp8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
         _native.load_ops(x)
         out = _rmsnorm_op(x, weight, residual, eps, norm_out)
     except RuntimeError:
-        _check("rmsnorm_mxfp8", x, x.shape[-1])
+        _check("rmsnorm_mxfp8", x)
         k = x.shape[1]
         assert k <= RMSNORM_MAX_K, f"rmsnorm_mxfp8: K={k} is above {RMSNORM_MAX_K}"
         assert weight.dim() == 1 and weight.shape[0] == k and weight.dtype == x.dtype, (
