@@ -198,3 +198,28 @@ def test_experts_of_extreme_shapes(cuda_device, m, e, n, k):
     for given in (x, rows):
         out = mxfp8_moe_linear(given, w, sid[:live].contiguous(), eid, ntp * 1000, tw, 16, 1, True)
         check_moe(out, a, codes, scales, ids, f"m={m} e={e}", tw)
+
+
+@pytest.mark.parametrize("m,k", [(3, 20480), (1300, 2880), (5, 1024), (7, 512), (2, 65536)])
+def test_rmsnorm_of_far_rows_between_others(cuda_device, m, k):
+    """Every form of the kernel, the sum taken from the residual's: far rows as in 64 bits, the others to the bit as in a
+    call without far ones."""
+    from vllm_qdq_plugin.qdq import mxfp8_quantize, rmsnorm_mxfp8
+    dev = cuda_device
+    gen = torch.Generator(device=dev).manual_seed(k)
+    x, r = (torch.randn(m, k, generator=gen, device=dev).to(torch.bfloat16) for _ in range(2))
+    w = (1 + 0.1 * torch.randn(k, generator=gen, device=dev)).to(torch.bfloat16)
+    near = rmsnorm_mxfp8(x, w, r, 0.0, norm_out=True)
+    far = torch.arange(m, device=dev) % 2 == 1
+    scale = torch.where(torch.arange(m, device=dev) % 4 == 1, 2.0 ** 100, 2.0 ** -90)[:, None]
+    x2, r2 = (torch.where(far[:, None], t.double() * scale, t.double()).to(torch.bfloat16) for t in (x, r))
+    rows, h, y = rmsnorm_mxfp8(x2, w, r2, 0.0, norm_out=True)
+    assert torch.equal(h, (x2.float() + r2.float()).to(torch.bfloat16))
+    assert torch.equal(y[~far], near[2][~far]) and torch.equal(rows.codes[~far], near[0].codes[~far])
+    d = h.double()
+    want = d / d.square().mean(1, keepdim=True).sqrt() * w.double()
+    assert ((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -17) * want.abs() + 2.0 ** -134).all()
+    codes, scales = mxfp8_quantize(y)
+    assert torch.equal(rows.codes, codes) and torch.equal(rows.scales, scales)
+    again = rmsnorm_mxfp8(x2, w, r2, 0.0)[0]
+    assert torch.equal(again.codes, codes) and torch.equal(again.scales, scales)

@@ -182,8 +182,7 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 // 2^128), from its stored h: summed as (h f)^2 with a power of two f, and
 // normalised as (h f) rsqrt(mean (h f)^2 + eps f^2) w.  It reads the row again:
 // scaled in the registers of the kernel below, it cost all rows the order of
-// their loads ([16384, 8192] 138.5 -> 150 us; this way 138.5, [32768, 1024]
-// 37.6 -> 38.8).
+// their loads ([16384, 8192] 138.5 -> 150 us).
 template <bool kWarpRow>
 __device__ __forceinline__ void rmsnorm_far_row(const uint16_t* h, const uint16_t* w, uint16_t* y, uint8_t* codes,
                                              uint8_t* scales, uint32_t upr, float* part, float f, float eps, float zero) {
@@ -217,6 +216,12 @@ __device__ __forceinline__ void rmsnorm_far_row(const uint16_t* h, const uint16_
     if (y != nullptr && col < upr) store_unit<false>(y + col * 16u, unit_of(a8));
     store_mxfp8<QDQ_DTYPE_BF16>(a8, codes, scales, col, col < upr, zero);
   }
+}
+
+template <bool kWarpRow>
+__device__ __noinline__ void rmsnorm_far_row_call(const uint16_t* h, const uint16_t* w, uint16_t* y, uint8_t* codes,
+                                                  uint8_t* scales, uint32_t upr, float* part, float f, float eps, float zero) {
+  rmsnorm_far_row<kWarpRow>(h, w, y, codes, scales, upr, part, f, eps, zero);
 }
 
 // ---------------------------------------------------------------------------
@@ -282,10 +287,17 @@ rmsnorm_mxfp8_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict_
     }
     // The barrier at the loop's end keeps this row's sums until every thread has read them.
     const float ss = row_sum<kWarpRow>(sq.x + sq.y, part);
-    // Out of fp32's range, or so near its lower end that squares are lost and eps does not outweigh them.
+    // Out of fp32's range, or so near its lower end that squares are lost and eps does not outweigh them.  A call of
+    // its own where a thread holds two units, whose registers it would crowd ([32768, 1024] 38.3 us, inlined 40.0, without
+    // the test 38.4; [16384, 8192] 145.8, 146.4, 143.4); inlined elsewhere ([777, 2880] 3.65 us, by a call 4.5).
     if (kDtype == QDQ_DTYPE_BF16 && (!(ss <= 0x1p120f) || (ss < 0x1p-90f && eps < 0x1p-60f))) {
-      rmsnorm_far_row<kWarpRow>(res != nullptr ? h_out + row * ldh : xr, w, y_out != nullptr ? y_out + row * ldy : nullptr,
-                                codes + row * ldc, scales + row * lds, upr, part, ss < 1.0f ? 0x1p90f : 0x1p-80f, eps, zero);
+      const uint16_t* hr = res != nullptr ? h_out + row * ldh : xr;
+      uint16_t* yr = y_out != nullptr ? y_out + row * ldy : nullptr;
+      const float f = ss < 1.0f ? 0x1p90f : 0x1p-80f;
+      if (kC == 2)
+        rmsnorm_far_row_call<kWarpRow>(hr, w, yr, codes + row * ldc, scales + row * lds, upr, part, f, eps, zero);
+      else
+        rmsnorm_far_row<kWarpRow>(hr, w, yr, codes + row * ldc, scales + row * lds, upr, part, f, eps, zero);
       if (!kWarpRow) __syncthreads();
       continue;
     }
