@@ -50,7 +50,7 @@ constexpr int T_EPI = 8;             // epilogue warps
 constexpr int T_SCALE = 4;           // scale warps = quads of stages in the scale ring
 constexpr int T_THREADS = 32 * (2 + T_SCALE + T_EPI);
 constexpr uint32_t T_TMEM = 512, T_SFW = 2 * NT_MAX, T_SFA = T_SFW + 4;
-constexpr uint32_t T_SF_COLS = 12;   // four sets of scale columns in turn: a stage's copies need not wait for the MMAs before it
+constexpr uint32_t T_SF_COLS = 12;   // a set of scale columns for each stage of a quad (one or two sets in turn: the same times)
 
 __host__ __device__ constexpr int t_stage_bytes(int nt) { return T_W + nt * TK; }       // codes
 __host__ __device__ constexpr int t_sf_bytes(int nt) { return nt > 128 ? 1024 : 512; }  // a stage's activation scales
@@ -1225,9 +1225,11 @@ mxf8_few_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_co
 // the same expert, cut into at most nbmax blocks.  One CTA; blocks are walked
 // in chunks of the CTA's size with carries, entries come out in order.
 // ---------------------------------------------------------------------------
-// Threads of the pass's CTAs.  Copying MXFP8 rows, three CTAs of 512 stand on an SM where one of 1024 did (64 tokens,
-// 4 of 128 experts: 281.6 -> 279.4 us a call; 911 tokens, 2 of 4: 9.7 -> 9.1); quantising, 1024 are faster (4096 tokens
-// of K = 4096: 40.7 us, with 512 43.3).
+// Threads of the pass's CTAs.  Copying MXFP8 rows, three CTAs of 512 stand on an SM where one of 1024 did (calls in us,
+// 512 and 1024 threads in turn: 64 tokens, 4 of 128 experts of 5760 x 2880 282.9 and 286.1, 4096 tokens 458 and 464; 911
+// tokens, 2 of 4 of 390 x 224 8.4 and 9.2; 4096, 4 of 32 of 256 x 2880 36.4 and 37.9; one of eight shapes the other way,
+// 2048 tokens, 2 of 8 of 512 x 8192 36.4 and 35.6); quantising, 1024 are faster (4096 tokens of K = 4096: 40.7, with 512
+// 43.3).
 constexpr int SEG_THREADS = 1024;
 __host__ __device__ constexpr int prepare_threads(bool raw) { return raw ? SEG_THREADS : SEG_THREADS / 2; }
 
@@ -1486,19 +1488,21 @@ int run_few(const char* who, const CUtensorMap& tw, const CUtensorMap& ta, FewAr
 // operand bytes at 80 a cycle and its issue (300, pairs 430), plus 80; the
 // launch takes as many stages as the busiest SM has items.  Against the best
 // of five forced choices the rule's was within 6 % on 14 shapes, e.g.
-// [4096 x 4096 -> 14336] pairs of 240 rows 171 us, single CTAs of 192 rows
-// 209; [4096 x 1024 -> 512] single CTAs of 128 rows 8.2 us, pairs 10.2.
+// [4096 x 4096 -> 14336] pairs of 240 rows 181 us, single CTAs of 192 rows 213,
+// and at the clock that a second of such calls settles at 208 and 252; [4096 x
+// 1024 -> 512] single CTAs of 128 rows 8.2 us, pairs 10.2.
 //
 // Grouped: `segments(nt)` estimates the segments at nt rows per item from what
 // the host knows, `rows` the rows of an average one.  Where every expert has one
 // segment (`experts` of them) its weights come from memory, which gives an SM no
 // stage in less than 700 cycles.  Both kernels then take the same time but for
 // starts, tails and idle halves of pairs, and pairs that cost up to 6 % more
-// stages are taken where their own stage is shorter (192 rows an item: 512
-// tokens, 8 experts of 14336 x 4096, 99.8 us, single CTAs 103.5; 4096 tokens, 128
-// experts of 2880 x 2880, 235 and 249) or an SM has 16 items or more (64 tokens,
-// 128 experts of 5760 x 2880: 284 and 293; with 7 items, 16 tokens, 8 experts of
-// 14336 x 4096: 87.8 and 84.3).
+// stages are taken where their own stage is shorter (192 rows an item; pairs and
+// single CTAs at the settled clock: 512 tokens, 8 experts of 14336 x 4096 102.6
+// and 112.8 us; 4096 tokens, 128 experts of 2880 x 2880 248 and 272, of 5760 x
+// 2880 457 and 510) or an SM has 16 items or more (128 experts of 5760 x 2880, 32
+// tokens 219.9 and 226.9, 64 tokens 283 and 296; of 2880 x 2880, 128 tokens 165
+// and 170.4; with 7 items, 16 tokens, 8 experts of 14336 x 4096, 82.6 and 79.3).
 struct TilePlan {
   bool pair;
   int nt;

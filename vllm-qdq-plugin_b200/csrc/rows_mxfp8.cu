@@ -7,9 +7,9 @@
 //
 // followed by MXFP8 of y: per 32 elements e = floor(log2 amax) - 8 and E4M3
 // codes of y / 2^e (mx_quant.cuh, the rule of qdq_mxfp8).  `round` is to the
-// tensors' 16-bit type: y is what the unfused operator would have stored, so
-// that the codes are those of mxfp8_qdq behind it.  All sums and products
-// before it are fp32.
+// tensors' 16-bit type, and all sums and products before it are fp32: the codes
+// are those of mxfp8_qdq behind an operator that rounds this formula once.  (One
+// that also rounds h * rsqrt before w, or silu(g) before u, stores another y.)
 //
 // Layout: codes [M, K] row-major bytes; scales row-major E8M0 bytes, K / 32 a
 // row, rows lds (a multiple of 16) apart, so that the product loads 16 scales

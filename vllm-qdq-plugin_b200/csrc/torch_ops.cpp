@@ -3,7 +3,8 @@
 // They allocate outputs and workspaces on torch's current stream and call the
 // C ABI (include/qdq_b200.h).  These calls sit on the path of single tokens,
 // where the host's time is the call's time, so they are C++ rather than ctypes:
-// on the measured host one norm call takes 8 us instead of 25 (GPU time 2.1).
+// one norm call of a single row takes 10 us on the host, of which the GPU works
+// 2.1, and through ctypes took 25 (a torch addition takes 4.6).
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -5,8 +5,9 @@ operators that end in them.
 `mxfp8_qdq` returns the values that MXFP8 leaves of an activation; these
 return the codes and scales themselves, for `gemm.mxfp8_linear` and
 `gemm.mxfp8_moe_linear` to multiply.  The codes are those of `mxfp8_qdq` (and
-so of the reference, src/vllm_qdq_plugin/qdq/mxfp8.py:73-125) on the 16-bit
-tensor that the unfused operator would have stored.  One HBM pass each
+so of the reference, src/vllm_qdq_plugin/qdq/mxfp8.py:73-125) on a 16-bit
+tensor that holds the operator's formula, rounded once (an unfused operator that
+rounds in between stores another).  One HBM pass each
 (`qdq_mxfp8_rows`, `qdq_rmsnorm_mxfp8`, `qdq_silu_mul_mxfp8` in
 include/qdq_b200.h).
 """
